@@ -34,11 +34,14 @@ typedef int32_t vtq_status;
 
 /* GGML tensor type tags (src/model/gguf.rs:127-139). */
 #define VTQ_F32 0
+#define VTQ_F16 1   /* batched serving operators only (activations, caches, outputs) */
 #define VTQ_Q4_0 2
 #define VTQ_Q5_0 6
 #define VTQ_Q8_0 8
 #define VTQ_Q4_K 12
 #define VTQ_Q6_K 14
+#define VTQ_I8 24   /* batched serving operators only: quantised tokens */
+#define VTQ_BF16 30 /* batched serving operators only (activations, caches, outputs) */
 
 /* vtq_linear flags. */
 #define VTQ_PTR_HOST 1u  /* x and y are host pointers; the call copies x in and y out and returns
@@ -296,6 +299,163 @@ vtq_status vtq_linear_gather_wait(vtq_ctx* ctx, const vtq_weight* w, const float
 vtq_status vtq_linear_list_gather(vtq_ctx* ctx, const vtq_list_item* items, int32_t n,
                                   vtq_gather* g, uint32_t flags, uint32_t wait_signals);
 vtq_status vtq_gather_destroy(vtq_gather* g);
+
+/* ---- Batched serving operators ----
+ * One serving step over many sequences: 8-bit linears over the step's tokens,
+ * the new keys and values into a paged cache with the position rotation on the
+ * way, attention of the new tokens over the cache with a prefix shared by all
+ * sequences read once for all, and the verification of drafted tokens. No
+ * counterpart in the reference, which decodes one sequence; nothing here is
+ * part of its bit-identity contract, and results are deterministic: the same
+ * inputs give the same bits, run after run.
+ *
+ * Device pointers only, in the manner of vtq_linear_device: asynchronous on
+ * `stream`, whose device has to be the current one; nothing is allocated and
+ * nothing is kept, scratch is the caller's (`ws`, 256-byte aligned; calls that
+ * may overlap need one each, captured graphs too). Shapes and pointers are
+ * checked on the host before anything is launched; a failed call's message is
+ * vtq_device_last_error(). Lengths, tables and token ids live on the device:
+ * kernels check them against the sizes given and skip what lies outside,
+ * OR-ing 2 into the optional status word. Strides are in elements; the last
+ * dimension of every tensor is contiguous. */
+/* Message of this thread's last failed call of this section ("" if none). */
+const char* vtq_device_last_error(void);
+
+/* Symmetric 8-bit codes of each token (row of x, F32 / F16 / BF16):
+ *   scale = max |x| / 127,  q = round-half-even(x / scale), 0 where scale is 0.
+ * The quotient is rounded as a real number, not after a division in 32 bits.
+ * A row with an infinity or a NaN gets scale NaN and q 0. */
+vtq_status vtq_quantize_tokens(int32_t x_dtype, const void* x, int64_t ldx, int64_t tokens,
+                               int64_t in_feat, int8_t* q, int64_t ldq, float* scale,
+                               void* stream);
+/* y[t][o] = (sum_i q[t][i] w[o][i]) * (x_scale[t] * w_scale[o]) + bias[o]: the
+ * sum exact in 32-bit integers, the product and sum behind it in 32-bit floats,
+ * one rounding to y's type (F32 / F16 / BF16). x is F32 / F16 / BF16 and
+ * quantised on the way as by vtq_quantize_tokens (x_scale NULL), or VTQ_I8 with
+ * its x_scale. w is [out_feat][ldw] signed bytes, 16-byte aligned, ldw a
+ * multiple of 16; what lies behind in_feat in a row is not used. bias may be
+ * NULL. in_feat <= 131072 (the integer sums cannot overflow below that).
+ * ws: vtq_linear_i8_workspace_bytes; 0 bytes need no ws. */
+typedef struct vtq_linear_i8_args {
+  const void* x;
+  const float* x_scale;
+  const int8_t* w;
+  const float* w_scale;
+  const float* bias;
+  void* y;
+  int64_t ldx, ldw, ldy;
+  int64_t tokens, in_feat, out_feat;
+  int32_t x_dtype, y_dtype;
+  uint32_t* status; /* or NULL; 1 is OR-ed in if a bounded wait ran out */
+} vtq_linear_i8_args;
+size_t vtq_linear_i8_workspace_bytes(int32_t x_dtype, int64_t tokens, int64_t in_feat,
+                                     int64_t out_feat);
+vtq_status vtq_linear_i8(const vtq_linear_i8_args* args, void* ws, size_t ws_bytes, void* stream);
+
+/* A paged key / value cache: `pages` pages of page_size positions, kv_heads
+ * heads of head_dim values (a multiple of 8, at most 256), F16 or BF16, 16-byte
+ * aligned, strides multiples of 8. Position p of sequence s lies in slot
+ * p % page_size of page table[s * table_ld + p / page_size]. */
+typedef struct vtq_paged_kv {
+  void* k;
+  void* v;
+  int64_t k_page, k_slot, k_head; /* strides */
+  int64_t v_page, v_slot, v_head;
+  const int32_t* table; /* [seqs][table_width] page numbers */
+  int64_t table_ld, table_width;
+  int64_t seqs, pages, page_size, kv_heads, head_dim;
+  int32_t dtype;
+} vtq_paged_kv;
+
+/* Appends k and v (F32 / F16 / BF16, [tokens][kv_heads][head_dim]) to the cache:
+ * token t at position pos[t] of sequence seq[t]. seq[t] < 0 marks padding, which
+ * is left alone everywhere. With rope (a [max_pos][rot_dim / 2] table of (cos,
+ * sin) pairs, 8-byte aligned) the first rot_dim values of each key head are
+ * rotated by the token's position on the way: pair i is (2i, 2i + 1), or
+ * (i, i + rot_dim / 2) with VTQ_ROPE_HALF, and becomes
+ * (a cos - b sin, a sin + b cos), in 32 bits, rounded once to the cache's type.
+ * With q (x's type, [tokens][heads][head_dim]) the queries are rotated alike
+ * into q_out, in the cache's type (not over q itself unless the types and
+ * strides are the same). Two tokens of one call at the same sequence and
+ * position: which one stays is not defined. */
+#define VTQ_ROPE_HALF 1u
+typedef struct vtq_append_kv_args {
+  vtq_paged_kv kv;
+  const void* k;
+  const void* v;
+  const void* q; /* or NULL */
+  void* q_out;
+  int64_t k_tok, k_head, v_tok, v_head, q_tok, q_head, qo_tok, qo_head; /* strides */
+  const int32_t* seq;
+  const int32_t* pos;
+  const float* rope; /* or NULL */
+  int64_t rot_dim, max_pos;
+  int64_t tokens, heads;
+  int32_t x_dtype;
+  uint32_t flags;
+  uint32_t* status; /* or NULL */
+} vtq_append_kv_args;
+vtq_status vtq_append_kv(const vtq_append_kv_args* args, void* stream);
+
+/* Attention of each sequence's newest tokens over its cached keys. Sequence s
+ * owns the query rows q_start[s] .. q_start[s + 1] (NULL: row s alone) and
+ * kv_len[s] cached positions, those of its query tokens the last of them: its
+ * query i of n sees the keys 0 .. kv_len[s] - n + i. Positions below shared_len
+ * are read through row 0 of the table for every sequence, once for all of them.
+ * out = softmax(scale q k) v, [tokens][heads][head_dim] in the cache's type; a
+ * query that sees no key gives zeros. Query head h reads kv head
+ * h / (heads / kv_heads). lse (optional, [tokens][heads] F32): the logarithm of
+ * the sum of exp(scale q k), -inf without a key. Rows of q that no sequence
+ * owns, and theirs of out, are left alone; what cached positions at or behind
+ * kv_len hold has no effect, whatever it is.
+ * Keys behind the table's width, and pages that do not exist, count as unseen
+ * and set the status word; row starts that decrease leave no sequence a row.
+ * At most 1024 sequences a call. ws: vtq_attention_paged_workspace_bytes. */
+typedef struct vtq_attention_args {
+  vtq_paged_kv kv;
+  const void* q;
+  void* out;
+  float* lse;
+  int64_t q_tok, q_head, o_tok, o_head, lse_tok; /* strides */
+  const int32_t* q_start;
+  const int32_t* kv_len;
+  int64_t tokens, heads, shared_len;
+  float scale;
+  uint32_t* status; /* or NULL */
+} vtq_attention_args;
+size_t vtq_attention_paged_workspace_bytes(const vtq_attention_args* args);
+vtq_status vtq_attention_paged(const vtq_attention_args* args, void* ws, size_t ws_bytes,
+                               void* stream);
+
+/* Verification of drafted tokens. draft is [seqs][drafts], n_draft (or NULL: all)
+ * how many of them each sequence has; tokens [seqs][drafts + 1] receives the
+ * accepted drafts, the token behind them, then -1; accepted [seqs] their count.
+ * vtq_verify_draft: target [seqs][drafts + 1][vocab] and proposal
+ * [seqs][drafts][vocab] (or NULL: each draft was certain) are probabilities
+ * (F32 / F16 / BF16), u [seqs][drafts + 1] numbers of [0, 1). Draft i is kept
+ * while u_i * proposal(x_i) < target(x_i); the token behind is drawn with
+ * u[drafts] from max(target - proposal, 0) of the first rejected row (from
+ * target where that is 0 everywhere), or from the row behind the last draft:
+ * the lowest v whose cumulated weight exceeds u times their sum. Decisions and
+ * sums are in 64 bits. A draft outside the vocabulary is rejected. Where no
+ * token has any weight the token is -1.
+ * vtq_verify_greedy: target holds logits; draft i is kept while it is the
+ * lowest index of the largest logit of row i, the token behind is the next
+ * row's (proposal and u are not used). */
+typedef struct vtq_verify_args {
+  const int32_t* draft;
+  const int32_t* n_draft;
+  const void* target;
+  const void* proposal;
+  const float* u;
+  int32_t* tokens;
+  int32_t* accepted;
+  int64_t ld_draft, target_seq, target_row, proposal_seq, proposal_row, ld_u, ld_tokens; /* strides */
+  int64_t seqs, drafts, vocab;
+  int32_t dtype;
+} vtq_verify_args;
+vtq_status vtq_verify_draft(const vtq_verify_args* args, void* stream);
+vtq_status vtq_verify_greedy(const vtq_verify_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,683 @@
+// attention_paged.cu -- attention of a batch's newest tokens over a paged key / value cache, with a
+// prefix that all sequences share.
+//
+//   out = softmax(scale q k^T) v, one pass over the keys with the running maximum m and sum l of each
+//   row's softmax:  m' = max(m, max s),  l' = l 2^(m - m') + sum 2^(s - m'),  o' likewise,
+// scores in units of log2. The keys of a sequence are cut where it suits the machine; each part leaves
+// (m, l, o) and attention_join_kernel adds the parts of a row.
+//
+// Work is a list of segments: (sequence, block of 16 query rows, kv head) over the sequence's own keys,
+// then (block of 16 rows of all sequences, kv head) over the shared prefix. A row is one query head of
+// one token: the heads of a kv head and the drafted tokens of a sequence fill the 16 rows of the MMA.
+// The list is cut into equal runs of key tiles, one run a warp, whatever the lengths are: every CTA
+// derives the same cut from the lengths on the device, so the host never needs them.
+#include <algorithm>
+#include <type_traits>
+
+#include "serve.h"
+#include "tc5.cuh"
+#include "vtq_internal.h"
+
+namespace vtq {
+
+vtq_status serve_check_kv(const char* fn, const vtq_paged_kv& kv);
+
+namespace {
+
+constexpr int kRows = 16;      // query rows of a segment: M of the MMA
+constexpr int kMaxSeqs = 1024;
+
+struct AttnParams {
+  vtq_attention_args a;
+  int group;        // query heads of a kv head
+  int tile;         // keys of a tile
+  int parts;        // warps of the whole grid
+  int keys_max;     // positions that the table can hold
+  int prefix;       // min(shared_len, keys_max)
+  float scale_log2;
+  bool q_wide;      // q rows can be read four bytes at a time
+  int* plan;        // the plan arrays below, for the joining kernel
+  float* part;      // slots of kRows (m, l) and o
+  int dim_padded;
+};
+
+// The cut of the work: prefix sums over the sequences (index B: the shared prefix). Tiles before, and
+// segments before, each sequence; its first query row; its length.
+struct Plan {
+  int *tiles, *segs, *q0, *len;  // [B + 2], [B + 2], [B + 1], [B + 1] (len[B]: of the prefix)
+};
+__host__ __device__ inline int plan_ints(int B) { return 4 * (B + 2) + 2; }
+
+__device__ __forceinline__ Plan plan_of(int* base, int B) {
+  return Plan{base + 2, base + 2 + (B + 2), base + 2 + 2 * (B + 2), base + 2 + 3 * (B + 2)};
+}
+
+__device__ __forceinline__ int seq_rows(const Plan& pl, int b) { return pl.q0[b + 1] - pl.q0[b]; }
+
+// Built by all threads of a CTA in its shared memory; base[0] = tiles in all, base[1] = parts in use.
+__device__ void build_plan(const AttnParams& p, int* base) {
+  const int B = (int)p.a.kv.seqs, T = (int)p.a.tokens, H = (int)p.a.kv.kv_heads;
+  const Plan pl = plan_of(base, B);
+  __shared__ int s_longest, s_bad, s_warp_t[32], s_warp_s[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) s_longest = s_bad = 0;
+  __syncthreads();
+  for (int b = tid; b <= B; b += blockDim.x) {
+    pl.q0[b] = p.a.q_start ? min(max(p.a.q_start[b], 0), T) : min(b, T);
+    if (b < B) {
+      const int len = max(p.a.kv_len[b], 0);
+      pl.len[b] = len;
+      atomicMax(&s_longest, len);
+    }
+  }
+  __syncthreads();
+  for (int b = tid; b < B; b += blockDim.x)
+    if (pl.q0[b + 1] < pl.q0[b]) s_bad = 1;
+  if (tid == 0) pl.len[B] = min(s_longest, p.prefix);
+  __syncthreads();
+  if (s_bad) {  // row starts that decrease: no sequence owns a row (the slots are counted for one owner a row)
+    for (int b = tid; b <= B; b += blockDim.x) pl.q0[b] = 0;
+    if (tid == 0 && p.a.status) atomicOr(p.a.status, SERVE_BAD_INDEX);
+    __syncthreads();
+  }
+  // Inclusive sums over runs of consecutive sequences, one run a thread.
+  const int n = B + 1, per = (n + (int)blockDim.x - 1) / (int)blockDim.x, b0 = min(tid * per, n), b1 = min(b0 + per, n);
+  int st = 0, ss = 0;
+  for (int pass = 0; pass < 2; pass++) {
+    for (int b = b0; b < b1; b++) {
+      int rows, keys;
+      if (b < B) {
+        rows = seq_rows(pl, b) * p.group;
+        keys = max(min(pl.len[b], p.keys_max) - p.prefix, 0);
+      } else {
+        rows = T * p.group;
+        keys = s_bad ? 0 : pl.len[B];
+      }
+      const int segs = (rows + kRows - 1) / kRows * H;
+      if (pass) pl.tiles[b] = st, pl.segs[b] = ss;
+      st += segs * ((keys + p.tile - 1) / p.tile);
+      ss += segs;
+    }
+    if (pass == 0) {
+      int it = st, is = ss;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, it, o), y = __shfl_up_sync(0xffffffffu, is, o);
+        if (lane >= o) it += x, is += y;
+      }
+      if (lane == 31) s_warp_t[warp] = it, s_warp_s[warp] = is;
+      __syncthreads();
+      int ot = it - st, os = is - ss;
+      for (int w = 0; w < warp; w++) ot += s_warp_t[w], os += s_warp_s[w];
+      st = ot, ss = os;
+    }
+  }
+  if (b0 < n && b1 == n) pl.tiles[n] = st, pl.segs[n] = ss;
+  __syncthreads();
+  if (tid == 0) {
+    base[0] = pl.tiles[n];
+    base[1] = min(pl.tiles[n], p.parts);
+  }
+  __syncthreads();
+}
+
+// Part w of W covers tiles [first(w), first(w + 1)) of `total`; part_of is its inverse.
+__device__ __forceinline__ int first_tile(int total, int W, int w) { return (int)((int64_t)total * w / W); }
+__device__ __forceinline__ int part_of(int total, int W, int t) { return (int)((((int64_t)t + 1) * W - 1) / total); }
+
+// Where a part stands: sequence, row block, head, tile.
+struct Cursor {
+  int b, mb, g, t, nt;  // nt tiles in a segment of b
+  int mbs;              // row blocks of b
+};
+
+__device__ __forceinline__ int seq_tiles(const AttnParams& p, const Plan& pl, int b, int B, int* mbs) {
+  const int H = (int)p.a.kv.kv_heads;
+  *mbs = (pl.segs[b + 1] - pl.segs[b]) / H;
+  const int segs = *mbs * H;
+  return segs ? (pl.tiles[b + 1] - pl.tiles[b]) / segs : 0;
+}
+
+__device__ Cursor seek(const AttnParams& p, const Plan& pl, int B, int tile) {
+  int lo = 0, hi = B;  // the last index whose tiles begin at or before `tile`
+  while (lo < hi) {
+    const int m = (lo + hi + 1) >> 1;
+    if (pl.tiles[m] <= tile) lo = m;
+    else hi = m - 1;
+  }
+  Cursor c;
+  c.b = lo;
+  c.nt = seq_tiles(p, pl, lo, B, &c.mbs);
+  const int at = tile - pl.tiles[lo], seg = c.nt ? at / c.nt : 0, H = (int)p.a.kv.kv_heads;
+  c.t = at - seg * c.nt;
+  c.mb = seg / H;
+  c.g = seg - c.mb * H;
+  return c;
+}
+
+// The next tile; true where it begins another segment. Never called behind the last tile.
+__device__ __forceinline__ bool advance(const AttnParams& p, const Plan& pl, int B, Cursor& c) {
+  if (++c.t < c.nt) return false;
+  c.t = 0;
+  if (++c.g == (int)p.a.kv.kv_heads) {
+    c.g = 0;
+    if (++c.mb == c.mbs) {
+      c.mb = 0;
+      do {
+        c.b++;
+        c.nt = c.b <= B ? seq_tiles(p, pl, c.b, B, &c.mbs) : 1;
+      } while (c.b <= B && c.nt == 0);
+    }
+  }
+  return true;
+}
+
+// The sequence that owns a row of q, or -1.
+__device__ __forceinline__ int owner(const Plan& pl, int B, int token) {
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int m = (lo + hi + 1) >> 1;
+    if (pl.q0[m] <= token) lo = m;
+    else hi = m - 1;
+  }
+  return token >= pl.q0[lo] && token < pl.q0[lo + 1] ? lo : -1;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  const int n = there ? 16 : 0;  // 0: the 16 bytes are filled with zeros, nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+// Whether either half of a word is an infinity or a NaN.
+template <typename T>
+__device__ __forceinline__ bool odd_word(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (w & e) == e || ((w >> 16) & e) == e;
+}
+
+// DP: head_dim rounded up to what the MMA loop takes (64, 96, 128, 256). KT keys a tile, a warp's
+// pipeline STAGES tiles of K and V deep; no barrier but the warp's own.
+template <typename T, int DP, int KT, int WARPS, int STAGES>
+__global__ void __launch_bounds__(32 * WARPS, 1) attention_part_kernel(const __grid_constant__ AttnParams p) {
+  constexpr int CH = DP / 8;                         // 16-byte chunks of a row
+  constexpr uint32_t kTileBytes = KT * DP * 2, kStage = 2 * kTileBytes;
+  extern __shared__ __align__(128) uint8_t smem[];
+  tc5::grid_release();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int B = (int)p.a.kv.seqs, H = (int)p.a.kv.kv_heads, D = (int)p.a.kv.head_dim;
+  int* base = reinterpret_cast<int*>(smem + WARPS * STAGES * kStage);
+  longlong2* rows = reinterpret_cast<longlong2*>(smem + WARPS * STAGES * kStage + (plan_ints(B) * 4 + 15) / 16 * 16) + warp * KT;
+  __shared__ uint32_t s_valid[WARPS][STAGES];
+  build_plan(p, base);
+  const Plan pl = plan_of(base, B);
+  const int total = base[0], W = base[1];
+  if (blockIdx.x == 0) {
+    for (int i = tid; i < plan_ints(B); i += blockDim.x) p.plan[i] = base[i];
+    int* own = p.plan + plan_ints(B);
+    for (int t = tid; t < (int)p.a.tokens; t += blockDim.x) own[t] = owner(pl, B, t);
+    if (p.a.status)
+      for (int b = tid; b < B; b += blockDim.x)
+        if (pl.len[b] > p.keys_max || p.a.kv_len[b] < 0) atomicOr(p.a.status, SERVE_BAD_INDEX);
+  }
+  const int w = warp * (int)gridDim.x + (int)blockIdx.x;  // few parts spread over the SMs first
+  if (w >= W) return;
+  const int tile0 = first_tile(total, W, w), tile1 = first_tile(total, W, w + 1);
+  const uint32_t stage0 = smem_u32(smem) + warp * STAGES * kStage;
+  auto swizzled = [](int key, int chunk) {
+    const int x = DP == 96 ? (key >> 1) & 3 : key & 7;  // eight rows' chunks in eight different bank groups
+    return (uint32_t)(key * DP * 2 + ((chunk ^ x) << 4));
+  };
+  const T* K = static_cast<const T*>(p.a.kv.k);
+  const T* V = static_cast<const T*>(p.a.kv.v);
+
+  // Starts tile `c` into stage s.
+  auto load = [&](const Cursor& c, int s) {
+    const bool shared = c.b == B;
+    const int key0 = (shared ? 0 : p.prefix) + c.t * KT;
+    const int end = shared ? pl.len[B] : min(pl.len[c.b], p.keys_max);
+    bool ok = false;
+    if (lane < KT) {
+      const int pos = key0 + lane;
+      int64_t ko = 0, vo = 0;
+      if (pos < end) {
+        const int page_size = (int)p.a.kv.page_size, at = pos / page_size;
+        const int64_t page = p.a.kv.table[(shared ? 0 : c.b) * p.a.kv.table_ld + at], slot = pos - at * page_size;
+        ok = page >= 0 && page < p.a.kv.pages;
+        if (ok) {
+          ko = page * p.a.kv.k_page + slot * p.a.kv.k_slot + c.g * p.a.kv.k_head;
+          vo = page * p.a.kv.v_page + slot * p.a.kv.v_slot + c.g * p.a.kv.v_head;
+        } else if (p.a.status) {
+          atomicOr(p.a.status, SERVE_BAD_INDEX);
+        }
+      }
+      rows[lane] = make_longlong2(ko, vo);
+    }
+    const uint32_t valid = __ballot_sync(0xffffffffu, ok);
+    if (lane == 0) s_valid[warp][s] = valid;
+    __syncwarp();
+    const uint32_t k_s = stage0 + s * kStage, v_s = k_s + kTileBytes;
+#pragma unroll
+    for (int i = 0; i < KT * CH / 32; i++) {
+      const int e = i * 32 + lane, key = e / CH, chunk = e - key * CH;
+      const longlong2 o = rows[key];
+      const bool there = ((valid >> key) & 1) && chunk * 8 < D;
+      copy16(k_s + swizzled(key, chunk), K + (there ? o.x + chunk * 8 : 0), there);
+      copy16(v_s + swizzled(key, chunk), V + (there ? o.y + chunk * 8 : 0), there);
+    }
+    __syncwarp();
+  };
+
+  Cursor in = seek(p, pl, B, tile0), c = in;
+  int next = tile0;
+  for (int s = 0; s < STAGES - 1; s++) {
+    if (next < tile1) {
+      load(in, s);
+      if (++next < tile1) advance(p, pl, B, in);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+
+  uint32_t qf[DP / 16][4];
+  float o[DP / 8][4];
+  float m0 = 0, m1 = 0, l0 = 0, l1 = 0;
+  int lim0 = 0, lim1 = 0, lim_min = 0, rows_in = 0;
+  bool begin = true;
+  const int r0 = lane >> 2, cq = 2 * (lane & 3);
+  for (int tile = tile0; tile < tile1; tile++) {
+    if (begin) {
+      // A new segment: its 16 query rows, and how far each of them sees.
+      const bool shared = c.b == B;
+      const int n = shared ? (int)p.a.tokens : seq_rows(pl, c.b), q0 = shared ? 0 : pl.q0[c.b];
+      rows_in = min(kRows, n * p.group - c.mb * kRows);
+      const T* qr[2];
+      int lim[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int r = r0 + 8 * h, row = c.mb * kRows + r, tok = row / p.group;
+        qr[h] = nullptr;
+        lim[h] = 0;
+        if (r < rows_in) {
+          qr[h] = static_cast<const T*>(p.a.q) + (int64_t)(q0 + tok) * p.a.q_tok + (int64_t)(c.g * p.group + row - tok * p.group) * p.a.q_head;
+          const int b = shared ? owner(pl, B, tok) : c.b;
+          if (b >= 0) {
+            const int i = q0 + tok - pl.q0[b];
+            lim[h] = min(pl.len[b] - seq_rows(pl, b) + i + 1, p.keys_max);
+          }
+        }
+      }
+      lim0 = lim[0], lim1 = lim[1];
+      lim_min = __reduce_min_sync(0xffffffffu, min(qr[0] ? lim0 : INT32_MAX, qr[1] ? lim1 : INT32_MAX));
+#pragma unroll
+      for (int k = 0; k < DP / 16; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const T* src = qr[e & 1];
+          const int d = 16 * k + 8 * (e >> 1) + cq;
+          uint32_t v = 0;
+          if (src && d < D) {
+            if (p.q_wide) {
+              v = *reinterpret_cast<const uint32_t*>(src + d);
+            } else {
+              const uint16_t* h = reinterpret_cast<const uint16_t*>(src + d);
+              v = (uint32_t)h[0] | (uint32_t)h[1] << 16;
+            }
+          }
+          qf[k][e] = v;
+        }
+#pragma unroll
+      for (int i = 0; i < DP / 8; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[i][e] = 0.0f;
+      m0 = m1 = -INFINITY;
+      l0 = l1 = 0.0f;
+    }
+    const int s = (tile - tile0) % STAGES;
+    if (next < tile1) {
+      load(in, (s + STAGES - 1) % STAGES);
+      if (++next < tile1) advance(p, pl, B, in);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    __syncwarp();
+    const uint32_t k_s = stage0 + s * kStage, v_s = k_s + kTileBytes;
+    const uint32_t valid = s_valid[warp][s];
+    const int key0 = (c.b == B ? 0 : p.prefix) + c.t * KT;
+    float sc[KT / 8][4];
+#pragma unroll
+    for (int i = 0; i < KT / 8; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) sc[i][e] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < DP / 16; k++)
+#pragma unroll
+      for (int n = 0; n < KT / 16; n++) {
+        uint32_t kf[4];
+        const int key = 16 * n + (lane & 7) + ((lane >> 4) << 3), chunk = 2 * k + ((lane >> 3) & 1);
+        ldsm4(k_s + swizzled(key, chunk), kf);
+        mma16<T>(sc[2 * n], qf[k], kf[0], kf[1]);
+        mma16<T>(sc[2 * n + 1], qf[k], kf[2], kf[3]);
+      }
+    const bool whole = valid == (KT == 32 ? 0xffffffffu : (1u << (KT & 31)) - 1u) && key0 + KT <= lim_min;
+    float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < KT / 8; n++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int j = 8 * n + cq + e;
+        sc[n][e] *= p.scale_log2;
+        sc[n][2 + e] *= p.scale_log2;
+        if (!whole) {
+          const bool there = (valid >> j) & 1;
+          if (!there || key0 + j >= lim0) sc[n][e] = -INFINITY;
+          if (!there || key0 + j >= lim1) sc[n][2 + e] = -INFINITY;
+        }
+        x0 = fmaxf(x0, sc[n][e]);
+        x1 = fmaxf(x1, sc[n][2 + e]);
+      }
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1) {
+      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+    }
+    const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+    const float u0 = n0 == -INFINITY ? 0.0f : n0, u1 = n1 == -INFINITY ? 0.0f : n1;
+    if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
+      const float f0 = exp2_fast(m0 - u0), f1 = exp2_fast(m1 - u1);
+      l0 *= f0, l1 *= f1;
+#pragma unroll
+      for (int i = 0; i < DP / 8; i++) o[i][0] *= f0, o[i][1] *= f0, o[i][2] *= f1, o[i][3] *= f1;
+    }
+    m0 = n0, m1 = n1;
+    uint32_t pf[KT / 16][4];
+#pragma unroll
+    for (int n = 0; n < KT / 8; n++) {
+      float e0 = exp2_fast(sc[n][0] - u0), e1 = exp2_fast(sc[n][1] - u0);
+      float e2 = exp2_fast(sc[n][2] - u1), e3 = exp2_fast(sc[n][3] - u1);
+      l0 += e0 + e1;
+      l1 += e2 + e3;
+      // The weights are rounded to the cache's type for the second product: relative to each
+      // weight, so a row's error stays that of its type, as the rounding of v itself.
+      pf[n >> 1][2 * (n & 1)] = pack2<T>(e0, e1);
+      pf[n >> 1][2 * (n & 1) + 1] = pack2<T>(e2, e3);
+    }
+    if (!whole) {
+      // A weight of 0 times an infinity or a NaN is no 0: values that some rows must not see are taken
+      // out of the tile, and added to those that do see them.
+      bool odd = false;
+#pragma unroll 1
+      for (int i = lane; i < KT * CH; i += 32) {
+        const uint4 v = *reinterpret_cast<const uint4*>(smem + (v_s - smem_u32(smem)) + i * 16);
+        odd |= odd_word<T>(v.x) || odd_word<T>(v.y) || odd_word<T>(v.z) || odd_word<T>(v.w);
+      }
+      if (__any_sync(0xffffffffu, odd)) {
+        T* vt = reinterpret_cast<T*>(smem + (v_s - smem_u32(smem)));
+#pragma unroll
+        for (int i = 0; i < DP / 8; i++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int d = 8 * i + cq + e;
+#pragma unroll 1
+            for (int key = 0; key < KT; key++) {
+              const float v = to_f32(vt[swizzled(key, d >> 3) / 2 + (d & 7)]);
+              if (fabsf(v) <= 3.4028235e38f) continue;
+              if (key0 + key < lim0) o[i][e] += v;
+              if (key0 + key < lim1) o[i][2 + e] += v;
+            }
+          }
+        __syncwarp();
+#pragma unroll 1
+        for (int i = lane; i < KT * DP; i += 32)
+          if (!(fabsf(to_f32(vt[i])) <= 3.4028235e38f)) vt[i] = from_f32<T>(0.0f);
+        __syncwarp();
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < KT / 16; k++)
+#pragma unroll
+      for (int i = 0; i < DP / 16; i++) {
+        uint32_t vf[4];
+        const int key = 16 * k + (lane & 15), chunk = 2 * i + (lane >> 4);
+        ldsm4_t(v_s + swizzled(key, chunk), vf);
+        mma16<T>(o[2 * i], pf[k], vf[0], vf[1]);
+        mma16<T>(o[2 * i + 1], pf[k], vf[2], vf[3]);
+      }
+    __syncwarp();
+    const Cursor seg = c;
+    begin = tile + 1 < tile1 ? advance(p, pl, B, c) : true;
+    if (begin) {
+      // The part's share of the segment ends here.
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+      }
+      float* slot = p.part + (int64_t)(w + pl.segs[seg.b] + seg.mb * H + seg.g) * (kRows * (DP + 2));
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int r = r0 + 8 * h;
+        if (r >= rows_in) continue;
+        if ((lane & 3) == 0) {
+          slot[2 * r] = h ? m1 : m0;
+          slot[2 * r + 1] = h ? l1 : l0;
+        }
+        float* dst = slot + 2 * kRows + r * DP + cq;
+#pragma unroll
+        for (int i = 0; i < DP / 8; i++)
+          *reinterpret_cast<float2*>(dst + 8 * i) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+      }
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Adds the parts of each row (query head of a token): one warp a row.
+template <typename T, int DP>
+__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttnParams p) {
+  tc5::grid_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int heads = (int)p.a.heads, H = (int)p.a.kv.kv_heads, B = (int)p.a.kv.seqs, D = (int)p.a.kv.head_dim;
+  if (row >= p.a.tokens * heads) return;
+  const int token = (int)(row / heads), head = (int)(row - (int64_t)token * heads), g = head / p.group;
+  const Plan pl = plan_of(p.plan, B);
+  const int b = p.plan[plan_ints(B) + token];
+  if (b < 0) return;  // no sequence owns the row
+  const int total = p.plan[0], W = p.plan[1];
+  // The row's place among the sequence's own rows, and among all rows for the prefix.
+  int w0[2], count[2], slot0[2], rr[2];
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const int s = k ? B : b, r = (k ? token : token - pl.q0[b]) * p.group + head - g * p.group, mb = r / kRows;
+    int mbs;
+    const int nt = seq_tiles(p, pl, s, B, &mbs);
+    rr[k] = r - mb * kRows;
+    const int t0 = pl.tiles[s] + (mb * H + g) * nt;
+    w0[k] = nt ? part_of(total, W, t0) : 0;
+    count[k] = nt ? part_of(total, W, t0 + nt - 1) - w0[k] + 1 : 0;
+    slot0[k] = w0[k] + pl.segs[s] + mb * H + g;
+  }
+  const int parts = count[0] + count[1];
+  constexpr int64_t kSlot = kRows * (DP + 2);
+  auto at = [&](int i, int& r) {
+    const int k = i >= count[0];
+    r = rr[k];
+    return p.part + (int64_t)(slot0[k] + i - (k ? count[0] : 0)) * kSlot;
+  };
+  float m = -INFINITY;
+  for (int i = lane; i < parts; i += 32) {
+    int r;
+    const float* s = at(i, r);
+    m = fmaxf(m, s[2 * r]);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  const float um = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, acc[DP / 32];
+#pragma unroll
+  for (int e = 0; e < DP / 32; e++) acc[e] = 0.0f;
+  for (int i0 = 0; i0 < parts; i0 += 32) {
+    float f = 0.0f;
+    if (i0 + lane < parts) {
+      int r;
+      const float* s = at(i0 + lane, r);
+      f = exp2_fast(s[2 * r] - um);
+      l += f * s[2 * r + 1];
+    }
+    const int n = min(32, parts - i0);
+#pragma unroll 4
+    for (int i = 0; i < n; i++) {
+      int r;
+      const float* s = at(i0 + i, r) + 2 * kRows + r * DP;
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+#pragma unroll
+      for (int e = 0; e < DP / 32; e++) acc[e] = fmaf(fi, s[lane + 32 * e], acc[e]);
+    }
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+  T* out = static_cast<T*>(p.a.out) + token * p.a.o_tok + head * p.a.o_head;
+#pragma unroll
+  for (int e = 0; e < DP / 32; e++)
+    if (lane + 32 * e < D) out[lane + 32 * e] = from_f32<T>(acc[e] * inv);
+  if (p.a.lse && lane == 0)
+    p.a.lse[token * p.a.lse_tok + head] = l == 0.0f ? -INFINITY : (um + log2f(l)) * 0.69314718055994531f;
+}
+
+int padded_dim(int64_t d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : 256; }
+int part_warps(int dp) { return dp == 256 ? 4 : 8; }
+
+size_t plan_bytes(const vtq_attention_args& a) {
+  return ((size_t)(plan_ints((int)a.kv.seqs) + a.tokens) * 4 + 255) / 256 * 256;
+}
+// Segments of any lengths: each sequence's rows and, once more, all rows for the prefix.
+int64_t most_segments(const vtq_attention_args& a) {
+  const int64_t group = a.heads / a.kv.kv_heads, rows = a.tokens * group;
+  return (rows / kRows + a.kv.seqs + (a.shared_len ? (rows + kRows - 1) / kRows : 0)) * a.kv.kv_heads;
+}
+
+vtq_status check(const char* fn, const vtq_attention_args* a) {
+  if (!a) return serve_fail(VTQ_ERR_INVALID_ARG, "%s: null arguments", fn);
+  if (vtq_status s = serve_check_kv(fn, a->kv)) return s;
+  if (a->tokens < 0 || a->heads < 1 || a->heads % a->kv.kv_heads || a->shared_len < 0)
+    return serve_fail(VTQ_ERR_INTERNAL, "%s: bad shape (heads not a multiple of kv_heads, or a negative size)", fn);
+  if (a->kv.seqs > kMaxSeqs)
+    return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "%s: not implemented (over %d sequences in one call)", fn, kMaxSeqs);
+  if (a->tokens > (1 << 20) || a->heads > 65536 || a->kv.table_width * a->kv.page_size > INT32_MAX / 2)
+    return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "%s: not implemented (over 2^20 tokens, 2^16 heads or 2^30 positions)", fn);
+  const int64_t tiles = (a->kv.table_width * a->kv.page_size + 15) / 16 + 1;
+  if (most_segments(*a) * tiles > INT32_MAX)
+    return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "%s: not implemented (query rows times table positions over 2^35)", fn);
+  return VTQ_OK;
+}
+
+template <typename T, int DP, int KT, int WARPS, int STAGES>
+cudaError_t launch(const AttnParams& p, cudaStream_t st) {
+  auto part = attention_part_kernel<T, DP, KT, WARPS, STAGES>;
+  const size_t smem = (size_t)WARPS * STAGES * 2 * KT * DP * 2 + (plan_ints((int)p.a.kv.seqs) * 4 + 15) / 16 * 16 +
+                      (size_t)WARPS * KT * sizeof(longlong2);
+  cudaError_t e = cudaFuncSetAttribute(part, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  kernel_launch_count() += 2;
+  part<<<(unsigned)(p.parts / WARPS), 32 * WARPS, smem, st>>>(p);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.a.tokens * p.a.heads + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, attention_join_kernel<T, DP>, p);
+}
+
+template <typename T>
+cudaError_t launch_dim(AttnParams& p, cudaStream_t st) {
+  switch (p.dim_padded) {
+    case 64: return launch<T, 64, 32, 8, 3>(p, st);
+    case 96: return launch<T, 96, 16, 8, 3>(p, st);
+    case 128: return launch<T, 128, 16, 8, 3>(p, st);
+    default: return launch<T, 256, 16, 4, 3>(p, st);
+  }
+}
+
+}  // namespace
+}  // namespace vtq
+
+using namespace vtq;
+
+extern "C" {
+
+size_t vtq_attention_paged_workspace_bytes(const vtq_attention_args* a) {
+  if (check("vtq_attention_paged", a) || a->tokens == 0 || a->kv.seqs == 0) return 0;
+  const int dp = padded_dim(a->kv.head_dim);
+  const int64_t slots = most_segments(*a) + (int64_t)num_sms() * part_warps(dp);
+  return plan_bytes(*a) + (size_t)slots * kRows * (dp + 2) * 4;
+}
+
+vtq_status vtq_attention_paged(const vtq_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
+  const char* fn = "vtq_attention_paged";
+  if (vtq_status s = check(fn, a)) return s;
+  if (a->tokens == 0 || a->kv.seqs == 0) return VTQ_OK;
+  if (!a->q || !a->out || !a->kv_len) return serve_fail(VTQ_ERR_INVALID_ARG, "%s: null pointer", fn);
+  const size_t need = vtq_attention_paged_workspace_bytes(a);
+  if (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255u))
+    return serve_fail(VTQ_ERR_INVALID_ARG, "%s: workspace missing, too small or not 256-byte aligned", fn);
+  AttnParams p;
+  p.a = *a;
+  p.group = (int)(a->heads / a->kv.kv_heads);
+  p.dim_padded = padded_dim(a->kv.head_dim);
+  p.tile = p.dim_padded == 64 ? 32 : 16;
+  p.parts = num_sms() * part_warps(p.dim_padded);
+  p.keys_max = (int)(a->kv.table_width * a->kv.page_size);
+  p.prefix = (int)std::min<int64_t>(a->shared_len, p.keys_max);
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.q_wide = (reinterpret_cast<uintptr_t>(a->q) & 3u) == 0 && a->q_tok % 2 == 0 && a->q_head % 2 == 0;
+  p.plan = static_cast<int*>(ws);
+  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan_bytes(*a));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return serve_cuda(a->kv.dtype == VTQ_F16 ? launch_dim<__half>(p, st) : launch_dim<__nv_bfloat16>(p, st), fn);
+}
+
+}  // extern "C"

@@ -43,6 +43,7 @@
 #include <vector>
 #include <unordered_map>
 
+#include "tc5.cuh"
 #include "vtq_device.cuh"
 #include "vtq_internal.h"
 
@@ -542,8 +543,10 @@ EncodeFn encoder() {
   return fn;
 }
 
+}  // namespace
+
 // 2D byte tensor map [rows][cols] with row stride `pitch`.
-cudaError_t byte_map(CUtensorMap* tm, const void* ptr, int64_t rows, int64_t cols, int64_t pitch,
+cudaError_t tma_byte_map(CUtensorMap* tm, const void* ptr, int64_t rows, int64_t cols, int64_t pitch,
                      uint32_t box_x, uint32_t box_y, CUtensorMapSwizzle sw) {
   EncodeFn enc = encoder();
   if (!enc) return cudaErrorInvalidValue;
@@ -557,6 +560,8 @@ cudaError_t byte_map(CUtensorMap* tm, const void* ptr, int64_t rows, int64_t col
              ? cudaSuccess
              : cudaErrorInvalidValue;
 }
+
+namespace {
 
 // Scratch for the quantised activations, one buffer per (device, stream): GEMMs
 // on different streams never share it, and work on one stream is ordered. A
@@ -656,8 +661,8 @@ cudaError_t launch_kq_gemm(const DevMatrix& m, const float* x, int64_t ldx, int6
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
   CUtensorMap tmx, tmw;
-  if ((e = byte_map(&tmx, xq, M, n, n, 128, GM, CU_TENSOR_MAP_SWIZZLE_128B)) != cudaSuccess) return e;
-  if ((e = byte_map(&tmw, m.data, R, m.pitch, m.pitch, 144, GR, CU_TENSOR_MAP_SWIZZLE_NONE)) !=
+  if ((e = tma_byte_map(&tmx, xq, M, n, n, 128, GM, CU_TENSOR_MAP_SWIZZLE_128B)) != cudaSuccess) return e;
+  if ((e = tma_byte_map(&tmw, m.data, R, m.pitch, m.pitch, 144, GR, CU_TENSOR_MAP_SWIZZLE_NONE)) !=
       cudaSuccess)
     return e;
   const int tiles_m = (M + GM - 1) / GM, ntiles = tiles_m * ((R + GR - 1) / GR);

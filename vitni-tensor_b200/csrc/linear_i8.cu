@@ -1,0 +1,416 @@
+// linear_i8.cu -- 8-bit linears over a batch of tokens: codes and a scale for each token, signed
+// 8-bit weights with a scale for each output channel.
+//
+//   y[t][o] = (sum_i q[t][i] w[o][i]) * (x_scale[t] w_scale[o]) + bias[o]
+//
+// The sum is a contraction of signed bytes on the tensor cores (tcgen05.mma kind::i8, 32-bit
+// accumulators in TMEM): exact, so the split over K and the order of the parts do not show.
+//
+// The weights are the MMA's rows (M = 128 output channels) and the tokens its columns (N = 16 .. 256):
+// a few tokens then waste columns that cost nothing to load, and a lane of TMEM is one output channel,
+// so that a warp's store of one column is 32 neighbouring channels of one token.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "serve.h"
+#include "tc5.cuh"
+#include "vtq_internal.h"
+
+namespace cg = cooperative_groups;
+
+namespace vtq {
+namespace {
+
+// ---- codes and scales of the tokens ----
+
+constexpr int kQThreads = 512, kQKeep = 4;  // values kept in registers: 4 x 8 a thread
+
+// Round-half-even of the real quotient x / s. The product with 1 / s is at most one off; the
+// remainder x - q s is exact in 32 bits (both are multiples of a common power of two and it is
+// no larger than s), so comparing it with s / 2 decides.
+__device__ __forceinline__ int code(float x, float s, float inv) {
+  float q = rintf(x * inv);
+  const float rem = fmaf(-q, s, x), h = 0.5f * s;
+  const bool odd = ((int)q) & 1;
+  if (rem > h || (rem == h && odd)) q += 1.0f;
+  else if (rem < -h || (rem == -h && odd)) q -= 1.0f;
+  return max(-127, min(127, (int)q));
+}
+
+template <typename X>
+__device__ __forceinline__ void load8(const X* row, int64_t i, int64_t n, bool wide, float (&v)[8]) {
+  if (wide && i + 8 <= n) {
+    if constexpr (sizeof(X) == 2) {
+      const uint4 w = *reinterpret_cast<const uint4*>(row + i);
+      const X* e = reinterpret_cast<const X*>(&w);
+#pragma unroll
+      for (int k = 0; k < 8; k++) v[k] = to_f32(e[k]);
+    } else {
+      const float4 a = *reinterpret_cast<const float4*>(row + i), b = *reinterpret_cast<const float4*>(row + i + 4);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = i + k < n ? to_f32(row[i + k]) : 0.0f;
+  }
+}
+
+// One CTA a token. Values of up to 16384 inputs stay in registers between the two passes.
+template <typename X>
+__global__ void __launch_bounds__(kQThreads)
+    quantize_kernel(const X* __restrict__ x, int64_t ldx, int64_t n, bool wide, int8_t* __restrict__ q,
+                    int64_t ldq, bool wide_q, float* __restrict__ scale) {
+  __shared__ uint32_t s_max[kQThreads / 32];
+  tc5::grid_release();
+  const X* row = x + (int64_t)blockIdx.x * ldx;
+  int8_t* out = q + (int64_t)blockIdx.x * ldq;
+  const int64_t step = (int64_t)blockDim.x * 8, i0 = (int64_t)threadIdx.x * 8;
+  float keep[kQKeep][8];
+  uint32_t m = 0;  // |x| as bits: ordered as the values, infinities and NaN above all
+#pragma unroll
+  for (int k = 0; k < kQKeep; k++) {
+    if (i0 + k * step < n) {
+      load8(row, i0 + k * step, n, wide, keep[k]);
+#pragma unroll
+      for (int e = 0; e < 8; e++) m = max(m, __float_as_uint(keep[k][e]) & 0x7fffffffu);
+    }
+  }
+  for (int64_t i = i0 + kQKeep * step; i < n; i += step) {
+    float v[8];
+    load8(row, i, n, wide, v);
+#pragma unroll
+    for (int e = 0; e < 8; e++) m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = 0;
+  for (int w = 0; w < (int)(blockDim.x >> 5); w++) m = max(m, s_max[w]);
+  const bool finite = m < 0x7f800000u;
+  float s = finite ? __fdiv_rn(__uint_as_float(m), 127.0f) : __uint_as_float(0x7fc00000u);
+  if (threadIdx.x == 0) scale[blockIdx.x] = s;
+  const bool some = finite && s > 0.0f;
+  const float up = s < 1e-30f ? 18446744073709551616.0f : 1.0f;  // keeps 1 / s finite; exact on both
+  s = s * up;
+  const float inv = some ? __fdiv_rn(1.0f, s) : 0.0f;
+  auto put = [&](int64_t i, const float (&v)[8]) {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const int c = some ? code(v[e] * up, s, inv) : 0;
+      w[e >> 2] |= (uint32_t)(c & 0xff) << (8 * (e & 3));
+    }
+    if (wide_q && i + 8 <= n) {
+      *reinterpret_cast<uint2*>(out + i) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (i + e < n) out[i + e] = (int8_t)(w[e >> 2] >> (8 * (e & 3)));
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < kQKeep; k++)
+    if (i0 + k * step < n) put(i0 + k * step, keep[k]);
+  for (int64_t i = i0 + kQKeep * step; i < n; i += step) {
+    float v[8];
+    load8(row, i, n, wide, v);
+    put(i, v);
+  }
+}
+
+template <typename X>
+cudaError_t launch_quantize(const X* x, int64_t ldx, int64_t tokens, int64_t n, int8_t* q, int64_t ldq,
+                            float* scale, cudaStream_t st) {
+  const bool wide = aligned16(x) && ldx % (16 / (int)sizeof(X)) == 0;
+  const bool wide_q = (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && ldq % 8 == 0;
+  const int threads = (int)std::min<int64_t>(kQThreads, std::max<int64_t>(32, ((n + 7) / 8 + 31) / 32 * 32));
+  kernel_launch_count()++;
+  quantize_kernel<X><<<(unsigned)tokens, threads, 0, st>>>(x, ldx, n, wide, q, ldq, wide_q, scale);
+  return cudaGetLastError();
+}
+
+cudaError_t quantize(int dtype, const void* x, int64_t ldx, int64_t tokens, int64_t n, int8_t* q, int64_t ldq,
+                     float* scale, cudaStream_t st) {
+  if (dtype == VTQ_F32) return launch_quantize(static_cast<const float*>(x), ldx, tokens, n, q, ldq, scale, st);
+  if (dtype == VTQ_F16) return launch_quantize(static_cast<const __half*>(x), ldx, tokens, n, q, ldq, scale, st);
+  return launch_quantize(static_cast<const __nv_bfloat16*>(x), ldx, tokens, n, q, ldq, scale, st);
+}
+
+// ---- the product ----
+
+struct I8Params {
+  int T, K, N;
+  int kblocks;  // of 128 inputs
+  const float* xs;
+  const float* ws;
+  const float* bias;
+  void* y;
+  int64_t ldy;
+  unsigned* status;
+};
+
+constexpr int BM = 128;          // output channels a tile
+constexpr uint32_t A_STAGE = BM * 128;
+constexpr int kThreads = 192;    // producer warp, MMA warp, 4 epilogue warps
+
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+
+template <typename Y>
+__device__ __forceinline__ void store_y(const I8Params& p, int t, int o, int acc, float wsc, float b) {
+  float v = __int2float_rn(acc) * (p.xs[t] * wsc);
+  if (p.bias) v += b;
+  static_cast<Y*>(p.y)[(int64_t)t * p.ldy + o] = from_f32<Y>(v);
+}
+
+// One tile of 128 channels x NT tokens; the CTAs of a cluster share its K and add their integer parts
+// through each other's shared memory.
+template <int NT, int STAGES, typename Y>
+__global__ void __launch_bounds__(kThreads)
+    i8_tile_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx,
+                   const __grid_constant__ I8Params p) {
+  constexpr uint32_t B_STAGE = NT * 128, STAGE = A_STAGE + B_STAGE;
+  constexpr uint32_t COLS = NT < 32 ? 32 : NT;
+  constexpr uint32_t kIdesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+  static_assert(STAGES * STAGE >= BM * NT * 4, "the parts reuse the stages");
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t s_bar[2 * STAGES + 1];
+  __shared__ uint32_t s_slot;
+  __shared__ int s_abort;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  int* part = reinterpret_cast<int*>(smem_raw + (base - smem_u32(smem_raw)));
+  auto FULL = [&](int i) { return smem_u32(&s_bar[i]); };
+  auto EMPTY = [&](int i) { return smem_u32(&s_bar[STAGES + i]); };
+  const uint32_t DONE = smem_u32(&s_bar[2 * STAGES]);
+  cg::cluster_group cl = cg::this_cluster();
+  const int rank = (int)cl.block_rank(), splits = (int)cl.num_blocks();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int o0 = (int)(blockIdx.x / splits) * BM, t0 = (int)blockIdx.y * NT;
+  const int kb0 = (int)((int64_t)p.kblocks * rank / splits), kb1 = (int)((int64_t)p.kblocks * (rank + 1) / splits);
+  const int nk = kb1 - kb0;
+  volatile int* abort_flag = &s_abort;
+
+  if (tid == 0) {
+    for (int i = 0; i < STAGES; i++) {
+      tc5::bar_init(FULL(i), 1);
+      tc5::bar_init(EMPTY(i), 1);
+    }
+    tc5::bar_init(DONE, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tc5::alloc(smem_u32(&s_slot), COLS);
+  tc5::fence_before();
+  __syncthreads();
+  tc5::fence_after();
+  const uint32_t tmem = s_slot;
+  auto fail = [&]() {
+    record_error(p.status, KERR_TIMEOUT);
+    *abort_flag = 1;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // The weights do not depend on the kernel before: as many as fit are on their way before its
+      // codes are waited for.
+      const int ahead = min(nk, STAGES);
+      for (int k = 0; k < ahead; k++) {
+        tc5::bar_expect(FULL(k), STAGE);
+        tc5::tma_2d(base + k * STAGE, &tmw, (kb0 + k) * 128, o0, FULL(k));
+      }
+      tc5::grid_wait();
+      for (int k = 0; k < ahead; k++)
+        tc5::tma_2d(base + k * STAGE + A_STAGE, &tmx, (kb0 + k) * 128, t0, FULL(k));
+      for (int k = ahead; k < nk; k++) {
+        const int s = k % STAGES;
+        if (!tc5::bar_wait(EMPTY(s), ((k / STAGES) + 1) & 1)) {
+          fail();
+          break;
+        }
+        tc5::bar_expect(FULL(s), STAGE);
+        tc5::tma_2d(base + s * STAGE, &tmw, (kb0 + k) * 128, o0, FULL(s));
+        tc5::tma_2d(base + s * STAGE + A_STAGE, &tmx, (kb0 + k) * 128, t0, FULL(s));
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      for (int k = 0; k < nk; k++) {
+        const int s = k % STAGES;
+        if (!tc5::bar_wait(FULL(s), (k / STAGES) & 1)) {
+          fail();
+          break;
+        }
+        tc5::fence_after();
+        const uint32_t sa = base + s * STAGE, sb = sa + A_STAGE;
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+          mma_i8(tmem, tc5::desc_sw128(sa + 32 * c), tc5::desc_sw128(sb + 32 * c), kIdesc, (k | c) ? 1u : 0u);
+        tc5::commit(EMPTY(s));
+      }
+      tc5::commit(DONE);
+    }
+  } else {
+    tc5::grid_wait();  // the token scales
+    const bool ok = tc5::bar_wait(DONE, 0);
+    if (!ok && lane == 0) fail();
+    tc5::fence_after();
+    const int quad = warp & 3, row = 32 * quad + lane, o = o0 + row;
+    const float wsc = o < p.N ? p.ws[o] : 0.0f, b = p.bias && o < p.N ? p.bias[o] : 0.0f;
+#pragma unroll 1
+    for (int c = 0; c < NT; c += 16) {
+      uint32_t r[16];
+      tc5::ld16(tmem + ((uint32_t)(32 * quad) << 16) + c, r);
+      tc5::wait_ld();
+      if (splits == 1) {
+        if (ok && !*abort_flag && o < p.N) {
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            if (t0 + c + i < p.T) store_y<Y>(p, t0 + c + i, o, (int)r[i], wsc, b);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++) part[(c + i) * BM + row] = nk ? (int)r[i] : 0;
+      }
+    }
+    tc5::fence_before();
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc5::fence_after();
+    tc5::dealloc(tmem, COLS);
+  }
+  if (splits > 1) {
+    cl.sync();
+    if (warp >= 2) {
+      const int row = 32 * (warp & 3) + lane, o = o0 + row;
+      const float wsc = o < p.N ? p.ws[o] : 0.0f, b = p.bias && o < p.N ? p.bias[o] : 0.0f;
+      for (int c = rank; c < NT && t0 + c < p.T; c += splits) {
+        int acc = 0;
+        for (int s = 0; s < splits; s++) acc += cl.map_shared_rank(part, s)[c * BM + row];
+        if (o < p.N && !*abort_flag) store_y<Y>(p, t0 + c, o, acc, wsc, b);
+      }
+    }
+    cl.sync();  // no CTA leaves while another still reads its part
+  }
+}
+
+template <int NT, int STAGES, typename Y>
+cudaError_t launch_tile(const CUtensorMap& tmw, const CUtensorMap& tmx, const I8Params& p, int splits, bool pdl,
+                        cudaStream_t st) {
+  constexpr size_t smem = (size_t)STAGES * (A_STAGE + NT * 128) + 1024;
+  cudaError_t e = cudaFuncSetAttribute(i8_tile_kernel<NT, STAGES, Y>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.N + BM - 1) / BM * splits), (unsigned)((p.T + NT - 1) / NT));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl && pdl_enabled() ? 2 : 1;
+  kernel_launch_count()++;
+  return cudaLaunchKernelEx(&cfg, i8_tile_kernel<NT, STAGES, Y>, tmw, tmx, p);
+}
+
+template <typename Y>
+cudaError_t product(const CUtensorMap& tmw, const CUtensorMap& tmx, const I8Params& p, int nt, int splits, bool pdl,
+                    cudaStream_t st) {
+  switch (nt) {
+    case 16: return launch_tile<16, 5, Y>(tmw, tmx, p, splits, pdl, st);
+    case 32: return launch_tile<32, 5, Y>(tmw, tmx, p, splits, pdl, st);
+    case 64: return launch_tile<64, 4, Y>(tmw, tmx, p, splits, pdl, st);
+    case 128: return launch_tile<128, 3, Y>(tmw, tmx, p, splits, pdl, st);
+    default: return launch_tile<256, 4, Y>(tmw, tmx, p, splits, pdl, st);
+  }
+}
+
+int64_t code_pitch(int64_t in_feat) { return (in_feat + 15) / 16 * 16; }
+
+}  // namespace
+}  // namespace vtq
+
+using namespace vtq;
+
+extern "C" {
+
+vtq_status vtq_quantize_tokens(int32_t x_dtype, const void* x, int64_t ldx, int64_t tokens, int64_t in_feat,
+                               int8_t* q, int64_t ldq, float* scale, void* stream) {
+  const char* fn = "vtq_quantize_tokens";
+  if (!serve_elt(x_dtype))
+    return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "%s: not implemented (x not F32 / F16 / BF16)", fn);
+  if (tokens < 0 || in_feat < 0 || tokens > INT32_MAX || ldq < in_feat)
+    return serve_fail(VTQ_ERR_INTERNAL, "%s: bad shape", fn);
+  if (tokens == 0) return VTQ_OK;
+  if ((!x && in_feat) || (!q && in_feat) || !scale) return serve_fail(VTQ_ERR_INVALID_ARG, "%s: null pointer", fn);
+  return serve_cuda(quantize(x_dtype, x, ldx, tokens, in_feat, q, ldq, scale, static_cast<cudaStream_t>(stream)), fn);
+}
+
+size_t vtq_linear_i8_workspace_bytes(int32_t x_dtype, int64_t tokens, int64_t in_feat, int64_t out_feat) {
+  (void)out_feat;
+  if (x_dtype == VTQ_I8 || tokens <= 0 || in_feat < 0) return 0;
+  return ((size_t)tokens * code_pitch(in_feat) + 255) / 256 * 256 + (size_t)tokens * 4;
+}
+
+vtq_status vtq_linear_i8(const vtq_linear_i8_args* a, void* ws, size_t ws_bytes, void* stream) {
+  const char* fn = "vtq_linear_i8";
+  if (!a) return serve_fail(VTQ_ERR_INVALID_ARG, "%s: null arguments", fn);
+  const bool codes = a->x_dtype == VTQ_I8;
+  if (!codes && !serve_elt(a->x_dtype))
+    return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "%s: not implemented (x not I8 / F32 / F16 / BF16)", fn);
+  if (!serve_elt(a->y_dtype))
+    return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "%s: not implemented (y not F32 / F16 / BF16)", fn);
+  if (a->tokens < 0 || a->in_feat < 1 || a->out_feat < 0 || a->ldw < a->in_feat)
+    return serve_fail(VTQ_ERR_INTERNAL, "%s: bad shape", fn);
+  if (a->in_feat > 131072 || a->out_feat > (1 << 28) || a->tokens > (1 << 20))
+    return serve_fail(VTQ_ERR_NOT_IMPLEMENTED,
+                      "%s: not implemented (in_feat over 131072, out_feat over 2^28 or tokens over 2^20)", fn);
+  if (a->tokens == 0 || a->out_feat == 0) return VTQ_OK;
+  if (!a->x || !a->w || !a->w_scale || !a->y || (codes && !a->x_scale))
+    return serve_fail(VTQ_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (!aligned16(a->w) || a->ldw % 16)
+    return serve_fail(VTQ_ERR_INTERNAL, "%s: w not 16-byte aligned, or ldw not a multiple of 16", fn);
+  if (codes && (!aligned16(a->x) || a->ldx % 16 || a->ldx < a->in_feat))
+    return serve_fail(VTQ_ERR_INTERNAL, "%s: codes not 16-byte aligned, or ldx not a multiple of 16", fn);
+  const size_t need = vtq_linear_i8_workspace_bytes(a->x_dtype, a->tokens, a->in_feat, a->out_feat);
+  if (need && (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255u)))
+    return serve_fail(VTQ_ERR_INVALID_ARG, "%s: workspace missing, too small or not 256-byte aligned", fn);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int8_t* q = static_cast<const int8_t*>(a->x);
+  const float* xs = a->x_scale;
+  int64_t ldq = a->ldx;
+  if (!codes) {
+    int8_t* qw = static_cast<int8_t*>(ws);
+    ldq = code_pitch(a->in_feat);
+    float* sw = reinterpret_cast<float*>(qw + ((size_t)a->tokens * ldq + 255) / 256 * 256);
+    if (vtq_status s = serve_cuda(quantize(a->x_dtype, a->x, a->ldx, a->tokens, a->in_feat, qw, ldq, sw, st), fn)) return s;
+    q = qw;
+    xs = sw;
+  }
+  // The smallest token tile that holds the batch; the K axis split until the CTAs fill the SMs.
+  const int T = (int)a->tokens, kb = (int)((a->in_feat + 127) / 128);
+  const int nt = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
+  const int64_t tiles = (a->out_feat + BM - 1) / BM * ((T + nt - 1) / nt);
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= 2 * num_sms() && kb >= splits * 4) splits *= 2;
+  CUtensorMap tmw, tmx;
+  cudaError_t e = tma_byte_map(&tmw, a->w, a->out_feat, a->in_feat, a->ldw, 128, BM, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (e == cudaSuccess) e = tma_byte_map(&tmx, q, T, a->in_feat, ldq, 128, (uint32_t)nt, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (e != cudaSuccess) return serve_cuda(e, fn);
+  const I8Params p{T, (int)a->in_feat, (int)a->out_feat, kb, xs, a->w_scale, a->bias, a->y, a->ldy, a->status};
+  if (a->y_dtype == VTQ_F32) e = product<float>(tmw, tmx, p, nt, splits, !codes, st);
+  else if (a->y_dtype == VTQ_F16) e = product<__half>(tmw, tmx, p, nt, splits, !codes, st);
+  else e = product<__nv_bfloat16>(tmw, tmx, p, nt, splits, !codes, st);
+  return serve_cuda(e, fn);
+}
+
+}  // extern "C"

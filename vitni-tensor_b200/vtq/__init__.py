@@ -43,6 +43,9 @@ EXPORTS = (
     "vtq_decode_timing", "vtq_decode_debug_buffer", "vtq_decode_step_kind",
     "vtq_exact_sum_host", "vtq_exact_sum_device", "vtq_decode_launches", "vtq_linear_list", "vtq_set_wait_limit",
     "vtq_linear_list_gather", "vtq_linear_device_workspace_bytes", "vtq_linear_device_ws",
+    "vtq_device_last_error", "vtq_quantize_tokens", "vtq_linear_i8_workspace_bytes", "vtq_linear_i8",
+    "vtq_append_kv", "vtq_attention_paged_workspace_bytes", "vtq_attention_paged", "vtq_verify_draft",
+    "vtq_verify_greedy",
 )
 
 
