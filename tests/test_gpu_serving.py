@@ -351,6 +351,91 @@ def test_attention(S, dtype, counts, lens, heads, kv, dim, page, shared, hnd):
         assert torch.equal(out, S.attention_paged(q, kp, vp, table, kv_len, shared_len=shared))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("counts,own,heads,kv,dim,page,shared,hnd", [
+    ([1] * 17, 9, 2, 2, 64, 16, 512, False),                # the fewest rows of the prefix's own kernel
+    ([1] * 33, 40, 12, 3, 80, 7, 1000, True),               # 132 rows: two blocks, a prefix that ends anywhere
+    ([2, 0, 5, 1] * 8, 12, 10, 2, 128, 64, 4097, False),
+    ([1] * 64, 70, 32, 8, 128, 16, 2048, True),
+    ([3] * 11, 5, 16, 2, 256, 32, 777, False),
+    ([1] * 130, 3, 4, 4, 72, 128, 6000, True),
+    ([4] * 5, 20, 64, 4, 96, 24, 20000, False)])
+def test_attention_long_prefix(S, dtype, counts, own, heads, kv, dim, page, shared, hnd):
+    g = gen(shared + dim)
+    lens = [shared + n + int(e) for n, e in zip(counts, torch.randint(0, own, (len(counts),), generator=g, device="cuda"))]
+    q, kp, vp, table, kv_len, start = attention_case(g, counts, lens, heads, kv, dim, page, shared, dtype, hnd)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out, lse = S.attention_paged(q, kp, vp, table, kv_len, q_start=start, shared_len=shared, return_lse=True, status=status)
+    want, size, want_lse = attention64(q, kp, vp, table, lens, counts, shared)
+    assert status.item() == 0
+    assert attention_close(out, want, size, dtype)
+    assert ((lse.double() - want_lse).abs() <= 2 ** -16 + 2 ** -20 * want_lse.abs()).all()
+    assert torch.equal(out, S.attention_paged(q, kp, vp, table, kv_len, q_start=start, shared_len=shared))
+    # queries at odd addresses
+    wide = torch.zeros(len(q), heads, dim + 3, dtype=dtype, device="cuda")
+    wide[..., 1:dim + 1] = q
+    assert torch.equal(out, S.attention_paged(wide[..., 1:dim + 1], kp, vp, table, kv_len, q_start=start, shared_len=shared))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_growing_and_negative_scores(S, dtype):
+    """Scores that rise along the prefix by hundreds, so that what was summed before is scaled down again and again;
+    and a scale below 0."""
+    counts, shared = [1] * 20, 1500
+    lens = [shared + 1 + i for i in range(20)]
+    q, kp, vp, table, kv_len, start = attention_case(gen(12), counts, lens, 8, 2, 64, 16, shared, dtype, False)
+    kp[table[0, :shared // 16].long()] *= torch.linspace(0, 6, shared // 16, device="cuda").to(dtype)[:, None, None, None]
+    q *= 4
+    for scale in (1.0, -0.125, 0.0):
+        out = S.attention_paged(q, kp, vp, table, kv_len, shared_len=shared, scale=scale)
+        k64 = scale if scale else 1e-300
+        want, size, _ = attention64(q, kp, vp, table, lens, counts, shared, k64)
+        # scores up to about 600 in 32 bits: 2^-12 of a weight
+        assert ((out.double() - want).abs() <= (half_step(dtype) + 2 ** -11) * size + half_step(dtype) * want.abs() + 2 ** -24).all()
+
+
+@pytest.mark.parametrize("shared", [40, 1024])
+def test_attention_padded_batch(S, shared):
+    """Empty sequences, one that ends inside the prefix and one at its end, next to ordinary ones; NaN all over the
+    slots that nobody reaches, and in keys of the prefix that only the longer ones reach."""
+    lens = [0, shared + 3, shared // 2, 0, shared, shared + 50, 1] + [shared + 9] * 20 + [0] * 5
+    counts = [1] * len(lens)
+    q, kp, vp, table, kv_len, start = attention_case(gen(13), counts, lens, 8, 4, 64, 16, shared, F16, False, math.nan)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out, lse = S.attention_paged(q, kp, vp, table, kv_len, shared_len=shared, return_lse=True, status=status)
+    want, size, want_lse = attention64(q, kp, vp, table, lens, counts, shared)
+    assert status.item() == 0
+    assert attention_close(out, want, size, F16)
+    assert (out[0] == 0).all() and torch.isinf(lse[0]).all()
+    assert torch.equal(torch.isinf(lse), torch.isinf(want_lse))
+    j = shared // 2 + 5  # behind the end of sequence 2
+    vp[table[0, j // 16].long(), j % 16, 2, 7] = math.inf
+    again = S.attention_paged(q, kp, vp, table, kv_len, shared_len=shared)
+    see = torch.tensor([n > j for n in lens], device="cuda")
+    assert torch.equal(again[~see], out[~see]) and torch.isposinf(again[see][:, 4:6, 7]).all()
+    # all of them empty: a table without any page
+    none = torch.full_like(table, -1)
+    out = S.attention_paged(q, kp, vp, none, torch.zeros_like(kv_len), shared_len=shared, status=status)
+    assert (out == 0).all() and status.item() == 0
+
+
+def test_attention_bad_page_of_a_long_prefix(S):
+    counts, shared = [1] * 24, 600
+    lens = [shared + 4] * 24
+    q, kp, vp, table, kv_len, start = attention_case(gen(14), counts, lens, 2, 2, 64, 8, shared, BF16, False)
+    bad = table.clone()
+    bad[0, 30], bad[0, 70] = 10 ** 8, -1
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = S.attention_paged(q, kp, vp, bad, kv_len, shared_len=shared, status=status)
+    assert status.item() == 2
+    keep = torch.tensor([j for j in range(604) if j // 8 not in (30, 70)], device="cuda")
+    for b in (0, 23):
+        rows = torch.where(keep < shared, 0, b)
+        k, v = (c[table[rows, keep // 8].long(), keep % 8].double() for c in (kp, vp))
+        p = torch.softmax(torch.einsum("hd,lhd->hl", q[b].double(), k) / 8, 1)
+        assert attention_close(out[b], torch.einsum("hl,lhd->hd", p, v), torch.einsum("hl,lhd->hd", p, v.abs()), BF16)
+
+
 @pytest.mark.parametrize("spare", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("shared", [0, 37])
 def test_attention_ignores_what_lies_behind(S, spare, shared):

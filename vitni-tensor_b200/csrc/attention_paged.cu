@@ -25,6 +25,7 @@ vtq_status serve_check_kv(const char* fn, const vtq_paged_kv& kv);
 namespace {
 
 constexpr int kRows = 16;      // query rows of a segment: M of the MMA
+constexpr int kTileRows = 128; // of a segment of the prefix on tcgen05
 constexpr int kMaxSeqs = 1024;
 
 struct AttnParams {
@@ -39,12 +40,17 @@ struct AttnParams {
   int* plan;        // the plan arrays below, for the joining kernel
   float* part;      // slots of kRows (m, l) and o
   int dim_padded;
+  // The prefix on the tensor cores' own tiles (attention_tile_kernel), where on_tiles is set:
+  bool on_tiles, q_copies;           // q_copies: q rows can be copied 16 bytes at a time
+  int tile_segs, tiles_each;         // blocks of kTileRows rows of a kv head, key tiles of each
+  int tiles_total, tile_parts;       // in all; CTAs that share them
+  float* tile_part;                  // slots of kTileRows (m, l) and o
 };
 
 // The cut of the work: prefix sums over the sequences (index B: the shared prefix). Tiles before, and
 // segments before, each sequence; its first query row; its length.
 struct Plan {
-  int *tiles, *segs, *q0, *len;  // [B + 2], [B + 2], [B + 1], [B + 1] (len[B]: of the prefix)
+  int *tiles, *segs, *q0, *len;  // [B + 2], [B + 2], [B + 1], [B + 1] (len[B]: of the prefix, 0 if nobody sees it)
 };
 __host__ __device__ inline int plan_ints(int B) { return 4 * (B + 2) + 2; }
 
@@ -54,27 +60,33 @@ __device__ __forceinline__ Plan plan_of(int* base, int B) {
 
 __device__ __forceinline__ int seq_rows(const Plan& pl, int b) { return pl.q0[b + 1] - pl.q0[b]; }
 
+// Whether every row of a sequence sees the whole prefix. The rows of one that does not (it ends inside
+// the prefix, or is empty) take no part in the prefix's segments: it has all its keys for its own, so
+// that those segments need no mask for rows, and what they hold cannot reach a row that must not see it.
+__device__ __forceinline__ bool sees_prefix(const AttnParams& p, const Plan& pl, int b) {
+  const int n = seq_rows(pl, b);
+  return n > 0 && pl.len[b] - n + 1 >= p.prefix;
+}
+
 // Built by all threads of a CTA in its shared memory; base[0] = tiles in all, base[1] = parts in use.
 __device__ void build_plan(const AttnParams& p, int* base) {
   const int B = (int)p.a.kv.seqs, T = (int)p.a.tokens, H = (int)p.a.kv.kv_heads;
   const Plan pl = plan_of(base, B);
-  __shared__ int s_longest, s_bad, s_warp_t[32], s_warp_s[32];
+  __shared__ int s_any, s_bad, s_warp_t[32], s_warp_s[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid == 0) s_longest = s_bad = 0;
+  if (tid == 0) s_any = s_bad = 0;
   __syncthreads();
   for (int b = tid; b <= B; b += blockDim.x) {
     pl.q0[b] = p.a.q_start ? min(max(p.a.q_start[b], 0), T) : min(b, T);
-    if (b < B) {
-      const int len = max(p.a.kv_len[b], 0);
-      pl.len[b] = len;
-      atomicMax(&s_longest, len);
-    }
+    if (b < B) pl.len[b] = max(p.a.kv_len[b], 0);
   }
   __syncthreads();
-  for (int b = tid; b < B; b += blockDim.x)
+  for (int b = tid; b < B; b += blockDim.x) {
     if (pl.q0[b + 1] < pl.q0[b]) s_bad = 1;
-  if (tid == 0) pl.len[B] = min(s_longest, p.prefix);
+    else if (sees_prefix(p, pl, b)) s_any = 1;
+  }
   __syncthreads();
+  if (tid == 0) pl.len[B] = s_any && !s_bad ? p.prefix : 0;
   if (s_bad) {  // row starts that decrease: no sequence owns a row (the slots are counted for one owner a row)
     for (int b = tid; b <= B; b += blockDim.x) pl.q0[b] = 0;
     if (tid == 0 && p.a.status) atomicOr(p.a.status, SERVE_BAD_INDEX);
@@ -88,10 +100,10 @@ __device__ void build_plan(const AttnParams& p, int* base) {
       int rows, keys;
       if (b < B) {
         rows = seq_rows(pl, b) * p.group;
-        keys = max(min(pl.len[b], p.keys_max) - p.prefix, 0);
+        keys = max(min(pl.len[b], p.keys_max) - (sees_prefix(p, pl, b) ? p.prefix : 0), 0);
       } else {
-        rows = T * p.group;
-        keys = s_bad ? 0 : pl.len[B];
+        rows = p.on_tiles ? 0 : T * p.group;  // the prefix has a kernel of its own then
+        keys = pl.len[B];
       }
       const int segs = (rows + kRows - 1) / kRows * H;
       if (pass) pl.tiles[b] = st, pl.segs[b] = ss;
@@ -119,6 +131,10 @@ __device__ void build_plan(const AttnParams& p, int* base) {
     base[1] = min(pl.tiles[n], p.parts);
   }
   __syncthreads();
+}
+
+__device__ __forceinline__ int first_key(const AttnParams& p, const Plan& pl, int b, int B) {
+  return b < B && sees_prefix(p, pl, b) ? p.prefix : 0;
 }
 
 // Part w of W covers tiles [first(w), first(w + 1)) of `total`; part_of is its inverse.
@@ -234,7 +250,7 @@ __device__ __forceinline__ bool odd_word(uint32_t w) {
   return (w & e) == e || ((w >> 16) & e) == e;
 }
 
-// DP: head_dim rounded up to what the MMA loop takes (64, 96, 128, 256). KT keys a tile, a warp's
+// DP: head_dim rounded up to what the MMA loop takes (64, 128, 256). KT keys a tile, a warp's
 // pipeline STAGES tiles of K and V deep; no barrier but the warp's own.
 template <typename T, int DP, int KT, int WARPS, int STAGES>
 __global__ void __launch_bounds__(32 * WARPS, 1) attention_part_kernel(const __grid_constant__ AttnParams p) {
@@ -259,12 +275,14 @@ __global__ void __launch_bounds__(32 * WARPS, 1) attention_part_kernel(const __g
         if (pl.len[b] > p.keys_max || p.a.kv_len[b] < 0) atomicOr(p.a.status, SERVE_BAD_INDEX);
   }
   const int w = warp * (int)gridDim.x + (int)blockIdx.x;  // few parts spread over the SMs first
-  if (w >= W) return;
+  if (w >= W) {
+    tc5::grid_wait();
+    return;
+  }
   const int tile0 = first_tile(total, W, w), tile1 = first_tile(total, W, w + 1);
   const uint32_t stage0 = smem_u32(smem) + warp * STAGES * kStage;
   auto swizzled = [](int key, int chunk) {
-    const int x = DP == 96 ? (key >> 1) & 3 : key & 7;  // eight rows' chunks in eight different bank groups
-    return (uint32_t)(key * DP * 2 + ((chunk ^ x) << 4));
+    return (uint32_t)(key * DP * 2 + ((chunk ^ (key & 7)) << 4));  // eight rows' chunks in eight bank groups
   };
   const T* K = static_cast<const T*>(p.a.kv.k);
   const T* V = static_cast<const T*>(p.a.kv.v);
@@ -272,7 +290,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) attention_part_kernel(const __g
   // Starts tile `c` into stage s.
   auto load = [&](const Cursor& c, int s) {
     const bool shared = c.b == B;
-    const int key0 = (shared ? 0 : p.prefix) + c.t * KT;
+    const int key0 = first_key(p, pl, c.b, B) + c.t * KT;
     const int end = shared ? pl.len[B] : min(pl.len[c.b], p.keys_max);
     bool ok = false;
     if (lane < KT) {
@@ -280,7 +298,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) attention_part_kernel(const __g
       int64_t ko = 0, vo = 0;
       if (pos < end) {
         const int page_size = (int)p.a.kv.page_size, at = pos / page_size;
-        const int64_t page = p.a.kv.table[(shared ? 0 : c.b) * p.a.kv.table_ld + at], slot = pos - at * page_size;
+        const int64_t page = p.a.kv.table[(pos < p.prefix ? 0 : c.b) * p.a.kv.table_ld + at], slot = pos - at * page_size;
         ok = page >= 0 && page < p.a.kv.pages;
         if (ok) {
           ko = page * p.a.kv.k_page + slot * p.a.kv.k_slot + c.g * p.a.kv.k_head;
@@ -337,11 +355,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) attention_part_kernel(const __g
         lim[h] = 0;
         if (r < rows_in) {
           qr[h] = static_cast<const T*>(p.a.q) + (int64_t)(q0 + tok) * p.a.q_tok + (int64_t)(c.g * p.group + row - tok * p.group) * p.a.q_head;
-          const int b = shared ? owner(pl, B, tok) : c.b;
-          if (b >= 0) {
-            const int i = q0 + tok - pl.q0[b];
-            lim[h] = min(pl.len[b] - seq_rows(pl, b) + i + 1, p.keys_max);
-          }
+          lim[h] = shared ? INT32_MAX : min(pl.len[c.b] - n + tok + 1, p.keys_max);
         }
       }
       lim0 = lim[0], lim1 = lim[1];
@@ -380,7 +394,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) attention_part_kernel(const __g
     __syncwarp();
     const uint32_t k_s = stage0 + s * kStage, v_s = k_s + kTileBytes;
     const uint32_t valid = s_valid[warp][s];
-    const int key0 = (c.b == B ? 0 : p.prefix) + c.t * KT;
+    const int key0 = first_key(p, pl, c.b, B) + c.t * KT;
     float sc[KT / 8][4];
 #pragma unroll
     for (int i = 0; i < KT / 8; i++)
@@ -507,6 +521,404 @@ __global__ void __launch_bounds__(32 * WARPS, 1) attention_part_kernel(const __g
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
+  tc5::grid_wait();  // the join waits for this kernel alone: the prefix's has to be done with it
+}
+
+// ---- the prefix on tcgen05 ----
+//
+// One CTA takes 128 query rows (heads of a kv head, tokens of all sequences) over a run of key tiles:
+//   warps 0-3  softmax: a thread a row. S from TMEM, weights back into TMEM as the second product's A.
+//   warps 4-7  loaders: pages gathered with 16-byte copies into swizzled tiles, STAGES deep
+//   warp 8     one thread issues S = Q K^T (K tile: N = KT keys) and O += P V (V as it lies: N-major)
+// S is double-buffered, so the next tile's first product runs beside the softmax of this one. O stays in
+// TMEM; it is scaled again only where a row's maximum has grown by more than 2^8 since the last time, until
+// then the weights are taken relative to the old one (at most 256, and l with them).
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// N-major operand, 128-byte swizzle: 64 values of N a row of 128 bytes, 8 rows (K) an atom of 1024;
+// `chunk` bytes to the next 64 values of N, 1024 to the next 8 of K.
+__device__ __forceinline__ uint64_t desc_n_major(uint32_t saddr, uint32_t chunk) {
+  return (uint64_t)((saddr >> 4) & 0x3fffu) | (uint64_t)(chunk >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float* r) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+        "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(u[0]),
+      "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]),
+      "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]),
+      "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]),
+      "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+constexpr int kTileThreads = 288;
+
+template <typename T, int DP, int KT, int STAGES>
+struct TileShape {
+  static constexpr uint32_t Q_BYTES = kTileRows * DP * 2, KV_BYTES = KT * DP * 2, STAGE = 2 * KV_BYTES;
+  static constexpr size_t SMEM = Q_BYTES + STAGES * STAGE + 1024;
+};
+
+template <typename T, int DP, int KT, int STAGES>
+__global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const __grid_constant__ AttnParams p) {
+  using L = TileShape<T, DP, KT, STAGES>;
+  constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
+  constexpr uint32_t kIdescS = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((uint32_t)(KT >> 3) << 17) | (8u << 24);
+  constexpr uint32_t kIdescO = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | (8u << 24);
+  constexpr uint32_t kColO = 2 * KT;  // columns: S / P twice, then O
+  static_assert(2 * KT + DP <= 512, "TMEM");
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t s_bar[4 * STAGES + 7];
+  __shared__ uint32_t s_valid[STAGES][4];
+  __shared__ uint32_t s_slot;
+  __shared__ int s_abort, s_any;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
+  auto bar = [&](int i) { return smem_u32(&s_bar[i]); };
+  auto K_FULL = [&](int s) { return bar(s); };
+  auto V_FULL = [&](int s) { return bar(STAGES + s); };
+  auto K_EMPTY = [&](int s) { return bar(2 * STAGES + s); };
+  auto V_EMPTY = [&](int s) { return bar(3 * STAGES + s); };
+  auto S_FULL = [&](int s) { return bar(4 * STAGES + s); };
+  auto P_FULL = [&](int s) { return bar(4 * STAGES + 2 + s); };
+  const uint32_t Q_FULL = bar(4 * STAGES + 4), Q_EMPTY = bar(4 * STAGES + 5), PV_DONE = bar(4 * STAGES + 6);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int B = (int)p.a.kv.seqs, D = (int)p.a.kv.head_dim;
+  volatile int* abort_flag = &s_abort;
+
+  tc5::grid_release();
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; s++) {
+      tc5::bar_init(K_FULL(s), 128);
+      tc5::bar_init(V_FULL(s), 128);
+      tc5::bar_init(K_EMPTY(s), 1);
+      tc5::bar_init(V_EMPTY(s), 1);
+    }
+    for (int s = 0; s < 2; s++) {
+      tc5::bar_init(S_FULL(s), 1);
+      tc5::bar_init(P_FULL(s), 128);
+    }
+    tc5::bar_init(Q_FULL, 128);
+    tc5::bar_init(Q_EMPTY, 1);
+    tc5::bar_init(PV_DONE, 1);
+    *abort_flag = 0;
+    s_any = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) tc5::alloc(smem_u32(&s_slot), 512);
+  __syncthreads();
+  // Nothing to do where no sequence sees the prefix (its pages need not exist then).
+  for (int b = tid; b < B; b += kTileThreads) {
+    const int T_ = (int)p.a.tokens;
+    const int q0 = p.a.q_start ? min(max(p.a.q_start[b], 0), T_) : b, q1 = p.a.q_start ? min(max(p.a.q_start[b + 1], 0), T_) : b + 1;
+    if (q1 > q0 && p.a.kv_len[b] - (q1 - q0) + 1 >= p.prefix) s_any = 1;
+  }
+  tc5::fence_before();
+  __syncthreads();
+  tc5::fence_after();
+  const uint32_t tmem = s_slot;
+  const int tile0 = first_tile(p.tiles_total, p.tile_parts, (int)blockIdx.x);
+  const int tile1 = s_any ? first_tile(p.tiles_total, p.tile_parts, (int)blockIdx.x + 1) : tile0;
+  auto fail = [&]() {
+    if (p.a.status) atomicOr(p.a.status, KERR_TIMEOUT);
+    *abort_flag = 1;
+  };
+  // Bytes into a K, V or Q tile of `rows` rows: blocks of 64 values, 128-byte rows, 16-byte chunks swizzled.
+  auto place = [](int rows, int row, int chunk) {
+    return (uint32_t)((chunk >> 3) * rows * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+  };
+
+  if (warp >= 4 && warp < 8) {
+    // ---- loaders: warp lw owns 32 keys of each 128 (16 of 64), 8 lanes a row of 128 bytes ----
+    const int lw = warp - 4, mine = KT / 4;
+    const T* K = static_cast<const T*>(p.a.kv.k);
+    const T* V = static_cast<const T*>(p.a.kv.v);
+    int told = tile0;  // tiles that the consumers have been told of
+    int q_seg = -1;
+    bool q_new = false;
+    auto tell = [&](int upto) {  // every copy of tiles before `upto` has landed
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      for (; told < upto; told++) {
+        const int s = (told - tile0) % STAGES;
+        if (q_new && told == upto - 1) {
+          tc5::bar_arrive(Q_FULL);
+          q_new = false;
+        }
+        tc5::bar_arrive(K_FULL(s));
+        tc5::bar_arrive(V_FULL(s));
+      }
+    };
+    int segs_seen = 0;
+    for (int t = tile0; t < tile1 && !*abort_flag; t++) {
+      const int j = t - tile0, s = j % STAGES, seg = t / p.tiles_each, kt = t - seg * p.tiles_each;
+      const int g = seg / p.tile_segs, mt = seg - g * p.tile_segs;
+      if (seg != q_seg) {
+        // Everything before is told of first, so that the segment's first tile alone carries Q.
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        tell(t);
+        if (segs_seen && !tc5::bar_wait(Q_EMPTY, (segs_seen - 1) & 1)) {
+          if (lane == 0) fail();
+          break;
+        }
+        segs_seen++;
+        q_seg = seg;
+        q_new = true;
+        const int rows = (int)p.a.tokens * p.group;
+        for (int i = 0; i < 8; i++) {
+          const int r = lw * 32 + i * 4 + (lane >> 3);
+          const int row = mt * kTileRows + r, tok = row / p.group;
+          const bool in = row < rows;
+          const T* src = static_cast<const T*>(p.a.q) + (in ? (int64_t)tok * p.a.q_tok + (int64_t)(g * p.group + row - tok * p.group) * p.a.q_head : 0);
+#pragma unroll
+          for (int c = 0; c < DP / 64; c++) {
+            const int chunk = c * 8 + (lane & 7);
+            const bool there = in && chunk * 8 < D;
+            const uint32_t at = place(kTileRows, r, chunk);
+            if (p.q_copies) {
+              copy16(base + at, src + (there ? chunk * 8 : 0), there);
+            } else {
+              T* dst = reinterpret_cast<T*>(gbase + at);
+#pragma unroll
+              for (int e = 0; e < 8; e++) dst[e] = there ? src[chunk * 8 + e] : from_f32<T>(0.0f);
+            }
+          }
+        }
+      }
+      // This lane's key of the tile.
+      const int pos = kt * KT + lw * mine + lane;
+      int64_t ko = 0, vo = 0;
+      bool ok = false;
+      if (lane < mine && pos < p.prefix) {
+        const int page_size = (int)p.a.kv.page_size, at = pos / page_size;
+        const int64_t page = p.a.kv.table[at], slot = pos - at * page_size;
+        ok = page >= 0 && page < p.a.kv.pages;
+        if (ok) {
+          ko = page * p.a.kv.k_page + slot * p.a.kv.k_slot + g * p.a.kv.k_head;
+          vo = page * p.a.kv.v_page + slot * p.a.kv.v_slot + g * p.a.kv.v_head;
+        } else if (p.a.status) {
+          atomicOr(p.a.status, SERVE_BAD_INDEX);
+        }
+      }
+      const uint32_t valid = __ballot_sync(0xffffffffu, ok);
+      if (j >= STAGES) {
+        const uint32_t ph = ((j / STAGES) + 1) & 1;
+        if (!mbar_try_wait(&s_bar[3 * STAGES + s], ph) || !mbar_try_wait(&s_bar[2 * STAGES + s], ph)) {
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+          tell(t);
+          if (!tc5::bar_wait(K_EMPTY(s), ph) || !tc5::bar_wait(V_EMPTY(s), ph)) {
+            if (lane == 0) fail();
+            break;
+          }
+        }
+        __syncwarp();
+      }
+      if (lane == 0) s_valid[s][lw] = valid;
+      const uint32_t k_s = base + L::Q_BYTES + s * L::STAGE, v_s = k_s + L::KV_BYTES;
+#pragma unroll
+      for (int i = 0; i < KT / 16; i++) {
+        const int r = i * 4 + (lane >> 3), key = lw * mine + r;
+        const bool in = (valid >> r) & 1;
+        const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+#pragma unroll
+        for (int c = 0; c < DP / 64; c++) {
+          const int chunk = c * 8 + (lane & 7);
+          const bool there = in && chunk * 8 < D;
+          copy16(k_s + place(KT, key, chunk), K + (there ? kr + chunk * 8 : 0), there);
+          copy16(v_s + place(KT, key, chunk), V + (there ? vr + chunk * 8 : 0), there);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      tell(t);  // the tile before
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!*abort_flag) tell(tile1);
+  } else if (warp == 8) {
+    if (lane == 0) {
+      int segs_seen = 0;
+      auto first_product = [&](int t) {
+        const int j = t - tile0, s = j % STAGES, kt = t % p.tiles_each;
+        if (t == tile0 || kt == 0) {
+          if (!tc5::bar_wait(Q_FULL, segs_seen & 1)) return false;
+          segs_seen++;
+        }
+        if (!tc5::bar_wait(K_FULL(s), (j / STAGES) & 1)) return false;
+        tc5::fence_after();
+        const uint32_t k_s = base + L::Q_BYTES + s * L::STAGE;
+#pragma unroll
+        for (int k = 0; k < DP / 16; k++)
+          mma_ss(tmem + (j & 1) * KT, tc5::desc_sw128(base + (k >> 2) * (kTileRows * 128) + (k & 3) * 32),
+                 tc5::desc_sw128(k_s + (k >> 2) * (KT * 128) + (k & 3) * 32), kIdescS, k > 0);
+        tc5::commit(S_FULL(j & 1));
+        tc5::commit(K_EMPTY(s));
+        if (t + 1 == tile1 || kt + 1 == p.tiles_each) tc5::commit(Q_EMPTY);
+        return true;
+      };
+      bool ok = tile0 < tile1 ? first_product(tile0) : true;
+      for (int t = tile0; t < tile1 && ok; t++) {
+        const int j = t - tile0, s = j % STAGES;
+        if (t + 1 < tile1) ok = first_product(t + 1);
+        ok = ok && tc5::bar_wait(P_FULL(j & 1), (j >> 1) & 1) && tc5::bar_wait(V_FULL(s), (j / STAGES) & 1);
+        if (!ok) break;
+        tc5::fence_after();
+        const uint32_t v_s = base + L::Q_BYTES + s * L::STAGE + L::KV_BYTES;
+        const bool start = t == tile0 || t % p.tiles_each == 0;
+#pragma unroll
+        for (int k = 0; k < KT / 16; k++)
+          mma_ts(tmem + kColO, tmem + (j & 1) * KT + 8 * k, desc_n_major(v_s + k * 2048, KT * 128), kIdescO, !start || k > 0);
+        tc5::commit(V_EMPTY(s));
+        tc5::commit(PV_DONE);
+      }
+      if (!ok) fail();
+    }
+  } else if (warp < 4) {
+    // ---- softmax: row tid ----
+    const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+    float m = -INFINITY, l = 0.0f;  // m: what the weights are relative to
+    for (int t = tile0; t < tile1; t++) {
+      const int j = t - tile0, s = j % STAGES, seg = t / p.tiles_each;
+      const bool start = t == tile0 || t % p.tiles_each == 0, last = t + 1 == tile1 || (t + 1) % p.tiles_each == 0;
+      if (!tc5::bar_wait(S_FULL(j & 1), (j >> 1) & 1)) {
+        if (lane == 0) fail();
+        break;
+      }
+      // (done long ago: waited for here too because it is what publishes s_valid)
+      if (!tc5::bar_wait(K_FULL(s), (j / STAGES) & 1)) {
+        if (lane == 0) fail();
+        break;
+      }
+      tc5::fence_after();
+      const uint32_t sp = tmem + lanes + (j & 1) * KT;
+      float x[KT];
+#pragma unroll
+      for (int c = 0; c < KT / 32; c++) tmem_ld32(sp + 32 * c, x + 32 * c);
+      tc5::wait_ld();
+      constexpr int kWord = KT / 4;  // keys of a loader warp: bits of a word of s_valid
+      bool whole = true;
+#pragma unroll
+      for (int w = 0; w < 4; w++) whole = whole && s_valid[s][w] == (kWord == 32 ? 0xffffffffu : (1u << (kWord & 31)) - 1u);
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < KT; i++)
+          if (!((s_valid[s][i / kWord] >> (i % kWord)) & 1)) x[i] = -INFINITY;
+      }
+      float top = x[0];
+#pragma unroll
+      for (int i = 1; i < KT; i++) top = fmaxf(top, x[i]);
+      // The scale may be negative or 0: the largest score is then that of the smallest product.
+      if (p.scale_log2 <= 0.0f) {
+        top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < KT; i++) top = fmaxf(top, x[i] == -INFINITY && !whole ? -INFINITY : x[i] * p.scale_log2);
+      } else {
+        top *= p.scale_log2;
+      }
+      if (start) {
+        m = top;
+        l = 0.0f;
+      } else {
+        const bool grow = top > m + 8.0f || (m == -INFINITY && top > -INFINITY);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float to = grow ? top : m;
+          const float f = m == -INFINITY ? 0.0f : exp2_fast(m - to);
+          if (!tc5::bar_wait(PV_DONE, (j - 1) & 1)) {
+            if (lane == 0) fail();
+            break;
+          }
+          tc5::fence_after();
+#pragma unroll 1
+          for (int c = 0; c < DP / 32; c++) {
+            float o[32];
+            tmem_ld32(tmem + lanes + kColO + 32 * c, o);
+            tc5::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] *= grow ? f : 1.0f;
+            tmem_st32(tmem + lanes + kColO + 32 * c, reinterpret_cast<const uint32_t*>(o));
+          }
+          tmem_wait_st();
+          if (grow) l *= f;
+          m = to;
+        }
+      }
+      const float u = m == -INFINITY ? 0.0f : m;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < KT / 64; c++) {
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+          const int k = 64 * c + 2 * i;
+          float a = fmaf(x[k], p.scale_log2, -u), b = fmaf(x[k + 1], p.scale_log2, -u);
+          if (p.scale_log2 <= 0.0f && !whole) {
+            if (x[k] == -INFINITY) a = -INFINITY;
+            if (x[k + 1] == -INFINITY) b = -INFINITY;
+          }
+          a = exp2_fast(a);
+          b = exp2_fast(b);
+          sum[i & 3] += a + b;
+          w[i] = pack2<T>(a, b);
+        }
+        tmem_st32(sp + 32 * c, w);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_wait_st();
+      tc5::fence_before();
+      tc5::bar_arrive(P_FULL(j & 1));
+      if (last) {
+        if (!tc5::bar_wait(PV_DONE, j & 1)) {
+          if (lane == 0) fail();
+          break;
+        }
+        tc5::fence_after();
+        float* slot = p.tile_part + (int64_t)((int)blockIdx.x + seg) * (kTileRows * (DP + 2));
+        const int mt = seg % p.tile_segs;
+        const bool in = mt * kTileRows + tid < (int)p.a.tokens * p.group;
+        if (in) *reinterpret_cast<float2*>(slot + 2 * tid) = make_float2(m, l);
+#pragma unroll 1
+        for (int c = 0; c < DP / 32; c++) {
+          float o[32];
+          tmem_ld32(tmem + lanes + kColO + 32 * c, o);
+          tc5::wait_ld();
+          if (in) {
+            float4* dst = reinterpret_cast<float4*>(slot + 2 * kTileRows + tid * DP + 32 * c);
+#pragma unroll
+            for (int i = 0; i < 8; i++) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+        }
+        tc5::fence_before();
+      }
+    }
+  }
+  tc5::fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc5::fence_after();
+    tc5::dealloc(tmem, 512);
+  }
 }
 
 // Adds the parts of each row (query head of a token): one warp a row.
@@ -523,30 +935,43 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
   if (b < 0) return;  // no sequence owns the row
   const int total = p.plan[0], W = p.plan[1];
   // The row's place among the sequence's own rows, and among all rows for the prefix.
-  int w0[2], count[2], slot0[2], rr[2];
+  int count[2], rr[2];
+  const float* slot0[2];
+  const bool with_prefix = sees_prefix(p, pl, b) && p.prefix > 0;
 #pragma unroll
   for (int k = 0; k < 2; k++) {
-    const int s = k ? B : b, r = (k ? token : token - pl.q0[b]) * p.group + head - g * p.group, mb = r / kRows;
+    const int s = k ? B : b, r = (k ? token : token - pl.q0[b]) * p.group + head - g * p.group;
+    count[k] = rr[k] = 0;
+    slot0[k] = nullptr;
+    if (k && !with_prefix) continue;
+    if (k && p.on_tiles) {
+      const int mt = r / kTileRows, seg = g * p.tile_segs + mt, w = part_of(p.tiles_total, p.tile_parts, seg * p.tiles_each);
+      rr[k] = r - mt * kTileRows;
+      count[k] = part_of(p.tiles_total, p.tile_parts, (seg + 1) * p.tiles_each - 1) - w + 1;
+      slot0[k] = p.tile_part + (int64_t)(w + seg) * (kTileRows * (DP + 2));
+      continue;
+    }
+    const int mb = r / kRows;
     int mbs;
     const int nt = seq_tiles(p, pl, s, B, &mbs);
+    if (!nt) continue;
+    const int t0 = pl.tiles[s] + (mb * H + g) * nt, w = part_of(total, W, t0);
     rr[k] = r - mb * kRows;
-    const int t0 = pl.tiles[s] + (mb * H + g) * nt;
-    w0[k] = nt ? part_of(total, W, t0) : 0;
-    count[k] = nt ? part_of(total, W, t0 + nt - 1) - w0[k] + 1 : 0;
-    slot0[k] = w0[k] + pl.segs[s] + mb * H + g;
+    count[k] = part_of(total, W, t0 + nt - 1) - w + 1;
+    slot0[k] = p.part + (int64_t)(w + pl.segs[s] + mb * H + g) * (kRows * (DP + 2));
   }
   const int parts = count[0] + count[1];
-  constexpr int64_t kSlot = kRows * (DP + 2);
-  auto at = [&](int i, int& r) {
-    const int k = i >= count[0];
-    r = rr[k];
-    return p.part + (int64_t)(slot0[k] + i - (k ? count[0] : 0)) * kSlot;
+  // Part i's (m, l) of the row, and its o.
+  auto at = [&](int i, const float*& o) {
+    const int k = i >= count[0], rows = k && p.on_tiles ? kTileRows : kRows;
+    const float* s = slot0[k] + (int64_t)(i - (k ? count[0] : 0)) * (rows * (DP + 2));
+    o = s + 2 * rows + rr[k] * DP;
+    return s + 2 * rr[k];
   };
   float m = -INFINITY;
   for (int i = lane; i < parts; i += 32) {
-    int r;
-    const float* s = at(i, r);
-    m = fmaxf(m, s[2 * r]);
+    const float* o;
+    m = fmaxf(m, *at(i, o));
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
@@ -557,16 +982,16 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
   for (int i0 = 0; i0 < parts; i0 += 32) {
     float f = 0.0f;
     if (i0 + lane < parts) {
-      int r;
-      const float* s = at(i0 + lane, r);
-      f = exp2_fast(s[2 * r] - um);
-      l += f * s[2 * r + 1];
+      const float* o;
+      const float2 ml = *reinterpret_cast<const float2*>(at(i0 + lane, o));
+      f = exp2_fast(ml.x - um);
+      l += f * ml.y;
     }
     const int n = min(32, parts - i0);
 #pragma unroll 4
     for (int i = 0; i < n; i++) {
-      int r;
-      const float* s = at(i0 + i, r) + 2 * kRows + r * DP;
+      const float* s;
+      at(i0 + i, s);
       const float fi = __shfl_sync(0xffffffffu, f, i);
 #pragma unroll
       for (int e = 0; e < DP / 32; e++) acc[e] = fmaf(fi, s[lane + 32 * e], acc[e]);
@@ -583,8 +1008,27 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     p.a.lse[token * p.a.lse_tok + head] = l == 0.0f ? -INFINITY : (um + log2f(l)) * 0.69314718055994531f;
 }
 
-int padded_dim(int64_t d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : 256; }
+int padded_dim(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 int part_warps(int dp) { return dp == 256 ? 4 : 8; }
+
+// Keys of a tile of the prefix kernel.
+int tile_keys(int dp) { return dp == 256 ? 64 : 128; }
+// Where the prefix goes to the tensor cores' own tiles.
+bool use_tiles(const vtq_attention_args& a) {
+  const int64_t rows = a.tokens * (a.heads / a.kv.kv_heads), prefix = std::min(a.shared_len, a.kv.table_width * a.kv.page_size);
+  return rows > 16 && prefix >= 512;
+}
+int64_t tile_total(const vtq_attention_args& a) {
+  const int64_t rows = a.tokens * (a.heads / a.kv.kv_heads), prefix = std::min(a.shared_len, a.kv.table_width * a.kv.page_size);
+  const int keys = tile_keys(padded_dim(a.kv.head_dim));
+  return a.kv.kv_heads * ((rows + kTileRows - 1) / kTileRows) * ((prefix + keys - 1) / keys);
+}
+size_t tile_bytes(const vtq_attention_args& a) {
+  if (!use_tiles(a)) return 0;
+  const int64_t rows = a.tokens * (a.heads / a.kv.kv_heads);
+  const int64_t slots = std::min<int64_t>(tile_total(a), num_sms()) + a.kv.kv_heads * ((rows + kTileRows - 1) / kTileRows);
+  return (size_t)slots * kTileRows * (padded_dim(a.kv.head_dim) + 2) * 4;
+}
 
 size_t plan_bytes(const vtq_attention_args& a) {
   return ((size_t)(plan_ints((int)a.kv.seqs) + a.tokens) * 4 + 255) / 256 * 256;
@@ -592,7 +1036,13 @@ size_t plan_bytes(const vtq_attention_args& a) {
 // Segments of any lengths: each sequence's rows and, once more, all rows for the prefix.
 int64_t most_segments(const vtq_attention_args& a) {
   const int64_t group = a.heads / a.kv.kv_heads, rows = a.tokens * group;
-  return (rows / kRows + a.kv.seqs + (a.shared_len ? (rows + kRows - 1) / kRows : 0)) * a.kv.kv_heads;
+  return (rows / kRows + a.kv.seqs + (a.shared_len && !use_tiles(a) ? (rows + kRows - 1) / kRows : 0)) * a.kv.kv_heads;
+}
+
+size_t part_bytes(const vtq_attention_args& a) {
+  const int dp = padded_dim(a.kv.head_dim);
+  const int64_t slots = most_segments(a) + (int64_t)num_sms() * part_warps(dp);
+  return ((size_t)slots * kRows * (dp + 2) * 4 + 255) / 256 * 256;
 }
 
 vtq_status check(const char* fn, const vtq_attention_args* a) {
@@ -605,7 +1055,7 @@ vtq_status check(const char* fn, const vtq_attention_args* a) {
   if (a->tokens > (1 << 20) || a->heads > 65536 || a->kv.table_width * a->kv.page_size > INT32_MAX / 2)
     return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "%s: not implemented (over 2^20 tokens, 2^16 heads or 2^30 positions)", fn);
   const int64_t tiles = (a->kv.table_width * a->kv.page_size + 15) / 16 + 1;
-  if (most_segments(*a) * tiles > INT32_MAX)
+  if (most_segments(*a) * tiles > INT32_MAX || tile_total(*a) > INT32_MAX)
     return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "%s: not implemented (query rows times table positions over 2^35)", fn);
   return VTQ_OK;
 }
@@ -617,17 +1067,31 @@ cudaError_t launch(const AttnParams& p, cudaStream_t st) {
                       (size_t)WARPS * KT * sizeof(longlong2);
   cudaError_t e = cudaFuncSetAttribute(part, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
+  constexpr int TKT = DP == 256 ? 64 : 128, TST = DP == 64 ? 5 : DP == 128 ? 3 : 2;
+  if (p.on_tiles) {
+    auto tiles = attention_tile_kernel<T, DP, TKT, TST>;
+    constexpr size_t tile_smem = TileShape<T, DP, TKT, TST>::SMEM;
+    if ((e = cudaFuncSetAttribute(tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tile_smem)) != cudaSuccess) return e;
+    kernel_launch_count()++;
+    tiles<<<(unsigned)p.tile_parts, kTileThreads, tile_smem, st>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  }
   kernel_launch_count() += 2;
-  part<<<(unsigned)(p.parts / WARPS), 32 * WARPS, smem, st>>>(p);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  // Each waits for the one before at its own point (griddepcontrol): the part kernel at its end.
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.a.tokens * p.a.heads + 3) / 4));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3((unsigned)(p.parts / WARPS));
+  cfg.blockDim = dim3(32 * WARPS);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
+  cfg.numAttrs = p.on_tiles && pdl_enabled() ? 1 : 0;
+  if ((e = cudaLaunchKernelEx(&cfg, part, p)) != cudaSuccess) return e;
+  cfg.gridDim = dim3((unsigned)((p.a.tokens * p.a.heads + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, attention_join_kernel<T, DP>, p);
 }
@@ -636,7 +1100,6 @@ template <typename T>
 cudaError_t launch_dim(AttnParams& p, cudaStream_t st) {
   switch (p.dim_padded) {
     case 64: return launch<T, 64, 32, 8, 3>(p, st);
-    case 96: return launch<T, 96, 16, 8, 3>(p, st);
     case 128: return launch<T, 128, 16, 8, 3>(p, st);
     default: return launch<T, 256, 16, 4, 3>(p, st);
   }
@@ -651,9 +1114,7 @@ extern "C" {
 
 size_t vtq_attention_paged_workspace_bytes(const vtq_attention_args* a) {
   if (check("vtq_attention_paged", a) || a->tokens == 0 || a->kv.seqs == 0) return 0;
-  const int dp = padded_dim(a->kv.head_dim);
-  const int64_t slots = most_segments(*a) + (int64_t)num_sms() * part_warps(dp);
-  return plan_bytes(*a) + (size_t)slots * kRows * (dp + 2) * 4;
+  return plan_bytes(*a) + part_bytes(*a) + tile_bytes(*a);
 }
 
 vtq_status vtq_attention_paged(const vtq_attention_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -664,7 +1125,7 @@ vtq_status vtq_attention_paged(const vtq_attention_args* a, void* ws, size_t ws_
   const size_t need = vtq_attention_paged_workspace_bytes(a);
   if (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255u))
     return serve_fail(VTQ_ERR_INVALID_ARG, "%s: workspace missing, too small or not 256-byte aligned", fn);
-  AttnParams p;
+  AttnParams p = {};
   p.a = *a;
   p.group = (int)(a->heads / a->kv.kv_heads);
   p.dim_padded = padded_dim(a->kv.head_dim);
@@ -676,6 +1137,16 @@ vtq_status vtq_attention_paged(const vtq_attention_args* a, void* ws, size_t ws_
   p.q_wide = (reinterpret_cast<uintptr_t>(a->q) & 3u) == 0 && a->q_tok % 2 == 0 && a->q_head % 2 == 0;
   p.plan = static_cast<int*>(ws);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan_bytes(*a));
+  p.on_tiles = use_tiles(*a);
+  if (p.on_tiles) {
+    const int keys = tile_keys(p.dim_padded);
+    p.q_copies = aligned16(a->q) && a->q_tok % 8 == 0 && a->q_head % 8 == 0;
+    p.tile_segs = (int)((a->tokens * p.group + kTileRows - 1) / kTileRows);
+    p.tiles_each = (p.prefix + keys - 1) / keys;
+    p.tiles_total = (int)tile_total(*a);
+    p.tile_parts = std::min(p.tiles_total, num_sms());
+    p.tile_part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.part) + part_bytes(*a));
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return serve_cuda(a->kv.dtype == VTQ_F16 ? launch_dim<__half>(p, st) : launch_dim<__nv_bfloat16>(p, st), fn);
 }

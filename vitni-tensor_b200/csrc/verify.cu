@@ -31,6 +31,7 @@ namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kStrips = 8, kBlock = 32 * kStrips;  // elements summed by one warp at a time
+static_assert(kWarps >= 4 && kWarps <= 32, "the joins below take one warp a row and one lane a warp");
 
 struct VerifyParams {
   const int32_t* draft;
@@ -53,12 +54,38 @@ __device__ __forceinline__ int draft_count(const VerifyParams& a, int b) {
   return a.n_draft ? min(max(a.n_draft[b], 0), a.K) : a.K;
 }
 
-// What is left of p at one token after q: r of the header comment. NaN counts as nothing.
+// What is left of p at one token after q: r of the header comment, as its 32-bit value and that
+// value's own rounding error (together exact). NaN counts as nothing. A conversion of each value to 64
+// bits instead takes the conversion unit's whole time: 109 us where this form takes a quarter of it
+// (128 rows of 100003 tokens).
+struct Left {
+  float r, e;
+};
 template <typename T>
-__device__ __forceinline__ double left(const T* p, const T* q, int64_t v, int64_t only, bool sub) {
-  double r = (double)to_f32(p[v]);
-  if (sub) r -= q ? (double)to_f32(q[v]) : (v == only ? 1.0 : 0.0);
-  return r > 0.0 ? r : 0.0;
+__device__ __forceinline__ Left left(float p, float q) {
+  Left w;
+  w.r = __fsub_rn(p, q);
+  if (!(w.r > 0.0f)) return Left{0.0f, 0.0f};
+  const float t = __fsub_rn(w.r, p);
+  w.e = __fsub_rn(__fsub_rn(p, __fsub_rn(w.r, t)), __fadd_rn(q, t));
+  return w;
+}
+// The kStrips values at e0, e0 + 32, ..: nothing behind v1.
+template <typename T>
+__device__ __forceinline__ void left_strips(const T* p, const T* q, int64_t e0, int64_t v1, int64_t only, bool sub,
+                                            Left (&r)[kStrips]) {
+  float a[kStrips], b[kStrips];
+#pragma unroll
+  for (int k = 0; k < kStrips; k++) {
+    const bool in = e0 + 32 * k < v1;
+    a[k] = in ? to_f32(p[e0 + 32 * k]) : 0.0f;
+    b[k] = in && sub && q ? to_f32(q[e0 + 32 * k]) : 0.0f;
+  }
+#pragma unroll
+  for (int k = 0; k < kStrips; k++) {
+    if (sub && e0 + 32 * k == only) b[k] = 1.0f;
+    r[k] = left<T>(a[k], b[k]);
+  }
 }
 
 __device__ __forceinline__ double warp_sum(double s) {
@@ -78,7 +105,7 @@ __device__ __forceinline__ double warp_scan(double s, int lane) {
 // One cluster a sequence. CTA c of the cluster owns the blocks of kBlock
 // tokens [c nb, (c + 1) nb).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_draft_kernel(const VerifyParams a, int nb) {
+__global__ void __launch_bounds__(kThreads, 2) verify_draft_kernel(const VerifyParams a, int nb) {
   extern __shared__ double sums[];  // nb: block sums, then their inclusive scan
   __shared__ int s_acc;
   __shared__ double s_total, s_warp[kWarps];
@@ -128,16 +155,18 @@ __global__ void __launch_bounds__(kThreads) verify_draft_kernel(const VerifyPara
     int64_t last = -1;  // the last token that has any weight
     for (int j = warp; j < mine; j += kWarps) {
       const int64_t e0 = v0 + (int64_t)j * kBlock + lane;
-      double r[kStrips];
-#pragma unroll
-      for (int k = 0; k < kStrips; k++) r[k] = e0 + 32 * k < v1 ? left(p, q, e0 + 32 * k, only, sub) : 0.0;
-      double s = 0.0;
+      Left r[kStrips];
+      left_strips(p, q, e0, v1, only, sub, r);
+      // This lane's sum as a 32-bit value and what its roundings lost: 2^-48 of it.
+      float hi = 0.0f, lo = 0.0f;
 #pragma unroll
       for (int k = 0; k < kStrips; k++) {
-        s += r[k];
-        if (r[k] > 0.0) last = e0 + 32 * k;
+        const float s = __fadd_rn(hi, r[k].r), t = __fsub_rn(s, hi);
+        lo = __fadd_rn(lo, __fadd_rn(__fadd_rn(__fsub_rn(hi, __fsub_rn(s, t)), __fsub_rn(r[k].r, t)), r[k].e));
+        hi = s;
+        if (r[k].r > 0.0f) last = e0 + 32 * k;
       }
-      s = warp_sum(s);
+      const double s = warp_sum((double)hi + (double)lo);
       if (lane == 0) sums[j] = s;
     }
 #pragma unroll
@@ -210,14 +239,13 @@ __global__ void __launch_bounds__(kThreads) verify_draft_kernel(const VerifyPara
         for (int j = lo; j >= 0 && tail < 0; j--) {
           double cum = j ? sums[j - 1] : 0.0;
           const int64_t e0 = v0 + (int64_t)j * kBlock + lane;
-          double r[kStrips];
-#pragma unroll
-          for (int k = 0; k < kStrips; k++) r[k] = e0 + 32 * k < v1 ? left(p, q, e0 + 32 * k, only, sub) : 0.0;
+          Left r[kStrips];
+          left_strips(p, q, e0, v1, only, sub, r);
 #pragma unroll
           for (int k = 0; k < kStrips; k++) {
-            const double c = warp_scan(r[k], lane);
-            const unsigned over = __ballot_sync(0xffffffffu, r[k] > 0.0 && start + (cum + c) > cut);
-            const unsigned some = __ballot_sync(0xffffffffu, r[k] > 0.0);
+            const double c = warp_scan((double)r[k].r + (double)r[k].e, lane);
+            const unsigned over = __ballot_sync(0xffffffffu, r[k].r > 0.0f && start + (cum + c) > cut);
+            const unsigned some = __ballot_sync(0xffffffffu, r[k].r > 0.0f);
             if (found < 0 && over) found = e0 - lane + 32 * k + __ffs(over) - 1;
             if (some) tail = e0 - lane + 32 * k + 31 - __clz(some);
             cum += __shfl_sync(0xffffffffu, c, 31);
@@ -231,18 +259,23 @@ __global__ void __launch_bounds__(kThreads) verify_draft_kernel(const VerifyPara
   }
 }
 
-// The order of a row's argmax: larger first, then the lower index. NaN is never larger, and a NaN at
-// index 0 is never passed (the order of the decode loop's own argmax).
-__device__ __forceinline__ bool better(float v, int64_t i, float best, int64_t at) {
-  return v > best || (v == best && i < at);
+// A row's argmax as the larger of 64-bit keys: the value's bits, put in the order of the values, above
+// the complement of the index, so that the lower index wins a tie. NaN is never larger (key 0), and a
+// NaN at index 0 is never passed (the order of the decode loop's own argmax).
+__device__ __forceinline__ void take(float x, uint32_t v, uint32_t& hi, uint32_t& lo) {
+  const uint32_t bits = __float_as_uint(__fadd_rn(x, 0.0f));  // -0 is 0
+  uint32_t k = bits ^ ((int32_t)bits < 0 ? 0xffffffffu : 0x80000000u);
+  if (x != x) k = v == 0 ? 0xffffffffu : 0u;
+  const uint32_t i = ~v;
+  if (k > hi || (k == hi && i > lo)) hi = k, lo = i;
 }
+
+constexpr int kGroup = 4;  // rows looked at together: a chain of drafts waits for two groups, not eight rows
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) verify_greedy_kernel(const VerifyParams a) {
-  __shared__ float s_v[2][kWarps];
-  __shared__ int64_t s_i[2][kWarps];
-  __shared__ float s_best[2];
-  __shared__ int64_t s_at[2];
+  __shared__ uint2 s_warp[kGroup][kWarps];
+  __shared__ uint2 s_key[2][kGroup];  // two sets: a CTA may be one group ahead of another's reads
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), size = (int)cl.num_blocks();
   const int b = blockIdx.x / size;
@@ -251,61 +284,77 @@ __global__ void __launch_bounds__(kThreads) verify_greedy_kernel(const VerifyPar
   const int32_t* draft = a.draft + (int64_t)b * a.ld_draft;
   int32_t* out = a.tokens + (int64_t)b * a.ld_tokens;
   const int n = draft_count(a, b);
+  const uint32_t V = (uint32_t)a.V, step = (uint32_t)(size * kThreads);
   int acc = 0;
   int32_t token = 0;
-  for (;; acc++) {
+  for (int set = 0;; set ^= 1) {
+    const int rows = min(kGroup, n + 1 - acc);
+    uint32_t hi[kGroup], lo[kGroup];
+#pragma unroll
+    for (int r = 0; r < kGroup; r++) hi[r] = lo[r] = 0;
     const T* p = P + acc * a.p_row;
-    float best = -INFINITY;
-    int64_t at = INT64_MAX;
-    for (int64_t v0 = (int64_t)rank * kThreads + tid; v0 < a.V; v0 += (int64_t)size * kThreads * 8) {
-      float x[8];
+    for (uint32_t v0 = (uint32_t)(rank * kThreads + tid); v0 < V; v0 += step * 4) {
+      float x[kGroup][4];
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const int64_t v = v0 + (int64_t)k * size * kThreads;
-        x[k] = v < a.V ? to_f32(p[v]) : -INFINITY;
-      }
+      for (int r = 0; r < kGroup; r++)
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const int64_t v = v0 + (int64_t)k * size * kThreads;
-        if (v < a.V && better(x[k], v, best, at)) best = x[k], at = v;
-      }
+        for (int k = 0; k < 4; k++) {
+          const uint32_t v = v0 + k * step;
+          x[r][k] = r < rows && v < V ? to_f32(p[r * a.p_row + v]) : __uint_as_float(0x7fc00000u);
+        }
+#pragma unroll
+      for (int r = 0; r < kGroup; r++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const uint32_t v = v0 + k * step;
+          if (v < V) take(x[r][k], v, hi[r], lo[r]);
+        }
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float ov = __shfl_xor_sync(0xffffffffu, best, o);
-      const int64_t oi = __shfl_xor_sync(0xffffffffu, at, o);
-      if (better(ov, oi, best, at)) best = ov, at = oi;
+    for (int r = 0; r < kGroup; r++) {
+      const uint32_t m = __reduce_max_sync(0xffffffffu, hi[r]);
+      const uint32_t i = __reduce_max_sync(0xffffffffu, hi[r] == m ? lo[r] : 0u);
+      if (lane == 0) s_warp[r][warp] = make_uint2(m, i);
     }
-    const int s = acc & 1;  // two sets: a CTA may be one row ahead of another's reads
-    if (lane == 0) s_v[s][warp] = best, s_i[s][warp] = at;
     __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < kWarps; w++)
-        if (better(s_v[s][w], s_i[s][w], best, at)) best = s_v[s][w], at = s_i[s][w];
-      s_best[s] = best;
-      s_at[s] = at;
+    if (warp < kGroup) {
+      const uint2 k = lane < kWarps ? s_warp[warp][lane] : make_uint2(0, 0);
+      const uint32_t m = __reduce_max_sync(0xffffffffu, k.x);
+      const uint32_t i = __reduce_max_sync(0xffffffffu, k.x == m ? k.y : 0u);
+      if (lane == 0) s_key[set][warp] = make_uint2(m, i);
     }
     cl.sync();
-    for (int c = 0; c < size; c++) {
-      const float ov = *cl.map_shared_rank(&s_best[s], c);
-      const int64_t oi = *cl.map_shared_rank(&s_at[s], c);
-      if (c == 0 || better(ov, oi, best, at)) best = ov, at = oi;
+    // Every warp of every CTA joins the same keys: lane = (CTA, row).
+    uint2 k = make_uint2(0, 0);
+    if (lane < size * kGroup) k = cl.map_shared_rank(&s_key[set][0], lane / kGroup)[lane % kGroup];
+#pragma unroll
+    for (int o = kGroup; o < 32; o <<= 1) {
+      const uint32_t oh = __shfl_xor_sync(0xffffffffu, k.x, o), ol = __shfl_xor_sync(0xffffffffu, k.y, o);
+      if (oh > k.x || (oh == k.x && ol > k.y)) k = make_uint2(oh, ol);
     }
-    const float first = to_f32(p[0]);
-    token = first != first || at == INT64_MAX ? 0 : (int32_t)at;
-    if (acc == n || draft[acc] != token) break;
+    const int32_t best = k.x ? (int32_t)~k.y : 0;  // of row acc + lane % kGroup; nothing but NaN: 0
+    const int r = lane % kGroup;
+    const bool keep = r < rows && acc + r < n && draft[acc + r] == best;
+    const unsigned gone = ~__ballot_sync(0xffffffffu, keep) & ((1u << kGroup) - 1);
+    if (gone) {
+      const int first = __ffs(gone) - 1;
+      acc += first;
+      token = __shfl_sync(0xffffffffu, best, first);
+      break;
+    }
+    acc += kGroup;
   }
   if (rank == 0) {
     for (int i = tid; i <= a.K; i += kThreads) out[i] = i < acc ? draft[i] : i == acc ? token : -1;
     if (tid == 0) a.accepted[b] = acc;
   }
-  cl.sync();  // no CTA leaves while another still reads its best
+  cl.sync();  // no CTA leaves while another still reads its keys
 }
 
-// CTAs a sequence: enough that all SMs read, each with some thousand tokens of its own.
+// CTAs a sequence: enough that every SM holds a few, each with some thousand tokens of its own.
 int cluster_size(int64_t seqs, int64_t V) {
   int c = 1;
-  while (c < 8 && seqs * c < num_sms() && V > (int64_t)c * 4096) c *= 2;
+  while (c < 8 && seqs * c < 3 * num_sms() && V > (int64_t)c * 2048) c *= 2;
   return c;
 }
 
