@@ -42,8 +42,10 @@ struct AttnParams {
   int dim_padded;
   // The prefix on the tensor cores' own tiles (attention_tile_kernel), where on_tiles is set:
   bool on_tiles, q_copies;           // q_copies: q rows can be copied 16 bytes at a time
-  int tile_segs, tiles_each;         // blocks of kTileRows rows of a kv head, key tiles of each
-  int tiles_total, tile_parts;       // in all; CTAs that share them
+  int tile_box;                      // positions of a TMA box: a page, or an even part of it; 0: none
+  int tile_rt, tile_streams;         // blocks of kTileRows rows of a segment; softmax warpgroups of a CTA
+  int tile_segs, tiles_each;         // segments of a kv head, steps (of tile_streams / tile_rt key tiles) of each
+  int tiles_total, tile_parts;       // steps in all; CTAs that share them
   float* tile_part;                  // slots of kTileRows (m, l) and o
 };
 
@@ -526,25 +528,30 @@ __global__ void __launch_bounds__(32 * WARPS, 1) attention_part_kernel(const __g
 
 // ---- the prefix on tcgen05 ----
 //
-// One CTA takes 128 query rows (heads of a kv head, tokens of all sequences) over a run of key tiles:
-//   warps 0-3  softmax: a thread a row. S from TMEM, weights back into TMEM as the second product's A.
-//   warps 4-7  loaders: pages gathered with 16-byte copies into swizzled tiles, STAGES deep
-//   warp 8     one thread issues S = Q K^T (K tile: N = KT keys) and O += P V (V as it lies: N-major)
-// S is double-buffered, so the next tile's first product runs beside the softmax of this one. O stays in
-// TMEM; it is scaled again only where a row's maximum has grown by more than 2^8 since the last time, until
-// then the weights are taken relative to the old one (at most 256, and l with them).
+// A CTA runs STREAMS streams of one softmax warpgroup each over a run of key tiles. With RT = 2 the
+// streams are two blocks of 128 query rows that share every key tile; with RT = 1 they are the even and
+// the odd key tiles of one block (two parts of the same rows, joined later), so that a stream's softmax
+// always runs beside the other stream's products.
+//   softmax warpgroups  a thread a row: S from TMEM, the weights back into TMEM as the second product's A
+//   3 loader warps      pages into a ring of swizzled K and V tiles, by TMA where a page holds 4 positions
+//                       or more (gathering rows with 16-byte copies takes three warps 5700 cycles a tile,
+//                       twice what the softmax needs)
+//   1 warp              one thread issues S = Q K^T (N = KT keys) and O += P V (V as it lies: N-major)
+// O stays in TMEM; it is scaled again only where a row's maximum has grown by more than 2^8 since the
+// last time, until then the weights are taken relative to the old one (at most 256, and l with them).
+// Head dims over 128 have room in TMEM for one stream; its S is double-buffered instead.
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one));
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc));
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one));
 }
 // N-major operand, 128-byte swizzle: 64 values of N a row of 128 bytes, 8 rows (K) an atom of 1024;
 // `chunk` bytes to the next 64 values of N, 1024 to the next 8 of K.
@@ -573,269 +580,450 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* u) {
       "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(u[0]),
+      "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]),
+      "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(addr)
+      : "memory");
+}
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-constexpr int kTileThreads = 288;
-
-template <typename T, int DP, int KT, int STAGES>
+template <typename T, int DP, int KT, int RT, int STREAMS, int NSLOT>
 struct TileShape {
-  static constexpr uint32_t Q_BYTES = kTileRows * DP * 2, KV_BYTES = KT * DP * 2, STAGE = 2 * KV_BYTES;
-  static constexpr size_t SMEM = Q_BYTES + STAGES * STAGE + 1024;
+  static constexpr uint32_t Q_TILE = kTileRows * DP * 2, Q_BYTES = RT * Q_TILE, SLOT = KT * DP * 2;
+  static constexpr int THREADS = STREAMS * 128 + 128;
+  static constexpr size_t SMEM = Q_BYTES + NSLOT * SLOT + 1024;
 };
+constexpr int kLoaders = 3, kMasks = 8;
+static_assert(2 * kMasks > 8 + 1, "a mask's place must not come round before its tile's V slot has");
 
-template <typename T, int DP, int KT, int STAGES>
-__global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const __grid_constant__ AttnParams p) {
-  using L = TileShape<T, DP, KT, STAGES>;
+template <typename T, int DP, int KT, int RT, int STREAMS, int NSLOT>
+__global__ void __launch_bounds__(TileShape<T, DP, KT, RT, STREAMS, NSLOT>::THREADS, 1)
+    attention_tile_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap tmk,
+                          const __grid_constant__ CUtensorMap tmv) {
+  using L = TileShape<T, DP, KT, RT, STREAMS, NSLOT>;
   constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
   constexpr uint32_t kIdescS = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((uint32_t)(KT >> 3) << 17) | (8u << 24);
   constexpr uint32_t kIdescO = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | (8u << 24);
-  constexpr uint32_t kColO = 2 * KT;  // columns: S / P twice, then O
-  static_assert(2 * KT + DP <= 512, "TMEM");
+  constexpr int TPS = STREAMS / RT;   // key tiles of a step: 2 where the streams are the tiles
+  constexpr uint32_t kColO = 2 * KT;  // columns: S / P twice, then each stream's O
+  constexpr int kGroups = KT / 4;     // of 4 keys: loader lw copies groups lw, lw + 3, ..
+  static_assert(2 * KT + STREAMS * DP <= 512 && NSLOT <= 8 && RT <= STREAMS, "TMEM, masks");
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t s_bar[4 * STAGES + 7];
-  __shared__ uint32_t s_valid[STAGES][4];
+  __shared__ __align__(8) uint64_t s_bar[2 * NSLOT + 8 + kMasks];
+  __shared__ uint32_t s_valid[kMasks][kLoaders][2];
   __shared__ uint32_t s_slot;
   __shared__ int s_abort, s_any;
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = base + L::Q_BYTES;
   uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
   auto bar = [&](int i) { return smem_u32(&s_bar[i]); };
-  auto K_FULL = [&](int s) { return bar(s); };
-  auto V_FULL = [&](int s) { return bar(STAGES + s); };
-  auto K_EMPTY = [&](int s) { return bar(2 * STAGES + s); };
-  auto V_EMPTY = [&](int s) { return bar(3 * STAGES + s); };
-  auto S_FULL = [&](int s) { return bar(4 * STAGES + s); };
-  auto P_FULL = [&](int s) { return bar(4 * STAGES + 2 + s); };
-  const uint32_t Q_FULL = bar(4 * STAGES + 4), Q_EMPTY = bar(4 * STAGES + 5), PV_DONE = bar(4 * STAGES + 6);
+  auto FULL = [&](int s) { return bar(s); };
+  auto EMPTY = [&](int s) { return bar(NSLOT + s); };
+  auto S_FULL = [&](int s) { return bar(2 * NSLOT + s); };      // of an S buffer: a stream's, or tile parity
+  auto P_FULL = [&](int s) { return bar(2 * NSLOT + 2 + s); };
+  auto PV_DONE = [&](int r) { return bar(2 * NSLOT + 4 + r); };  // of a stream
+  const uint32_t Q_FULL = bar(2 * NSLOT + 6), Q_EMPTY = bar(2 * NSLOT + 7);
+  auto MASK = [&](int i) { return bar(2 * NSLOT + 8 + i); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int B = (int)p.a.kv.seqs, D = (int)p.a.kv.head_dim;
   volatile int* abort_flag = &s_abort;
 
   tc5::grid_release();
   if (tid == 0) {
-    for (int s = 0; s < STAGES; s++) {
-      tc5::bar_init(K_FULL(s), 128);
-      tc5::bar_init(V_FULL(s), 128);
-      tc5::bar_init(K_EMPTY(s), 1);
-      tc5::bar_init(V_EMPTY(s), 1);
+    for (int s = 0; s < NSLOT; s++) {
+      tc5::bar_init(FULL(s), 32 * kLoaders);
+      tc5::bar_init(EMPTY(s), 1);
     }
     for (int s = 0; s < 2; s++) {
       tc5::bar_init(S_FULL(s), 1);
       tc5::bar_init(P_FULL(s), 128);
+      tc5::bar_init(PV_DONE(s), 1);
     }
-    tc5::bar_init(Q_FULL, 128);
+    tc5::bar_init(Q_FULL, 32 * kLoaders);
     tc5::bar_init(Q_EMPTY, 1);
-    tc5::bar_init(PV_DONE, 1);
+    for (int i = 0; i < kMasks; i++) tc5::bar_init(MASK(i), kLoaders);
     *abort_flag = 0;
     s_any = 0;
     fence_mbar_init();
   }
-  if (warp == 8) tc5::alloc(smem_u32(&s_slot), 512);
+  constexpr int kMmaWarp = 4 * STREAMS + kLoaders;
+  if (warp == kMmaWarp) tc5::alloc(smem_u32(&s_slot), 512);
   __syncthreads();
   // Nothing to do where no sequence sees the prefix (its pages need not exist then).
-  for (int b = tid; b < B; b += kTileThreads) {
-    const int T_ = (int)p.a.tokens;
-    const int q0 = p.a.q_start ? min(max(p.a.q_start[b], 0), T_) : b, q1 = p.a.q_start ? min(max(p.a.q_start[b + 1], 0), T_) : b + 1;
+  for (int b = tid; b < B; b += L::THREADS) {
+    const int n = (int)p.a.tokens;
+    const int q0 = p.a.q_start ? min(max(p.a.q_start[b], 0), n) : b, q1 = p.a.q_start ? min(max(p.a.q_start[b + 1], 0), n) : b + 1;
     if (q1 > q0 && p.a.kv_len[b] - (q1 - q0) + 1 >= p.prefix) s_any = 1;
   }
   tc5::fence_before();
   __syncthreads();
   tc5::fence_after();
   const uint32_t tmem = s_slot;
-  const int tile0 = first_tile(p.tiles_total, p.tile_parts, (int)blockIdx.x);
-  const int tile1 = s_any ? first_tile(p.tiles_total, p.tile_parts, (int)blockIdx.x + 1) : tile0;
+  // Steps [step0, step1) of all segments; a segment is (kv head g, block of RT x 128 rows).
+  const int step0 = first_tile(p.tiles_total, p.tile_parts, (int)blockIdx.x);
+  const int steps = s_any ? first_tile(p.tiles_total, p.tile_parts, (int)blockIdx.x + 1) - step0 : 0;
+  const int each = p.tiles_each, rows = (int)p.a.tokens * p.group;
   auto fail = [&]() {
     if (p.a.status) atomicOr(p.a.status, KERR_TIMEOUT);
     *abort_flag = 1;
   };
-  // Bytes into a K, V or Q tile of `rows` rows: blocks of 64 values, 128-byte rows, 16-byte chunks swizzled.
-  auto place = [](int rows, int row, int chunk) {
-    return (uint32_t)((chunk >> 3) * rows * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+  // Whether stream r has rows in a segment.
+  auto live = [&](int seg, int r) { return RT == 1 || ((seg % p.tile_segs) * RT + r) * kTileRows < rows; };
+  // Bytes into a K, V or Q tile of `n` rows: blocks of 64 values, 128-byte rows, 16-byte chunks swizzled.
+  auto place = [](int n, int row, int chunk) {
+    return (uint32_t)((chunk >> 3) * n * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
   };
 
-  if (warp >= 4 && warp < 8) {
-    // ---- loaders: warp lw owns 32 keys of each 128 (16 of 64), 8 lanes a row of 128 bytes ----
-    const int lw = warp - 4, mine = KT / 4;
-    const T* K = static_cast<const T*>(p.a.kv.k);
-    const T* V = static_cast<const T*>(p.a.kv.v);
-    int told = tile0;  // tiles that the consumers have been told of
-    int q_seg = -1;
-    bool q_new = false;
-    auto tell = [&](int upto) {  // every copy of tiles before `upto` has landed
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      for (; told < upto; told++) {
-        const int s = (told - tile0) % STAGES;
-        if (q_new && told == upto - 1) {
-          tc5::bar_arrive(Q_FULL);
-          q_new = false;
-        }
-        tc5::bar_arrive(K_FULL(s));
-        tc5::bar_arrive(V_FULL(s));
-      }
-    };
-    int segs_seen = 0;
-    for (int t = tile0; t < tile1 && !*abort_flag; t++) {
-      const int j = t - tile0, s = j % STAGES, seg = t / p.tiles_each, kt = t - seg * p.tiles_each;
-      const int g = seg / p.tile_segs, mt = seg - g * p.tile_segs;
-      if (seg != q_seg) {
-        // Everything before is told of first, so that the segment's first tile alone carries Q.
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        tell(t);
-        if (segs_seen && !tc5::bar_wait(Q_EMPTY, (segs_seen - 1) & 1)) {
-          if (lane == 0) fail();
-          break;
-        }
-        segs_seen++;
-        q_seg = seg;
-        q_new = true;
-        const int rows = (int)p.a.tokens * p.group;
-        for (int i = 0; i < 8; i++) {
-          const int r = lw * 32 + i * 4 + (lane >> 3);
-          const int row = mt * kTileRows + r, tok = row / p.group;
-          const bool in = row < rows;
-          const T* src = static_cast<const T*>(p.a.q) + (in ? (int64_t)tok * p.a.q_tok + (int64_t)(g * p.group + row - tok * p.group) * p.a.q_head : 0);
-#pragma unroll
-          for (int c = 0; c < DP / 64; c++) {
-            const int chunk = c * 8 + (lane & 7);
-            const bool there = in && chunk * 8 < D;
-            const uint32_t at = place(kTileRows, r, chunk);
-            if (p.q_copies) {
-              copy16(base + at, src + (there ? chunk * 8 : 0), there);
-            } else {
-              T* dst = reinterpret_cast<T*>(gbase + at);
-#pragma unroll
-              for (int e = 0; e < 8; e++) dst[e] = there ? src[chunk * 8 + e] : from_f32<T>(0.0f);
-            }
-          }
-        }
-      }
-      // This lane's key of the tile.
-      const int pos = kt * KT + lw * mine + lane;
-      int64_t ko = 0, vo = 0;
-      bool ok = false;
-      if (lane < mine && pos < p.prefix) {
-        const int page_size = (int)p.a.kv.page_size, at = pos / page_size;
-        const int64_t page = p.a.kv.table[at], slot = pos - at * page_size;
-        ok = page >= 0 && page < p.a.kv.pages;
-        if (ok) {
-          ko = page * p.a.kv.k_page + slot * p.a.kv.k_slot + g * p.a.kv.k_head;
-          vo = page * p.a.kv.v_page + slot * p.a.kv.v_slot + g * p.a.kv.v_head;
-        } else if (p.a.status) {
-          atomicOr(p.a.status, SERVE_BAD_INDEX);
-        }
-      }
-      const uint32_t valid = __ballot_sync(0xffffffffu, ok);
-      if (j >= STAGES) {
-        const uint32_t ph = ((j / STAGES) + 1) & 1;
-        if (!mbar_try_wait(&s_bar[3 * STAGES + s], ph) || !mbar_try_wait(&s_bar[2 * STAGES + s], ph)) {
-          asm volatile("cp.async.wait_group 0;" ::: "memory");
-          tell(t);
-          if (!tc5::bar_wait(K_EMPTY(s), ph) || !tc5::bar_wait(V_EMPTY(s), ph)) {
-            if (lane == 0) fail();
-            break;
-          }
-        }
-        __syncwarp();
-      }
-      if (lane == 0) s_valid[s][lw] = valid;
-      const uint32_t k_s = base + L::Q_BYTES + s * L::STAGE, v_s = k_s + L::KV_BYTES;
-#pragma unroll
-      for (int i = 0; i < KT / 16; i++) {
-        const int r = i * 4 + (lane >> 3), key = lw * mine + r;
-        const bool in = (valid >> r) & 1;
-        const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
-#pragma unroll
-        for (int c = 0; c < DP / 64; c++) {
-          const int chunk = c * 8 + (lane & 7);
-          const bool there = in && chunk * 8 < D;
-          copy16(k_s + place(KT, key, chunk), K + (there ? kr + chunk * 8 : 0), there);
-          copy16(v_s + place(KT, key, chunk), V + (there ? vr + chunk * 8 : 0), there);
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
-      tell(t);  // the tile before
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (!*abort_flag) tell(tile1);
-  } else if (warp == 8) {
-    if (lane == 0) {
+  if (warp >= 4 * STREAMS) {
+    if (warp < kMmaWarp) {
+      // ---- loaders: tile n of this CTA in ring places 2 n (K) and 2 n + 1 (V); 8 lanes a row of 128 bytes ----
+      const int lw = warp - 4 * STREAMS, sub = lane >> 3;
+      const T* K = static_cast<const T*>(p.a.kv.k);
+      const T* V = static_cast<const T*>(p.a.kv.v);
+      const int page_size = (int)p.a.kv.page_size;
+      const int box = p.tile_box, boxes = box ? KT / box : 0;  // keys of a TMA box, boxes of a tile (32 at most)
+      int told = 0;  // ring places that the consumers have been told of
+      auto tell = [&](int upto) {  // the copies of every place before `upto` have landed
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        for (; told < upto; told++) tc5::bar_arrive(FULL(told % NSLOT));
+      };
+      // This lane's two keys of a tile (rows 32 h + lane of those that this warp copies).
+      auto key_of = [&](int h) {
+        const int k = 32 * h + lane, grp = lw + kLoaders * (k >> 2);
+        return grp < kGroups ? 4 * grp + (k & 3) : -1;
+      };
+      const int key_a = key_of(0), key_b = key_of(1);
+      // The page of a position; -1 behind the prefix.
+      auto page_at = [&](int pos) { return pos < p.prefix ? p.a.kv.table[pos / page_size] : -1; };
+      int seg = step0 / each, kt = (step0 - seg * each) * TPS;
+      int g = seg / p.tile_segs;
+      bool new_seg = true;
       int segs_seen = 0;
-      auto first_product = [&](int t) {
-        const int j = t - tile0, s = j % STAGES, kt = t % p.tiles_each;
-        if (t == tile0 || kt == 0) {
-          if (!tc5::bar_wait(Q_FULL, segs_seen & 1)) return false;
-          segs_seen++;
+      const int tiles = steps * TPS;
+      bool ok = true;
+      // Waits until ring place n may be filled; meanwhile tells of whatever has landed.
+      auto claim = [&](int n) {
+        if (n < NSLOT) return true;
+        const uint32_t ph = tc5::phase(n, NSLOT, true);
+        if (!tc5::bar_try(EMPTY(n % NSLOT), ph)) {
+          if (told < n) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            tell(n);
+          }
+          if (!tc5::bar_wait(EMPTY(n % NSLOT), ph)) return false;
         }
-        if (!tc5::bar_wait(K_FULL(s), (j / STAGES) & 1)) return false;
-        tc5::fence_after();
-        const uint32_t k_s = base + L::Q_BYTES + s * L::STAGE;
-#pragma unroll
-        for (int k = 0; k < DP / 16; k++)
-          mma_ss(tmem + (j & 1) * KT, tc5::desc_sw128(base + (k >> 2) * (kTileRows * 128) + (k & 3) * 32),
-                 tc5::desc_sw128(k_s + (k >> 2) * (KT * 128) + (k & 3) * 32), kIdescS, k > 0);
-        tc5::commit(S_FULL(j & 1));
-        tc5::commit(K_EMPTY(s));
-        if (t + 1 == tile1 || kt + 1 == p.tiles_each) tc5::commit(Q_EMPTY);
         return true;
       };
-      bool ok = tile0 < tile1 ? first_product(tile0) : true;
-      for (int t = tile0; t < tile1 && ok; t++) {
-        const int j = t - tile0, s = j % STAGES;
-        if (t + 1 < tile1) ok = first_product(t + 1);
-        ok = ok && tc5::bar_wait(P_FULL(j & 1), (j >> 1) & 1) && tc5::bar_wait(V_FULL(s), (j / STAGES) & 1);
-        if (!ok) break;
-        tc5::fence_after();
-        const uint32_t v_s = base + L::Q_BYTES + s * L::STAGE + L::KV_BYTES;
-        const bool start = t == tile0 || t % p.tiles_each == 0;
+      // The page of this lane's box of the next tile, read a tile ahead.
+      int box_page = lane < boxes && steps ? page_at(kt * KT + lane * box) : -1;
+      for (int n = 0; n < tiles && ok && !*abort_flag; n++) {
+        const bool with_q = new_seg;
+        if (new_seg) {
+          if (segs_seen) {
+            // The products with the Q before need every tile so far.
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            tell(2 * n);
+            if (!tc5::bar_wait(Q_EMPTY, tc5::phase(segs_seen - 1, 1))) {
+              ok = false;
+              break;
+            }
+          }
+          segs_seen++;
+          new_seg = false;
+          const int row0 = (seg - g * p.tile_segs) * RT * kTileRows;
+#pragma unroll 1
+          for (int r = lw * 4 + sub; r < RT * kTileRows; r += 4 * kLoaders) {
+            const int row = row0 + r, tok = row / p.group;
+            const bool in = row < rows;
+            const T* src = static_cast<const T*>(p.a.q) + (in ? (int64_t)tok * p.a.q_tok + (int64_t)(g * p.group + row - tok * p.group) * p.a.q_head : 0);
 #pragma unroll
-        for (int k = 0; k < KT / 16; k++)
-          mma_ts(tmem + kColO, tmem + (j & 1) * KT + 8 * k, desc_n_major(v_s + k * 2048, KT * 128), kIdescO, !start || k > 0);
-        tc5::commit(V_EMPTY(s));
-        tc5::commit(PV_DONE);
+            for (int c = 0; c < DP / 64; c++) {
+              const int chunk = c * 8 + (lane & 7);
+              const bool there = in && chunk * 8 < D;
+              const uint32_t at = (r / kTileRows) * L::Q_TILE + place(kTileRows, r % kTileRows, chunk);
+              if (p.q_copies) {
+                copy16(base + at, src + (there ? chunk * 8 : 0), there);
+              } else {
+                T* dst = reinterpret_cast<T*>(gbase + at);
+#pragma unroll
+                for (int e = 0; e < 8; e++) dst[e] = there ? src[chunk * 8 + e] : from_f32<T>(0.0f);
+              }
+            }
+          }
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          __syncwarp();
+        }
+        const uint32_t k_s = ring + (2 * n % NSLOT) * L::SLOT, v_s = ring + ((2 * n + 1) % NSLOT) * L::SLOT;
+        // A tile that lies whole in pages that exist comes by TMA, a box for each page (or piece of one):
+        // every loader warp sees the same pages and takes the same way. The prefix's last tile, one with a
+        // bad page, and pages of fewer than 4 positions are gathered row by row, zeros in the gaps (what
+        // lies behind the prefix in its last page may be anything, and 0 times NaN is no 0).
+        const int box_pos = kt * KT + lane * box;
+        const bool by_box = boxes && !__any_sync(0xffffffffu, lane < boxes && (box_page < 0 || box_page >= p.a.kv.pages || box_pos + box > p.prefix));
+        const int this_kt = kt, this_g = g, this_page = box_page;
+        if (++kt == each * TPS) {
+          kt = 0;
+          new_seg = true;
+          if (++seg, seg % p.tile_segs == 0) g++;
+        }
+        if (lane < boxes && n + 1 < tiles) box_page = page_at(kt * KT + lane * box);
+        if (by_box) {
+          if (told < 2 * n) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            tell(2 * n);
+          }
+#pragma unroll 1
+          for (int h = 0; h < 2 && ok; h++) {
+            ok = claim(2 * n + h);
+            __syncwarp();
+            if (!ok) break;
+            if (h == 0 && lane == 0) {
+#pragma unroll
+              for (int w = 0; w < 2; w++) {
+                const int keys = 4 * ((kGroups - lw + kLoaders - 1) / kLoaders) - 32 * w;
+                s_valid[n % kMasks][lw][w] = keys >= 32 ? 0xffffffffu : keys > 0 ? (1u << keys) - 1u : 0u;
+              }
+              tc5::bar_arrive(MASK(n % kMasks));
+            }
+            const uint32_t full = FULL((2 * n + h) % NSLOT);
+            if (lw == h && lane == 0) tc5::bar_expect(full, L::SLOT);
+            else tc5::bar_arrive(full);
+            told = 2 * n + h + 1;
+            __syncwarp();
+            if (lw == h && lane < boxes) {
+              const uint32_t dst = (h ? v_s : k_s) + lane * box * 128;
+              const int slot = box_pos % page_size;
+#pragma unroll
+              for (int c = 0; c < DP / 64; c++) tc5::tma_4d(dst + c * KT * 128, h ? &tmv : &tmk, 64 * c, slot, this_g, this_page, full);
+            }
+          }
+        } else {
+          // Offsets of this lane's keys.
+          int64_t ka = 0, va = 0, kb = 0, vb = 0;
+          auto offsets = [&](int key, int64_t& ko, int64_t& vo) {
+            const int pos = this_kt * KT + key;
+            if (key < 0 || pos >= p.prefix) return false;
+            const int page = page_at(pos);
+            if (page < 0 || page >= p.a.kv.pages) {
+              if (p.a.status) atomicOr(p.a.status, SERVE_BAD_INDEX);
+              return false;
+            }
+            const int64_t slot = pos % page_size;
+            ko = page * p.a.kv.k_page + slot * p.a.kv.k_slot + this_g * p.a.kv.k_head;
+            vo = page * p.a.kv.v_page + slot * p.a.kv.v_slot + this_g * p.a.kv.v_head;
+            return true;
+          };
+          const uint32_t in_a = __ballot_sync(0xffffffffu, offsets(key_a, ka, va));
+          const uint32_t in_b = __ballot_sync(0xffffffffu, offsets(key_b, kb, vb));
+#pragma unroll 1
+          for (int h = 0; h < 2 && ok; h++) {
+            ok = claim(2 * n + h);
+            __syncwarp();
+            if (!ok) break;
+            if (h == 0 && lane == 0) {
+              s_valid[n % kMasks][lw][0] = in_a;
+              s_valid[n % kMasks][lw][1] = in_b;
+              tc5::bar_arrive(MASK(n % kMasks));
+            }
+            const T* from = h ? V : K;
+            const int64_t oa = h ? va : ka, ob = h ? vb : kb;
+            const uint32_t dst = h ? v_s : k_s;
+#pragma unroll 4
+            for (int i = 0; i < (kGroups + kLoaders - 1) / kLoaders; i++) {
+              const int grp = lw + kLoaders * i, src = (4 * i + sub) & 31;
+              const int64_t o = __shfl_sync(0xffffffffu, i < 8 ? oa : ob, src);
+              const bool in = ((i < 8 ? in_a : in_b) >> src) & 1;
+              if (grp < kGroups) {
+#pragma unroll
+                for (int c = 0; c < DP / 64; c++) {
+                  const int chunk = c * 8 + (lane & 7);
+                  const bool there = in && chunk * 8 < D;
+                  copy16(dst + place(KT, 4 * grp + sub, chunk), from + (there ? o + chunk * 8 : 0), there);
+                }
+              }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+          }
+          if (!ok) break;
+          asm volatile("cp.async.wait_group 2;" ::: "memory");
+          if (told < 2 * n) tell(2 * n);
+        }
+        if (with_q) {
+          if (by_box) asm volatile("cp.async.wait_group 0;" ::: "memory");
+          else asm volatile("cp.async.wait_group 2;" ::: "memory");
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          tc5::bar_arrive(Q_FULL);
+        }
       }
-      if (!ok) fail();
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      if (ok && !*abort_flag) tell(2 * tiles);
+      else if (lane == 0) fail();
+    } else {
+      // ---- products ----
+      const uint32_t one = tc5::elect();
+      int segs_seen = 0;
+      bool ok = true;
+      // S of step i for stream r: its key tile is n. `seg_of` and `in_of`: the segment of a step and the
+      // step's place in it, for this step and the next (divisions are slow next to an MMA).
+      int seg_of[2], in_of[2];
+      seg_of[0] = step0 / each;
+      in_of[0] = step0 - seg_of[0] * each;
+      auto follow = [&]() {
+        in_of[1] = in_of[0] + 1 == each ? 0 : in_of[0] + 1;
+        seg_of[1] = seg_of[0] + (in_of[1] == 0);
+      };
+      follow();
+      auto first = [&](int i, int r, int k_) {
+        const int n = i * TPS + (TPS == 2 ? r : 0), buf = STREAMS == 2 ? r : (n & 1), at = 2 * n % NSLOT;
+        const int in = in_of[k_];
+        if (r == 0 && (i == 0 || in == 0)) {
+          if (!tc5::bar_wait(Q_FULL, tc5::phase(segs_seen, 1))) return false;
+          segs_seen++;
+        }
+        if ((TPS == 2 || r == 0) && !tc5::bar_wait(FULL(at), tc5::phase(2 * n, NSLOT))) return false;
+        tc5::fence_after();
+        const bool on = live(seg_of[k_], r);
+        const uint32_t qs = base + (RT == 2 ? r : 0) * L::Q_TILE, ks = ring + at * L::SLOT;
+        if (on) {
+#pragma unroll
+          for (int k = 0; k < DP / 16; k++)
+            mma_ss(tmem + buf * KT, tc5::desc_sw128(qs + (k >> 2) * (kTileRows * 128) + (k & 3) * 32),
+                   tc5::desc_sw128(ks + (k >> 2) * (KT * 128) + (k & 3) * 32), kIdescS, k > 0, one);
+          tc5::commit(S_FULL(buf), one);
+        }
+        if (TPS == 2 || r == RT - 1) tc5::commit(EMPTY(at), one);
+        if (r == STREAMS - 1 && (i + 1 == steps || in + 1 == each)) tc5::commit(Q_EMPTY, one);
+        return true;
+      };
+      // O of stream r += P V at step i; u: how many P the buffer has had.
+      int used[2] = {0, 0};
+      auto second = [&](int i, int r) {
+        const int n = i * TPS + (TPS == 2 ? r : 0), buf = STREAMS == 2 ? r : (n & 1), at = (2 * n + 1) % NSLOT;
+        const bool on = live(seg_of[0], r);
+        if (on && !tc5::bar_wait(P_FULL(buf), used[buf]++ & 1)) return false;
+        if ((TPS == 2 || r == 0) && !tc5::bar_wait(FULL(at), tc5::phase(2 * n + 1, NSLOT))) return false;
+        tc5::fence_after();
+        const bool start = i == 0 || in_of[0] == 0;
+        const uint32_t vs = ring + at * L::SLOT;
+        if (on) {
+#pragma unroll
+          for (int k = 0; k < KT / 16; k++)
+            mma_ts(tmem + kColO + r * DP, tmem + buf * KT + 8 * k, desc_n_major(vs + k * 2048, KT * 128), kIdescO, !start || k > 0, one);
+          tc5::commit(PV_DONE(r), one);
+        }
+        if (TPS == 2 || r == RT - 1) tc5::commit(EMPTY(at), one);
+        return true;
+      };
+      if (steps) {
+        for (int r = 0; r < STREAMS && ok; r++) ok = first(0, r, 0);
+        for (int i = 0; i < steps && ok; i++) {
+#pragma unroll
+          for (int r = 0; r < STREAMS; r++) {
+            if constexpr (STREAMS == 1) {
+              ok = (i + 1 == steps || first(i + 1, 0, 1)) && second(i, 0);
+            } else {
+              ok = ok && second(i, r) && (i + 1 == steps || first(i + 1, r, 1));
+            }
+          }
+          seg_of[0] = seg_of[1];
+          in_of[0] = in_of[1];
+          follow();
+        }
+      }
+      if (!ok && lane == 0) fail();
     }
-  } else if (warp < 4) {
-    // ---- softmax: row tid ----
-    const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+  } else {
+    // ---- softmax: row `row` of stream r ----
+    const int r = warp >> 2, row = tid & 127;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, so = tmem + lanes + kColO + r * DP;
     float m = -INFINITY, l = 0.0f;  // m: what the weights are relative to
-    for (int t = tile0; t < tile1; t++) {
-      const int j = t - tile0, s = j % STAGES, seg = t / p.tiles_each;
-      const bool start = t == tile0 || t % p.tiles_each == 0, last = t + 1 == tile1 || (t + 1) % p.tiles_each == 0;
-      if (!tc5::bar_wait(S_FULL(j & 1), (j >> 1) & 1)) {
-        if (lane == 0) fail();
-        break;
-      }
-      // (done long ago: waited for here too because it is what publishes s_valid)
-      if (!tc5::bar_wait(K_FULL(s), (j / STAGES) & 1)) {
+    int used = 0;                   // tiles that this stream has had
+    int seg = step0 / each, in = step0 - seg * each;
+    for (int i = 0; i < steps; i++) {
+      const bool start = i == 0 || in == 0, last = i + 1 == steps || in + 1 == each;
+      const int this_seg = seg;
+      if (++in == each) in = 0, seg++;
+      if (!live(this_seg, r)) continue;
+      const int n = i * TPS + (TPS == 2 ? r : 0), buf = STREAMS == 2 ? r : (n & 1);
+      const uint32_t sp = tmem + lanes + buf * KT;
+      bool whole = tc5::bar_wait(MASK(n % kMasks), tc5::phase(n, kMasks));
+      if (!whole || !tc5::bar_wait(S_FULL(buf), (STREAMS == 2 ? used : used >> 1) & 1)) {
         if (lane == 0) fail();
         break;
       }
       tc5::fence_after();
-      const uint32_t sp = tmem + lanes + (j & 1) * KT;
-      float x[KT];
+      // The row is read twice, 32 columns at a time, in loops that stay in the instruction cache: the same
+      // arithmetic unrolled over a whole row waits more for instructions than for anything else (2.4 of
+      // 4 cycles an instruction, 86 us on 64 sequences behind 32768 keys).
 #pragma unroll
-      for (int c = 0; c < KT / 32; c++) tmem_ld32(sp + 32 * c, x + 32 * c);
-      tc5::wait_ld();
-      constexpr int kWord = KT / 4;  // keys of a loader warp: bits of a word of s_valid
-      bool whole = true;
-#pragma unroll
-      for (int w = 0; w < 4; w++) whole = whole && s_valid[s][w] == (kWord == 32 ? 0xffffffffu : (1u << (kWord & 31)) - 1u);
-      if (!whole) {
-#pragma unroll
-        for (int i = 0; i < KT; i++)
-          if (!((s_valid[s][i / kWord] >> (i % kWord)) & 1)) x[i] = -INFINITY;
+      for (int w = 0; w < kLoaders; w++) {
+        const int keys = 4 * ((kGroups - w + kLoaders - 1) / kLoaders);
+        const uint32_t lo = keys >= 32 ? 0xffffffffu : (1u << (keys & 31)) - 1u, hi = keys > 32 ? (1u << (keys - 32)) - 1u : 0u;
+        whole = whole && s_valid[n % kMasks][w][0] == lo && s_valid[n % kMasks][w][1] == hi;
       }
-      float top = x[0];
+      if (!whole) {
+        // The prefix's end, or a page that does not exist: those scores become what no other can exceed.
+        const float never = p.scale_log2 > 0.0f ? -INFINITY : INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < KT / 32; c++) {
+          float x[32];
+          tmem_ld32(sp + 32 * c, x);
+          tc5::wait_ld();
 #pragma unroll
-      for (int i = 1; i < KT; i++) top = fmaxf(top, x[i]);
-      // The scale may be negative or 0: the largest score is then that of the smallest product.
-      if (p.scale_log2 <= 0.0f) {
-        top = -INFINITY;
+          for (int j = 0; j < 32; j++) {
+            const int grp = 8 * c + (j >> 2), w = grp % kLoaders, k = 4 * (grp / kLoaders) + (j & 3);
+            if (!((s_valid[n % kMasks][w][k >> 5] >> (k & 31)) & 1)) x[j] = never;
+          }
+          tmem_st32(sp + 32 * c, reinterpret_cast<const uint32_t*>(x));
+        }
+        tmem_wait_st();
+      }
+      float top;
+      if (p.scale_log2 > 0.0f) {
+        float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < KT / 64; c++) {
+          float x[64];
+          tmem_ld32(sp + 64 * c, x);
+          tmem_ld32(sp + 64 * c + 32, x + 32);
+          tc5::wait_ld();
+          float a = fmaxf(x[0], x[1]), b = fmaxf(x[2], x[3]);
 #pragma unroll
-        for (int i = 0; i < KT; i++) top = fmaxf(top, x[i] == -INFINITY && !whole ? -INFINITY : x[i] * p.scale_log2);
-      } else {
-        top *= p.scale_log2;
+          for (int j = 4; j < 64; j += 4) {
+            t0 = fmaxf(fmaxf(x[j], x[j + 1]), t0);
+            t1 = fmaxf(fmaxf(x[j + 2], x[j + 3]), t1);
+          }
+          t0 = fmaxf(t0, a);
+          t1 = fmaxf(t1, b);
+        }
+        top = fmaxf(t0, t1) * p.scale_log2;
+      } else {  // the largest score is that of the smallest product
+        float low = INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < KT / 32; c++) {
+          float x[32];
+          tmem_ld32(sp + 32 * c, x);
+          tc5::wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; j++) low = fminf(low, x[j]);
+        }
+        top = low * p.scale_log2;
       }
       if (start) {
         m = top;
@@ -844,8 +1032,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         const bool grow = top > m + 8.0f || (m == -INFINITY && top > -INFINITY);
         if (__any_sync(0xffffffffu, grow)) {
           const float to = grow ? top : m;
-          const float f = m == -INFINITY ? 0.0f : exp2_fast(m - to);
-          if (!tc5::bar_wait(PV_DONE, (j - 1) & 1)) {
+          const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : exp2_fast(m - to);
+          if (!tc5::bar_wait(PV_DONE(r), (used - 1) & 1)) {
             if (lane == 0) fail();
             break;
           }
@@ -853,60 +1041,64 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
 #pragma unroll 1
           for (int c = 0; c < DP / 32; c++) {
             float o[32];
-            tmem_ld32(tmem + lanes + kColO + 32 * c, o);
+            tmem_ld32(so + 32 * c, o);
             tc5::wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; i++) o[i] *= grow ? f : 1.0f;
-            tmem_st32(tmem + lanes + kColO + 32 * c, reinterpret_cast<const uint32_t*>(o));
+            for (int j = 0; j < 32; j++) o[j] *= f;
+            tmem_st32(so + 32 * c, reinterpret_cast<const uint32_t*>(o));
           }
           tmem_wait_st();
-          if (grow) l *= f;
+          l *= f;
           m = to;
         }
       }
       const float u = m == -INFINITY ? 0.0f : m;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      // P in the place of S: 16 columns for 32, so that a chunk never lands on columns not read yet.
+      const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), u2 = make_float2(-u, -u);
+      float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
+      float x[32];
+      tmem_ld32(sp, x);
+#pragma unroll 1
+      for (int c = 0; c < KT / 32; c++) {
+        tc5::wait_ld();
+        float2 e[16];
 #pragma unroll
-      for (int c = 0; c < KT / 64; c++) {
-        uint32_t w[32];
+        for (int j = 0; j < 16; j++) e[j] = fma2(make_float2(x[2 * j], x[2 * j + 1]), scale2, u2);
+        if (c + 1 < KT / 32) tmem_ld32(sp + 32 * (c + 1), x);
+        uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 32; i++) {
-          const int k = 64 * c + 2 * i;
-          float a = fmaf(x[k], p.scale_log2, -u), b = fmaf(x[k + 1], p.scale_log2, -u);
-          if (p.scale_log2 <= 0.0f && !whole) {
-            if (x[k] == -INFINITY) a = -INFINITY;
-            if (x[k + 1] == -INFINITY) b = -INFINITY;
-          }
-          a = exp2_fast(a);
-          b = exp2_fast(b);
-          sum[i & 3] += a + b;
-          w[i] = pack2<T>(a, b);
+        for (int j = 0; j < 16; j++) {
+          e[j].x = exp2_fast(e[j].x);
+          e[j].y = exp2_fast(e[j].y);
+          if (j & 1) sum1 = add2(sum1, e[j]);
+          else sum0 = add2(sum0, e[j]);
+          w[j] = pack2<T>(e[j].x, e[j].y);
         }
-        tmem_st32(sp + 32 * c, w);
+        tmem_st16(sp + 16 * c, w);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
       tmem_wait_st();
       tc5::fence_before();
-      tc5::bar_arrive(P_FULL(j & 1));
+      tc5::bar_arrive(P_FULL(buf));
+      used++;
       if (last) {
-        if (!tc5::bar_wait(PV_DONE, j & 1)) {
+        if (!tc5::bar_wait(PV_DONE(r), (used - 1) & 1)) {
           if (lane == 0) fail();
           break;
         }
         tc5::fence_after();
-        float* slot = p.tile_part + (int64_t)((int)blockIdx.x + seg) * (kTileRows * (DP + 2));
-        const int mt = seg % p.tile_segs;
-        const bool in = mt * kTileRows + tid < (int)p.a.tokens * p.group;
-        if (in) *reinterpret_cast<float2*>(slot + 2 * tid) = make_float2(m, l);
+        float* slot = p.tile_part + (int64_t)(((int)blockIdx.x + this_seg) * STREAMS + r) * (kTileRows * (DP + 2));
+        const bool there = ((this_seg % p.tile_segs) * RT + (RT == 2 ? r : 0)) * kTileRows + row < rows;
+        if (there) *reinterpret_cast<float2*>(slot + 2 * row) = make_float2(m, l);
 #pragma unroll 1
         for (int c = 0; c < DP / 32; c++) {
           float o[32];
-          tmem_ld32(tmem + lanes + kColO + 32 * c, o);
+          tmem_ld32(so + 32 * c, o);
           tc5::wait_ld();
-          if (in) {
-            float4* dst = reinterpret_cast<float4*>(slot + 2 * kTileRows + tid * DP + 32 * c);
+          if (there) {
+            float4* dst = reinterpret_cast<float4*>(slot + 2 * kTileRows + row * DP + 32 * c);
 #pragma unroll
-            for (int i = 0; i < 8; i++) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            for (int j = 0; j < 8; j++) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
           }
         }
         tc5::fence_before();
@@ -915,7 +1107,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   }
   tc5::fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kMmaWarp) {
     tc5::fence_after();
     tc5::dealloc(tmem, 512);
   }
@@ -945,10 +1137,12 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     slot0[k] = nullptr;
     if (k && !with_prefix) continue;
     if (k && p.on_tiles) {
-      const int mt = r / kTileRows, seg = g * p.tile_segs + mt, w = part_of(p.tiles_total, p.tile_parts, seg * p.tiles_each);
-      rr[k] = r - mt * kTileRows;
-      count[k] = part_of(p.tiles_total, p.tile_parts, (seg + 1) * p.tiles_each - 1) - w + 1;
-      slot0[k] = p.tile_part + (int64_t)(w + seg) * (kTileRows * (DP + 2));
+      // A CTA leaves a part for each stream: of other rows, or of the same rows' other keys.
+      const int mt = r / (kTileRows * p.tile_rt), seg = g * p.tile_segs + mt, w = part_of(p.tiles_total, p.tile_parts, seg * p.tiles_each);
+      const int in = r - mt * kTileRows * p.tile_rt, stream = in / kTileRows;
+      rr[k] = in - stream * kTileRows;
+      count[k] = (part_of(p.tiles_total, p.tile_parts, (seg + 1) * p.tiles_each - 1) - w + 1) * (p.tile_streams / p.tile_rt);
+      slot0[k] = p.tile_part + ((int64_t)(w + seg) * p.tile_streams + stream) * (kTileRows * (DP + 2));
       continue;
     }
     const int mb = r / kRows;
@@ -964,7 +1158,8 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
   // Part i's (m, l) of the row, and its o.
   auto at = [&](int i, const float*& o) {
     const int k = i >= count[0], rows = k && p.on_tiles ? kTileRows : kRows;
-    const float* s = slot0[k] + (int64_t)(i - (k ? count[0] : 0)) * (rows * (DP + 2));
+    const int step = rows * (DP + 2) * (k && p.on_tiles ? p.tile_rt : 1);
+    const float* s = slot0[k] + (int64_t)(i - (k ? count[0] : 0)) * step;
     o = s + 2 * rows + rr[k] * DP;
     return s + 2 * rr[k];
   };
@@ -1011,22 +1206,31 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
 int padded_dim(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 int part_warps(int dp) { return dp == 256 ? 4 : 8; }
 
-// Keys of a tile of the prefix kernel.
-int tile_keys(int dp) { return dp == 256 ? 64 : 128; }
-// Where the prefix goes to the tensor cores' own tiles.
-bool use_tiles(const vtq_attention_args& a) {
+// How the prefix goes to the tensor cores' own tiles, and where: more rows than the 16 that one read of
+// a key serves in the part kernel, and keys enough to pay for another launch.
+struct TileCut {
+  bool on;
+  int keys, rt, streams, segs, each;  // keys of a tile; see AttnParams
+  int64_t total;
+};
+TileCut tile_cut(const vtq_attention_args& a) {
+  TileCut c = {};
   const int64_t rows = a.tokens * (a.heads / a.kv.kv_heads), prefix = std::min(a.shared_len, a.kv.table_width * a.kv.page_size);
-  return rows > 16 && prefix >= 512;
-}
-int64_t tile_total(const vtq_attention_args& a) {
-  const int64_t rows = a.tokens * (a.heads / a.kv.kv_heads), prefix = std::min(a.shared_len, a.kv.table_width * a.kv.page_size);
-  const int keys = tile_keys(padded_dim(a.kv.head_dim));
-  return a.kv.kv_heads * ((rows + kTileRows - 1) / kTileRows) * ((prefix + keys - 1) / keys);
+  c.on = rows > 16 && prefix >= 512;
+  const bool wide = a.kv.head_dim > 128;
+  c.keys = wide ? 64 : 128;
+  c.streams = wide ? 1 : 2;
+  c.rt = !wide && rows > kTileRows ? 2 : 1;
+  c.segs = (int)((rows + kTileRows * c.rt - 1) / (kTileRows * c.rt));
+  const int step = c.keys * c.streams / c.rt;
+  c.each = (int)((prefix + step - 1) / step);
+  c.total = a.kv.kv_heads * (int64_t)c.segs * c.each;
+  return c;
 }
 size_t tile_bytes(const vtq_attention_args& a) {
-  if (!use_tiles(a)) return 0;
-  const int64_t rows = a.tokens * (a.heads / a.kv.kv_heads);
-  const int64_t slots = std::min<int64_t>(tile_total(a), num_sms()) + a.kv.kv_heads * ((rows + kTileRows - 1) / kTileRows);
+  const TileCut c = tile_cut(a);
+  if (!c.on) return 0;
+  const int64_t slots = (std::min<int64_t>(c.total, num_sms()) + a.kv.kv_heads * c.segs) * c.streams;
   return (size_t)slots * kTileRows * (padded_dim(a.kv.head_dim) + 2) * 4;
 }
 
@@ -1036,7 +1240,7 @@ size_t plan_bytes(const vtq_attention_args& a) {
 // Segments of any lengths: each sequence's rows and, once more, all rows for the prefix.
 int64_t most_segments(const vtq_attention_args& a) {
   const int64_t group = a.heads / a.kv.kv_heads, rows = a.tokens * group;
-  return (rows / kRows + a.kv.seqs + (a.shared_len && !use_tiles(a) ? (rows + kRows - 1) / kRows : 0)) * a.kv.kv_heads;
+  return (rows / kRows + a.kv.seqs + (a.shared_len && !tile_cut(a).on ? (rows + kRows - 1) / kRows : 0)) * a.kv.kv_heads;
 }
 
 size_t part_bytes(const vtq_attention_args& a) {
@@ -1055,9 +1259,36 @@ vtq_status check(const char* fn, const vtq_attention_args* a) {
   if (a->tokens > (1 << 20) || a->heads > 65536 || a->kv.table_width * a->kv.page_size > INT32_MAX / 2)
     return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "%s: not implemented (over 2^20 tokens, 2^16 heads or 2^30 positions)", fn);
   const int64_t tiles = (a->kv.table_width * a->kv.page_size + 15) / 16 + 1;
-  if (most_segments(*a) * tiles > INT32_MAX || tile_total(*a) > INT32_MAX)
+  if (most_segments(*a) * tiles > INT32_MAX || tile_cut(*a).total > INT32_MAX)
     return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "%s: not implemented (query rows times table positions over 2^35)", fn);
   return VTQ_OK;
+}
+
+template <typename T, int DP, int KT, int RT, int STREAMS, int NSLOT>
+cudaError_t launch_tiles(const AttnParams& p, cudaStream_t st) {
+  using L = TileShape<T, DP, KT, RT, STREAMS, NSLOT>;
+  auto tiles = attention_tile_kernel<T, DP, KT, RT, STREAMS, NSLOT>;
+  const cudaError_t e = cudaFuncSetAttribute(tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::SMEM);
+  if (e != cudaSuccess) return e;
+  // A box is the largest power of two of positions that pages are made of.
+  AttnParams q = p;
+  CUtensorMap tmk = {}, tmv = {};
+  const vtq_paged_kv& kv = p.a.kv;
+  q.tile_box = 1;
+  while (q.tile_box < KT && kv.page_size % (2 * q.tile_box) == 0) q.tile_box *= 2;
+  if (KT / q.tile_box > 32) {
+    q.tile_box = 0;
+  } else {
+    const uint64_t dim[4] = {(uint64_t)kv.head_dim, (uint64_t)kv.page_size, (uint64_t)kv.kv_heads, (uint64_t)kv.pages};
+    const uint64_t ks[3] = {2 * (uint64_t)kv.k_slot, 2 * (uint64_t)kv.k_head, 2 * (uint64_t)kv.k_page};
+    const uint64_t vs[3] = {2 * (uint64_t)kv.v_slot, 2 * (uint64_t)kv.v_head, 2 * (uint64_t)kv.v_page};
+    if (tma_half_map(&tmk, kv.k, dim, ks, 64, (uint32_t)q.tile_box) != cudaSuccess ||
+        tma_half_map(&tmv, kv.v, dim, vs, 64, (uint32_t)q.tile_box) != cudaSuccess)
+      q.tile_box = 0;  // strides that TMA does not take: rows are gathered
+  }
+  kernel_launch_count()++;
+  tiles<<<(unsigned)p.tile_parts, L::THREADS, L::SMEM, st>>>(q, tmk, tmv);
+  return cudaGetLastError();
 }
 
 template <typename T, int DP, int KT, int WARPS, int STAGES>
@@ -1067,14 +1298,11 @@ cudaError_t launch(const AttnParams& p, cudaStream_t st) {
                       (size_t)WARPS * KT * sizeof(longlong2);
   cudaError_t e = cudaFuncSetAttribute(part, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  constexpr int TKT = DP == 256 ? 64 : 128, TST = DP == 64 ? 5 : DP == 128 ? 3 : 2;
   if (p.on_tiles) {
-    auto tiles = attention_tile_kernel<T, DP, TKT, TST>;
-    constexpr size_t tile_smem = TileShape<T, DP, TKT, TST>::SMEM;
-    if ((e = cudaFuncSetAttribute(tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tile_smem)) != cudaSuccess) return e;
-    kernel_launch_count()++;
-    tiles<<<(unsigned)p.tile_parts, kTileThreads, tile_smem, st>>>(p);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    if constexpr (DP == 256) e = launch_tiles<T, 256, 64, 1, 1, 5>(p, st);
+    else if constexpr (DP == 128) e = p.tile_rt == 2 ? launch_tiles<T, 128, 128, 2, 2, 5>(p, st) : launch_tiles<T, 128, 128, 1, 2, 6>(p, st);
+    else e = p.tile_rt == 2 ? launch_tiles<T, 64, 128, 2, 2, 8>(p, st) : launch_tiles<T, 64, 128, 1, 2, 8>(p, st);
+    if (e != cudaSuccess) return e;
   }
   kernel_launch_count() += 2;
   // Each waits for the one before at its own point (griddepcontrol): the part kernel at its end.
@@ -1133,17 +1361,20 @@ vtq_status vtq_attention_paged(const vtq_attention_args* a, void* ws, size_t ws_
   p.parts = num_sms() * part_warps(p.dim_padded);
   p.keys_max = (int)(a->kv.table_width * a->kv.page_size);
   p.prefix = (int)std::min<int64_t>(a->shared_len, p.keys_max);
-  p.scale_log2 = a->scale * 1.4426950408889634f;
+  // A scale of 0 weighs every key alike: so does one that no product reaches.
+  p.scale_log2 = a->scale == 0.0f ? 1e-30f : a->scale * 1.4426950408889634f;
   p.q_wide = (reinterpret_cast<uintptr_t>(a->q) & 3u) == 0 && a->q_tok % 2 == 0 && a->q_head % 2 == 0;
   p.plan = static_cast<int*>(ws);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan_bytes(*a));
-  p.on_tiles = use_tiles(*a);
-  if (p.on_tiles) {
-    const int keys = tile_keys(p.dim_padded);
+  const TileCut c = tile_cut(*a);
+  p.on_tiles = c.on;
+  if (c.on) {
     p.q_copies = aligned16(a->q) && a->q_tok % 8 == 0 && a->q_head % 8 == 0;
-    p.tile_segs = (int)((a->tokens * p.group + kTileRows - 1) / kTileRows);
-    p.tiles_each = (p.prefix + keys - 1) / keys;
-    p.tiles_total = (int)tile_total(*a);
+    p.tile_rt = c.rt;
+    p.tile_streams = c.streams;
+    p.tile_segs = c.segs;
+    p.tiles_each = c.each;
+    p.tiles_total = (int)c.total;
     p.tile_parts = std::min(p.tiles_total, num_sms());
     p.tile_part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.part) + part_bytes(*a));
   }

@@ -545,6 +545,20 @@ EncodeFn encoder() {
 
 }  // namespace
 
+// 4D map of 16-bit values, boxes of box0 x box1 x 1 x 1, 128-byte swizzle; dim[0] contiguous, strides in bytes.
+cudaError_t tma_half_map(CUtensorMap* tm, const void* ptr, const uint64_t (&dim)[4], const uint64_t (&stride)[3],
+                         uint32_t box0, uint32_t box1) {
+  EncodeFn enc = encoder();
+  if (!enc) return cudaErrorInvalidValue;
+  const cuuint64_t gdim[4] = {dim[0], dim[1], dim[2], dim[3]}, gstride[3] = {stride[0], stride[1], stride[2]};
+  const cuuint32_t box[4] = {box0, box1, 1, 1}, es[4] = {1, 1, 1, 1};
+  return enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(ptr), gdim, gstride, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? cudaSuccess
+             : cudaErrorInvalidValue;
+}
+
 // 2D byte tensor map [rows][cols] with row stride `pitch`.
 cudaError_t tma_byte_map(CUtensorMap* tm, const void* ptr, int64_t rows, int64_t cols, int64_t pitch,
                      uint32_t box_x, uint32_t box_y, CUtensorMapSwizzle sw) {

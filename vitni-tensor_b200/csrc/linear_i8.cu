@@ -154,11 +154,11 @@ constexpr int BM = 128;          // output channels a tile
 constexpr uint32_t A_STAGE = BM * 128;
 constexpr int kThreads = 192;    // producer warp, MMA warp, 4 epilogue warps
 
-__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one));
 }
 
 template <typename Y>
@@ -238,22 +238,21 @@ __global__ void __launch_bounds__(kThreads)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      for (int k = 0; k < nk; k++) {
-        const int s = k % STAGES;
-        if (!tc5::bar_wait(FULL(s), (k / STAGES) & 1)) {
-          fail();
-          break;
-        }
-        tc5::fence_after();
-        const uint32_t sa = base + s * STAGE, sb = sa + A_STAGE;
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-          mma_i8(tmem, tc5::desc_sw128(sa + 32 * c), tc5::desc_sw128(sb + 32 * c), kIdesc, (k | c) ? 1u : 0u);
-        tc5::commit(EMPTY(s));
+    const uint32_t one = tc5::elect();
+    for (int k = 0; k < nk; k++) {
+      const int s = k % STAGES;
+      if (!tc5::bar_wait(FULL(s), (k / STAGES) & 1)) {
+        if (lane == 0) fail();
+        break;
       }
-      tc5::commit(DONE);
+      tc5::fence_after();
+      const uint32_t sa = base + s * STAGE, sb = sa + A_STAGE;
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+        mma_i8(tmem, tc5::desc_sw128(sa + 32 * c), tc5::desc_sw128(sb + 32 * c), kIdesc, (k | c) ? 1u : 0u, one);
+      tc5::commit(EMPTY(s), one);
     }
+    tc5::commit(DONE, one);
   } else {
     tc5::grid_wait();  // the token scales
     const bool ok = tc5::bar_wait(DONE, 0);

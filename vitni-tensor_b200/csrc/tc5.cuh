@@ -14,11 +14,32 @@ __device__ __forceinline__ void bar_init(uint32_t bar, unsigned count) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// The phase that `n` uses of a ring of `size` completes: waited for by its consumers, or (`before`) the
+// phase before it by the producer who is to fill it again.
+__device__ __forceinline__ uint32_t phase(int n, int size, bool before = false) {
+  return (uint32_t)(n / size + (before ? 1 : 0)) & 1u;
+}
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded by the SM's own clock (cheaper to read than %globaltimer): 2^32 cycles, about 2 s.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-  return mbar_wait_bounded(reinterpret_cast<uint64_t*>(__cvta_shared_to_generic(bar)), parity);
+  if (bar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!bar_try(bar, parity))
+    if (clock64() - t0 > (1ll << 32)) return false;
+  return true;
 }
 
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* tm, int x, int y, uint32_t bar) {
@@ -29,15 +50,34 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* tm, int 
       : "memory");
 }
 
+__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* tm, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
+      "{%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(tm), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+
 // Shared-memory operand, K-major, 128-byte swizzle: 8-row groups 1024 bytes apart.
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3fffu) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 |
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-__device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-               : "memory");
+// One lane of a converged warp. The warp that issues MMAs runs its whole loop converged and hands this to
+// each MMA and commit as a predicate: descriptors and addresses then stay in uniform registers (in a branch
+// of one lane every MMA waits some 100 cycles for its operands to get there).
+__device__ __forceinline__ uint32_t elect() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is;
+}
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t one) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(one)
+      : "memory");
 }
 __device__ __forceinline__ void fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -69,6 +109,9 @@ __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.la
 
 }  // namespace tc5
 
+// 4D map of 16-bit values, boxes of box0 x box1 x 1 x 1, 128-byte swizzle; strides in bytes.
+cudaError_t tma_half_map(CUtensorMap* tm, const void* ptr, const uint64_t (&dim)[4], const uint64_t (&stride)[3],
+                         uint32_t box0, uint32_t box1);
 // 2D byte tensor map [rows][cols], row stride `pitch` bytes, boxes of box_x bytes by box_y rows.
 cudaError_t tma_byte_map(CUtensorMap* tm, const void* ptr, int64_t rows, int64_t cols, int64_t pitch,
                          uint32_t box_x, uint32_t box_y, CUtensorMapSwizzle sw);
