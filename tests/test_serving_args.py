@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import vtq
+from tests import _serving_abi as A
 from vtq import serving as S
 
 FAKE = 1 << 20  # an aligned address that nothing reads
@@ -13,75 +14,54 @@ FAKE = 1 << 20  # an aligned address that nothing reads
 
 def refused(fn, want, text, *args):
     assert fn(*args) == want
-    assert text in S._lib().vtq_device_last_error().decode()
-
-
-def test_structures_match_the_header():
-    """Every field of the header's structures, in order and size."""
-    import os
-    import re
-    src = open(os.path.join(os.path.dirname(__file__), "..", "include", "vtq.h")).read()
-    src = re.sub(r"/\*.*?\*/", "", src, flags=re.S)
-    size = {"int64_t": ctypes.c_int64, "int32_t": ctypes.c_int32, "uint32_t": ctypes.c_uint32, "float": ctypes.c_float,
-            "vtq_paged_kv": S._PagedKV}
-    for cls in (S._LinearI8, S._PagedKV, S._AppendKV, S._Attention, S._Verify):
-        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (cls.__name__, cls.__name__), src, flags=re.S).group(1)
-        fields = []
-        for decl in body.split(";"):
-            m = re.match(r"\s*(?:const )?(\w+)\s*(.*)", decl.strip(), flags=re.S)
-            if not m or not m.group(2):
-                continue
-            for name in m.group(2).split(","):
-                name = name.strip()
-                fields.append((name.lstrip("* "), ctypes.c_void_p if "*" in name else size[m.group(1)]))
-        assert fields == list(cls._fields_)
+    assert text in A.last_error()
 
 
 def test_quantize_tokens():
-    f = S._lib().vtq_quantize_tokens
-    refused(f, vtq.ERR_NOT_IMPLEMENTED, "not F32", S.I8, FAKE, 8, 1, 8, FAKE, 16, FAKE, None)
-    refused(f, vtq.ERR_INTERNAL, "shape", S.F32, FAKE, 8, -1, 8, FAKE, 16, FAKE, None)
-    refused(f, vtq.ERR_INTERNAL, "shape", S.F32, FAKE, 8, 1, 8, FAKE, 7, FAKE, None)
-    refused(f, vtq.ERR_INVALID_ARG, "null", S.F32, None, 8, 1, 8, FAKE, 16, FAKE, None)
-    assert f(S.F32, None, 8, 0, 8, None, 8, None, None) == vtq.OK
+    f = A.function("vtq_quantize_tokens")
+    refused(f, vtq.ERR_NOT_IMPLEMENTED, "not F32", A.I8, FAKE, 8, 1, 8, FAKE, 16, FAKE, None)
+    refused(f, vtq.ERR_INTERNAL, "shape", A.F32, FAKE, 8, -1, 8, FAKE, 16, FAKE, None)
+    refused(f, vtq.ERR_INTERNAL, "shape", A.F32, FAKE, 8, 1, 8, FAKE, 7, FAKE, None)
+    refused(f, vtq.ERR_INVALID_ARG, "null", A.F32, None, 8, 1, 8, FAKE, 16, FAKE, None)
+    assert f(A.F32, None, 8, 0, 8, None, 8, None, None) == vtq.OK
 
 
 def i8_args(**kw):
     a = dict(x=FAKE, x_scale=None, w=FAKE, w_scale=FAKE, bias=None, y=FAKE, ldx=64, ldw=64, ldy=32, tokens=4, in_feat=64,
-             out_feat=32, x_dtype=S.F32, y_dtype=S.F32, status=None)
+             out_feat=32, x_dtype=A.F32, y_dtype=A.F32, status=None)
     a.update(kw)
-    return S._LinearI8(**a)
+    return A.LinearI8(**a)
 
 
 @pytest.mark.parametrize("kw,want,text", [
-    (dict(x_dtype=7), vtq.ERR_NOT_IMPLEMENTED, "x not"), (dict(y_dtype=S.I8), vtq.ERR_NOT_IMPLEMENTED, "y not"),
+    (dict(x_dtype=7), vtq.ERR_NOT_IMPLEMENTED, "x not"), (dict(y_dtype=A.I8), vtq.ERR_NOT_IMPLEMENTED, "y not"),
     (dict(in_feat=0), vtq.ERR_INTERNAL, "shape"), (dict(tokens=-1), vtq.ERR_INTERNAL, "shape"),
     (dict(ldw=48), vtq.ERR_INTERNAL, "shape"), (dict(in_feat=131073, ldw=131088), vtq.ERR_NOT_IMPLEMENTED, "131072"),
     (dict(tokens=(1 << 20) + 1), vtq.ERR_NOT_IMPLEMENTED, "tokens"), (dict(w=None), vtq.ERR_INVALID_ARG, "null"),
     (dict(w=FAKE + 8), vtq.ERR_INTERNAL, "16-byte"), (dict(ldw=72), vtq.ERR_INTERNAL, "multiple of 16"),
-    (dict(x_dtype=S.I8), vtq.ERR_INVALID_ARG, "null"), (dict(x_dtype=S.I8, x_scale=FAKE, ldx=65), vtq.ERR_INTERNAL, "codes"),
+    (dict(x_dtype=A.I8), vtq.ERR_INVALID_ARG, "null"), (dict(x_dtype=A.I8, x_scale=FAKE, ldx=65), vtq.ERR_INTERNAL, "codes"),
     (dict(), vtq.ERR_INVALID_ARG, "workspace")])
 def test_linear_i8(kw, want, text):
-    refused(S._lib().vtq_linear_i8, want, text, ctypes.byref(i8_args(**kw)), None, 0, None)
+    refused(A.function("vtq_linear_i8"), want, text, ctypes.byref(i8_args(**kw)), None, 0, None)
 
 
 def test_linear_i8_nothing_to_do():
-    f = S._lib().vtq_linear_i8
+    f = A.function("vtq_linear_i8")
     assert f(ctypes.byref(i8_args(tokens=0, x=None, y=None)), None, 0, None) == vtq.OK
     refused(f, vtq.ERR_INVALID_ARG, "null", None, None, 0, None)
-    assert S._lib().vtq_linear_i8_workspace_bytes(S.I8, 100, 64, 64) == 0
-    assert S._lib().vtq_linear_i8_workspace_bytes(S.F32, 3, 100, 64) >= 3 * 112 + 3 * 4
+    assert A.function("vtq_linear_i8_workspace_bytes")(A.I8, 100, 64, 64) == 0
+    assert A.function("vtq_linear_i8_workspace_bytes")(A.F32, 3, 100, 64) >= 3 * 112 + 3 * 4
 
 
 def kv_args(**kw):
     a = dict(k=FAKE, v=FAKE, k_page=4096, k_slot=256, k_head=64, v_page=4096, v_slot=256, v_head=64, table=FAKE, table_ld=8,
-             table_width=8, seqs=2, pages=16, page_size=16, kv_heads=4, head_dim=64, dtype=S.F16)
+             table_width=8, seqs=2, pages=16, page_size=16, kv_heads=4, head_dim=64, dtype=A.F16)
     a.update(kw)
-    return S._PagedKV(**a)
+    return A.PagedKV(**a)
 
 
 BAD_CACHES = [
-    (dict(dtype=S.F32), vtq.ERR_NOT_IMPLEMENTED, "F16"), (dict(page_size=0), vtq.ERR_INTERNAL, "shape"),
+    (dict(dtype=A.F32), vtq.ERR_NOT_IMPLEMENTED, "F16"), (dict(page_size=0), vtq.ERR_INTERNAL, "shape"),
     (dict(head_dim=60), vtq.ERR_NOT_IMPLEMENTED, "head_dim"), (dict(head_dim=264), vtq.ERR_NOT_IMPLEMENTED, "head_dim"),
     (dict(k=None), vtq.ERR_INVALID_ARG, "null"), (dict(table=None), vtq.ERR_INVALID_ARG, "null"),
     (dict(v=FAKE + 2), vtq.ERR_INTERNAL, "aligned"), (dict(k_slot=257), vtq.ERR_INTERNAL, "aligned"),
@@ -90,39 +70,39 @@ BAD_CACHES = [
 
 def append_args(kv=None, **kw):
     a = dict(kv=kv_args(**(kv or {})), k=FAKE, v=FAKE, q=None, q_out=None, k_tok=256, k_head=64, v_tok=256, v_head=64, seq=FAKE,
-             pos=FAKE, rope=FAKE, rot_dim=64, max_pos=100, tokens=3, heads=0, x_dtype=S.F32, flags=0)
+             pos=FAKE, rope=FAKE, rot_dim=64, max_pos=100, tokens=3, heads=0, x_dtype=A.F32, flags=0)
     a.update(kw)
-    return S._AppendKV(**a)
+    return A.AppendKV(**a)
 
 
 @pytest.mark.parametrize("kv,want,text", BAD_CACHES)
 def test_append_refuses_caches(kv, want, text):
-    refused(S._lib().vtq_append_kv, want, text, ctypes.byref(append_args(kv)), None)
+    refused(A.function("vtq_append_kv"), want, text, ctypes.byref(append_args(kv)), None)
 
 
 @pytest.mark.parametrize("kw,want,text", [
-    (dict(x_dtype=S.I8), vtq.ERR_NOT_IMPLEMENTED, "k / v"), (dict(tokens=-2), vtq.ERR_INTERNAL, "shape"),
+    (dict(x_dtype=A.I8), vtq.ERR_NOT_IMPLEMENTED, "k / v"), (dict(tokens=-2), vtq.ERR_INTERNAL, "shape"),
     (dict(rot_dim=63), vtq.ERR_INTERNAL, "rot_dim"), (dict(rot_dim=66), vtq.ERR_INTERNAL, "rot_dim"),
     (dict(rot_dim=0), vtq.ERR_INTERNAL, "rot_dim"), (dict(rope=None), vtq.ERR_INTERNAL, "rot_dim"),
     (dict(rope=FAKE + 4), vtq.ERR_INTERNAL, "rope"), (dict(k=None), vtq.ERR_INVALID_ARG, "null"),
     (dict(q=FAKE, heads=0), vtq.ERR_INTERNAL, "shape"), (dict(q=FAKE, heads=4), vtq.ERR_INVALID_ARG, "null")])
 def test_append(kw, want, text):
-    refused(S._lib().vtq_append_kv, want, text, ctypes.byref(append_args(**kw)), None)
+    refused(A.function("vtq_append_kv"), want, text, ctypes.byref(append_args(**kw)), None)
 
 
 def attention_args(kv=None, **kw):
     a = dict(kv=kv_args(**(kv or {})), q=FAKE, out=FAKE, lse=None, q_tok=512, q_head=64, o_tok=512, o_head=64, lse_tok=8,
              q_start=None, kv_len=FAKE, tokens=2, heads=8, shared_len=0, scale=0.1, status=None)
     a.update(kw)
-    return S._Attention(**a)
+    return A.Attention(**a)
 
 
 @pytest.mark.parametrize("kv,want,text", BAD_CACHES + [
     (dict(seqs=1025), vtq.ERR_NOT_IMPLEMENTED, "sequences"), (dict(table_width=1 << 27), vtq.ERR_NOT_IMPLEMENTED, "positions")])
 def test_attention_refuses_caches(kv, want, text):
     a = attention_args(kv)
-    assert S._lib().vtq_attention_paged_workspace_bytes(ctypes.byref(a)) == 0 or "null" in text
-    refused(S._lib().vtq_attention_paged, want, text, ctypes.byref(a), None, 0, None)
+    assert A.function("vtq_attention_paged_workspace_bytes")(ctypes.byref(a)) == 0 or "null" in text
+    refused(A.function("vtq_attention_paged"), want, text, ctypes.byref(a), None, 0, None)
 
 
 @pytest.mark.parametrize("kw,want,text", [
@@ -130,26 +110,26 @@ def test_attention_refuses_caches(kv, want, text):
     (dict(q=None), vtq.ERR_INVALID_ARG, "null"), (dict(tokens=1 << 21), vtq.ERR_NOT_IMPLEMENTED, "tokens"),
     (dict(), vtq.ERR_INVALID_ARG, "workspace")])
 def test_attention(kw, want, text):
-    refused(S._lib().vtq_attention_paged, want, text, ctypes.byref(attention_args(**kw)), None, 0, None)
+    refused(A.function("vtq_attention_paged"), want, text, ctypes.byref(attention_args(**kw)), None, 0, None)
 
 
 def verify_args(**kw):
     a = dict(draft=FAKE, n_draft=None, target=FAKE, proposal=None, u=FAKE, tokens=FAKE, accepted=FAKE, ld_draft=2, target_seq=30,
-             target_row=10, ld_u=3, ld_tokens=3, seqs=4, drafts=2, vocab=10, dtype=S.F32)
+             target_row=10, ld_u=3, ld_tokens=3, seqs=4, drafts=2, vocab=10, dtype=A.F32)
     a.update(kw)
-    return S._Verify(**a)
+    return A.Verify(**a)
 
 
 @pytest.mark.parametrize("kw,want,text", [
-    (dict(dtype=S.I8), vtq.ERR_NOT_IMPLEMENTED, "rows"), (dict(vocab=0), vtq.ERR_INTERNAL, "shape"),
+    (dict(dtype=A.I8), vtq.ERR_NOT_IMPLEMENTED, "rows"), (dict(vocab=0), vtq.ERR_INTERNAL, "shape"),
     (dict(seqs=-1), vtq.ERR_INTERNAL, "shape"), (dict(vocab=1 << 25), vtq.ERR_NOT_IMPLEMENTED, "2^24"),
     (dict(draft=None), vtq.ERR_INVALID_ARG, "null"), (dict(target=None), vtq.ERR_INVALID_ARG, "null"),
     (dict(tokens=None), vtq.ERR_INVALID_ARG, "null")])
 def test_verify(kw, want, text):
-    for f in (S._lib().vtq_verify_draft, S._lib().vtq_verify_greedy):
+    for f in (A.function("vtq_verify_draft"), A.function("vtq_verify_greedy")):
         refused(f, want, text, ctypes.byref(verify_args(**kw)), None)
         assert f(ctypes.byref(verify_args(seqs=0)), None) == vtq.OK
-    refused(S._lib().vtq_verify_draft, vtq.ERR_INVALID_ARG, "null", ctypes.byref(verify_args(u=None)), None)
+    refused(A.function("vtq_verify_draft"), vtq.ERR_INVALID_ARG, "null", ctypes.byref(verify_args(u=None)), None)
 
 
 def test_python_refuses_cpu_tensors_and_wrong_arguments():

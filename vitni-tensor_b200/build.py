@@ -1,4 +1,5 @@
-"""Build the sm_100a shared library ``vtq/libvtq.so`` in-tree with nvcc.
+"""Build the sm_100a shared library ``vtq/libvtq.so`` in-tree with nvcc, and the torch
+binding of the batched serving operators, ``vtq/_serving.so``, with the host compiler.
 
 Usage: python vitni-tensor_b200/build.py [--force]
 Every .cu under csrc/ is compiled for sm_100a only, with fp32 contraction
@@ -6,6 +7,7 @@ disabled (-fmad=false): bit parity with the reference depends on every fp32
 multiply and add being rounded separately.
 """
 import os
+import shutil
 import subprocess
 import sys
 
@@ -30,7 +32,7 @@ def sources():
 def deps():
     out = []
     for d in (CSRC, os.path.join(HERE, "..", "include")):
-        out += [os.path.join(d, f) for f in os.listdir(d)]
+        out += [os.path.join(d, f) for f in os.listdir(d) if not f.endswith(".cpp")]
     return out
 
 
@@ -56,5 +58,30 @@ def build(force=False, verbose=False):
     return OUT
 
 
+def build_binding(force=False, verbose=False):
+    """vtq/_serving.so from csrc/serving_bind.cpp, against this interpreter's torch and libvtq.so."""
+    src, out = os.path.join(CSRC, "serving_bind.cpp"), os.path.join(HERE, "vtq", "_serving.so")
+    header = os.path.join(HERE, "..", "include", "vtq.h")
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(p) for p in (src, header)):
+        return out
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    nvcc = shutil.which(os.environ.get("NVCC", "nvcc"))
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc)))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", src, "-o", out,
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(cuda, "include"),
+           *("-I" + p for p in cpp_extension.include_paths()), "-L" + lib, "-ltorch_python", "-ltorch", "-ltorch_cpu",
+           "-ltorch_cuda", "-lc10", "-lc10_cuda", "-L" + os.path.join(HERE, "vtq"), "-l:libvtq.so", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+    return out
+
+
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose=True))
+    print(build_binding(force="--force" in sys.argv, verbose=True))
