@@ -1,0 +1,263 @@
+// attention_plan.cuh -- attention_paged: parameters, the cut of the work that every CTA derives from the
+// lengths on the device, and small pieces that both kinds of work use.
+#pragma once
+#include <type_traits>
+
+#include "serve.h"
+#include "tc5.cuh"
+#include "vtq_internal.h"
+
+namespace vtq {
+
+namespace {
+
+constexpr int kRows = 16;      // query rows of a segment: M of the MMA
+constexpr int kTileRows = 128; // of a segment of the prefix on tcgen05
+constexpr int kMaxSeqs = 1024;
+
+struct AttnParams {
+  vtq_attention_args a;
+  int group;        // query heads of a kv head
+  int tile;         // keys of a part's tile
+  int ctas, warps;  // of the grid; warps of a CTA that take parts
+  int box;          // positions of a TMA box: a page, or an even part of it; 0: none, rows are gathered
+  int keys_max;     // positions that the table can hold
+  int prefix;       // min(shared_len, keys_max)
+  float scale_log2;
+  bool q_wide, o_wide;  // q rows can be read, rows of out written, four bytes at a time
+  int4* rows;       // for the joining kernel: each token's Row,
+  int2* seg_parts;  // the first and the last part of each segment,
+  int2* seg_ctas;   // and the first and last CTA of each segment of the prefix's own tiles
+  float* part;      // slots of kRows (m, l) and o
+  int dim_padded;
+  // The prefix on the tensor cores' own tiles (attention_tile.cuh), where on_tiles is set:
+  bool on_tiles, q_copies;           // q_copies: q rows can be copied 16 bytes at a time
+  int tile_rt, tile_streams;         // blocks of kTileRows rows of a segment; softmax warpgroups of a CTA
+  int tile_segs, tiles_each;         // segments of a kv head, steps (of tile_streams / tile_rt key tiles) of each
+  int tiles_total;                   // steps in all
+  int step_cost, part_cost;          // what a CTA takes for a step, and for a part's tile
+  float* tile_part;                  // slots of kTileRows (m, l) and o
+};
+
+// What the joining kernel has to know of a token, as an int4: x its sequence's first segment (-1: no keys of
+// its own), y its first row among the sequence's rows, z the first segment of the prefix (-1: it does not see
+// it, or there is none; 0 where the prefix has its own tiles), w whether any sequence owns it.
+
+// The cut of the work: prefix sums over the sequences (index B: the shared prefix). Tiles before, and
+// segments before, each sequence; its first query row; its length.
+struct Plan {
+  int *tiles, *segs, *q0, *len;  // [B + 2], [B + 2], [B + 1], [B + 1] (len[B]: of the prefix, 0 if nobody sees it)
+};
+__host__ __device__ inline int plan_ints(int B) { return 4 * (B + 2) + 4; }
+
+__device__ __forceinline__ Plan plan_of(int* base, int B) {
+  return Plan{base + 4, base + 4 + (B + 2), base + 4 + 2 * (B + 2), base + 4 + 3 * (B + 2)};
+}
+
+__device__ __forceinline__ int seq_rows(const Plan& pl, int b) { return pl.q0[b + 1] - pl.q0[b]; }
+
+// Whether every row of a sequence sees the whole prefix. The rows of one that does not (it ends inside
+// the prefix, or is empty) take no part in the prefix's segments: it has all its keys for its own, so
+// that those segments need no mask for rows, and what they hold cannot reach a row that must not see it.
+__device__ __forceinline__ bool sees_prefix(const AttnParams& p, const Plan& pl, int b) {
+  const int n = seq_rows(pl, b);
+  return n > 0 && pl.len[b] - n + 1 >= p.prefix;
+}
+
+// Built by all threads of a CTA in its shared memory; base[0] = the parts' tiles in all, base[1] = parts in
+// use, base[2] = CTAs that work on the prefix's own tiles (the first ones), by the two sides' cost.
+__device__ void build_plan(const AttnParams& p, int* base) {
+  const int B = (int)p.a.kv.seqs, T = (int)p.a.tokens, H = (int)p.a.kv.kv_heads;
+  const Plan pl = plan_of(base, B);
+  __shared__ int s_any, s_bad, s_warp_t[32], s_warp_s[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) s_any = s_bad = 0;
+  __syncthreads();
+  for (int b = tid; b <= B; b += blockDim.x) {
+    pl.q0[b] = p.a.q_start ? min(max(p.a.q_start[b], 0), T) : min(b, T);
+    if (b < B) pl.len[b] = max(p.a.kv_len[b], 0);
+  }
+  __syncthreads();
+  for (int b = tid; b < B; b += blockDim.x) {
+    if (pl.q0[b + 1] < pl.q0[b]) s_bad = 1;
+    else if (sees_prefix(p, pl, b)) s_any = 1;
+  }
+  __syncthreads();
+  if (tid == 0) pl.len[B] = s_any && !s_bad ? p.prefix : 0;
+  if (s_bad) {  // row starts that decrease: no sequence owns a row (the slots are counted for one owner a row)
+    for (int b = tid; b <= B; b += blockDim.x) pl.q0[b] = 0;
+    if (tid == 0 && p.a.status) atomicOr(p.a.status, SERVE_BAD_INDEX);
+    __syncthreads();
+  }
+  // Inclusive sums over runs of consecutive sequences, one run a thread.
+  const int n = B + 1, per = (n + (int)blockDim.x - 1) / (int)blockDim.x, b0 = min(tid * per, n), b1 = min(b0 + per, n);
+  int st = 0, ss = 0;
+  for (int pass = 0; pass < 2; pass++) {
+    for (int b = b0; b < b1; b++) {
+      int rows, keys;
+      if (b < B) {
+        rows = seq_rows(pl, b) * p.group;
+        keys = min(pl.len[b], p.keys_max);
+        if (sees_prefix(p, pl, b)) keys = keys > p.prefix ? keys - p.prefix / p.tile * p.tile : 0;
+      } else {
+        rows = p.on_tiles ? 0 : T * p.group;  // the prefix has a kernel of its own then
+        keys = pl.len[B];
+      }
+      const int segs = (rows + kRows - 1) / kRows * H;
+      if (pass) pl.tiles[b] = st, pl.segs[b] = ss;
+      st += segs * ((keys + p.tile - 1) / p.tile);
+      ss += segs;
+    }
+    if (pass == 0) {
+      int it = st, is = ss;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, it, o), y = __shfl_up_sync(0xffffffffu, is, o);
+        if (lane >= o) it += x, is += y;
+      }
+      if (lane == 31) s_warp_t[warp] = it, s_warp_s[warp] = is;
+      __syncthreads();
+      int ot = it - st, os = is - ss;
+      for (int w = 0; w < warp; w++) ot += s_warp_t[w], os += s_warp_s[w];
+      st = ot, ss = os;
+    }
+  }
+  if (b0 < n && b1 == n) pl.tiles[n] = st, pl.segs[n] = ss;
+  __syncthreads();
+  if (tid == 0) {
+    const int64_t steps = p.on_tiles && pl.len[B] ? p.tiles_total : 0, tiles = pl.tiles[n];
+    const int64_t a = steps * p.step_cost, b = tiles * p.part_cost;
+    int x = 0;
+    if (steps) x = tiles ? (int)min(max((p.ctas * a + (a + b) / 2) / (a + b), (int64_t)1), (int64_t)p.ctas - 1) : p.ctas;
+    x = (int)min((int64_t)x, steps);
+    base[0] = (int)tiles;
+    base[1] = (int)min(tiles, (int64_t)(p.ctas - x) * p.warps);
+    base[2] = x;
+    base[3] = pl.segs[B];
+  }
+  __syncthreads();
+}
+
+// Part w of W covers tiles [first(w), first(w + 1)) of `total`; part_of is its inverse.
+__device__ __forceinline__ int first_tile(int total, int W, int w) { return (int)((int64_t)total * w / W); }
+__device__ __forceinline__ int part_of(int total, int W, int t) { return (int)((((int64_t)t + 1) * W - 1) / total); }
+
+// Where a part stands: sequence, row block, head, tile. Tiles lie on multiples of their size, so that pages
+// and boxes do not straddle them: the first one of a sequence behind the prefix may begin inside it.
+struct Cursor {
+  int b, mb, g, t, nt;  // nt tiles in a segment of b
+  int mbs;              // row blocks of b
+  int first, lo, end;   // of b: its first tile's position; its keys are lo .. end
+};
+
+__device__ __forceinline__ int seq_tiles(const AttnParams& p, const Plan& pl, int b, int B, int* mbs) {
+  const int H = (int)p.a.kv.kv_heads;
+  *mbs = (pl.segs[b + 1] - pl.segs[b]) / H;
+  const int segs = *mbs * H;
+  return segs ? (pl.tiles[b + 1] - pl.tiles[b]) / segs : 0;
+}
+
+__device__ __forceinline__ void enter(const AttnParams& p, const Plan& pl, int B, Cursor& c) {
+  c.nt = seq_tiles(p, pl, c.b, B, &c.mbs);
+  c.lo = c.b < B && sees_prefix(p, pl, c.b) ? p.prefix : 0;
+  c.first = c.lo / p.tile * p.tile;
+  c.end = c.b < B ? min(pl.len[c.b], p.keys_max) : pl.len[B];
+}
+
+__device__ Cursor seek(const AttnParams& p, const Plan& pl, int B, int tile) {
+  int lo = 0, hi = B;  // the last index whose tiles begin at or before `tile`
+  while (lo < hi) {
+    const int m = (lo + hi + 1) >> 1;
+    if (pl.tiles[m] <= tile) lo = m;
+    else hi = m - 1;
+  }
+  Cursor c;
+  c.b = lo;
+  enter(p, pl, B, c);
+  const int at = tile - pl.tiles[lo], seg = c.nt ? at / c.nt : 0, H = (int)p.a.kv.kv_heads;
+  c.t = at - seg * c.nt;
+  c.mb = seg / H;
+  c.g = seg - c.mb * H;
+  return c;
+}
+
+// The next tile; true where it begins another segment. Never called behind the last tile.
+__device__ __forceinline__ bool advance(const AttnParams& p, const Plan& pl, int B, Cursor& c) {
+  if (++c.t < c.nt) return false;
+  c.t = 0;
+  if (++c.g == (int)p.a.kv.kv_heads) {
+    c.g = 0;
+    if (++c.mb == c.mbs) {
+      c.mb = 0;
+      do {
+        if (++c.b <= B) enter(p, pl, B, c);
+      } while (c.b <= B && c.nt == 0);
+    }
+  }
+  return true;
+}
+
+// The sequence that owns a row of q, or -1.
+__device__ __forceinline__ int owner(const Plan& pl, int B, int token) {
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int m = (lo + hi + 1) >> 1;
+    if (pl.q0[m] <= token) lo = m;
+    else hi = m - 1;
+  }
+  return token >= pl.q0[lo] && token < pl.q0[lo + 1] ? lo : -1;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  const int n = there ? 16 : 0;  // 0: the 16 bytes are filled with zeros, nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+// Whether either half of a word is an infinity or a NaN.
+template <typename T>
+__device__ __forceinline__ bool odd_word(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (w & e) == e || ((w >> 16) & e) == e;
+}
+
+}  // namespace
+}  // namespace vtq
