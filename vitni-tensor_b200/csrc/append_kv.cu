@@ -3,10 +3,10 @@
 //
 //   (a, b) -> (a cos - b sin, a sin + b cos),  cos / sin of pos * frequency from a 32-bit table
 //
-// Bound: HBM by bytes (each input read once, each output written once), latency for a decode step.
-// One CTA takes one token; each of its threads takes one unit of 16 values (a rotated unit: 8 pairs)
-// or 8 (values that are not rotated), so that a decode step has every load in flight at once: the
-// inputs' loads do not wait for the table's, which need pos, seq and the page number first.
+// Bound: HBM by bytes (each input read once, each output written once), latency for a decode step. A
+// thread takes a unit: 16 bytes of neighbouring values (and, where the pairs are (i, i + rot / 2), the 16
+// bytes of their partners), so that a warp's loads and stores are whole lines: two neighbouring 16-byte
+// pieces a thread instead keep L1 half busy with the same sectors twice.
 #include <algorithm>
 
 #include "serve.h"
@@ -17,152 +17,229 @@ namespace {
 
 struct AppendParams {
   vtq_append_kv_args a;
-  int rot_units, rest_units;  // of one q / k head: units of 2 VEC rotated values, units of VEC others
-  int v_units;                // of one v head: units of VEC values
+  int rot_units, rest_units;  // of one q / k head: rotated units, units of W other values
+  int v_units;                // of one v head
   int units;                  // of a token
 };
 
-// VEC consecutive values as 32-bit floats.
-template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
-  if constexpr (VEC == 8 && sizeof(T) == 2) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = to_f32(e[i]);
-  } else if constexpr (VEC == 8) {
-    const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+// W consecutive values as they lie in memory; WIDE: in 16-byte pieces.
+template <typename X, int W, bool WIDE>
+struct alignas(WIDE ? 16 : sizeof(X)) Raw {
+  X v[W];
+};
+template <typename X, int W, bool WIDE>
+__device__ __forceinline__ Raw<X, W, WIDE> load_raw(const X* p) {
+  Raw<X, W, WIDE> r;
+  if constexpr (WIDE) {
+    static_assert(sizeof(X) * W == 16, "one load");
+    *reinterpret_cast<uint4*>(&r) = *reinterpret_cast<const uint4*>(p);
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; i++) v[i] = to_f32(p[i]);
+    for (int i = 0; i < W; i++) r.v[i] = p[i];
+  }
+  return r;
+}
+
+template <typename C, int W, bool WIDE>
+__device__ __forceinline__ void store(C* p, const float (&v)[W]) {
+  if constexpr (WIDE) {
+    struct alignas(2 * W) {
+      C e[W];
+    } w;
+#pragma unroll
+    for (int i = 0; i < W; i++) w.e[i] = from_f32<C>(v[i]);
+    if constexpr (W == 8) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(&w);
+    else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(&w);
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; i++) p[i] = from_f32<C>(v[i]);
   }
 }
 
-template <typename C, int VEC>
-__device__ __forceinline__ void store_vec(C* p, const float (&v)[VEC]) {
-  if constexpr (VEC == 8) {
-    uint4 w;
-    C* e = reinterpret_cast<C*>(&w);
+// P pairs' (cos, sin).
+template <int P, bool WIDE>
+__device__ __forceinline__ void load_turn(const float* cs, float (&c)[P], float (&s)[P]) {
+  if constexpr (WIDE) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) e[i] = from_f32<C>(v[i]);
-    *reinterpret_cast<uint4*>(p) = w;
+    for (int i = 0; i < P; i += 2) {
+      const float4 w = *reinterpret_cast<const float4*>(cs + 2 * i);
+      c[i] = w.x, s[i] = w.y, c[i + 1] = w.z, s[i + 1] = w.w;
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; i++) p[i] = from_f32<C>(v[i]);
+    for (int i = 0; i < P; i++) {
+      const float2 w = *reinterpret_cast<const float2*>(cs + 2 * i);
+      c[i] = w.x;
+      s[i] = w.y;
+    }
   }
 }
 
-template <typename X, typename C, int VEC>
-__global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ AppendParams p) {
+// Where a token goes: offsets of its slot in the caches (-1: nowhere) and its position (-1: the token is
+// left out altogether).
+struct Place {
+  int64_t k, v;
+  int pos;
+};
+__device__ __forceinline__ Place place_of(const vtq_append_kv_args& a, int64_t t) {
+  Place w{-1, -1, -1};
+  const int seq = a.seq[t];
+  if (seq < 0) return w;  // padding
+  const int pos = a.pos[t], page_size = (int)a.kv.page_size;
+  int64_t page = -1;
+  if (pos >= 0 && (!a.rope || pos < a.max_pos)) {
+    w.pos = pos;
+    if (seq < a.kv.seqs && pos / page_size < a.kv.table_width) page = a.kv.table[seq * a.kv.table_ld + pos / page_size];
+  }
+  if (page >= 0 && page < a.kv.pages) {
+    w.k = page * a.kv.k_page + pos % page_size * a.kv.k_slot;
+    w.v = page * a.kv.v_page + pos % page_size * a.kv.v_slot;
+  } else if (a.status) {
+    atomicOr(a.status, SERVE_BAD_INDEX);
+  }
+  return w;
+}
+
+// A CTA takes an even share of the tokens, TOK at a time: one thread a token finds its place, then every
+// thread has its unit of U tokens at a time, the next ones' values on their way. (Every thread finding the place itself makes the divisions
+// most of the kernel: 51 us on 8081 tokens of 32 + 2 x 4 fp32 heads of 64.) HALF: a unit is W values and
+// their W partners; otherwise W values, pairs of neighbours.
+template <typename X, typename C, int W, int TOK, bool HALF, bool WIDE>
+__global__ void __launch_bounds__(TOK > 1 ? 256 : 512, TOK > 1 ? 4 : 1) append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int P = HALF ? W : W / 2;  // pairs of a rotated unit
+  constexpr int U = TOK < 4 ? TOK : HALF ? (W == 8 ? 1 : 2) : W == 8 ? 2 : 4;
+  __shared__ Place s_place[TOK];
   const vtq_append_kv_args& a = p.a;
-  const int64_t t = blockIdx.x;
-  const int seq = a.seq[t], pos = a.pos[t];
-  if (seq < 0) return;  // padding
   const int head_units = p.rot_units + p.rest_units;
   const int q_units = a.q ? (int)a.heads * head_units : 0, k_units = (int)a.kv.kv_heads * head_units;
   const int half = (int)a.rot_dim / 2;
-  const bool by_half = a.flags & VTQ_ROPE_HALF;
-  bool turnable = pos >= 0 && (!a.rope || pos < a.max_pos);
-  int64_t page = -1;
-  if (turnable && seq < a.kv.seqs && pos / a.kv.page_size < a.kv.table_width) {
-    page = a.kv.table[seq * a.kv.table_ld + pos / a.kv.page_size];
-    if (page >= a.kv.pages) page = -1;
-  }
-  const int64_t slot = pos >= 0 ? pos % a.kv.page_size : 0;
-  if (page < 0 && threadIdx.x == 0 && a.status) atomicOr(a.status, SERVE_BAD_INDEX);
-  if (!turnable) return;
-  for (int u = threadIdx.x; u < p.units; u += blockDim.x) {
-    const X* src;
-    C* dst = nullptr;
-    int at;  // unit within the head
-    bool is_v = false;
-    if (u < q_units) {
-      const int h = u / head_units;
-      at = u - h * head_units;
-      src = static_cast<const X*>(a.q) + t * a.q_tok + h * a.q_head;
-      dst = static_cast<C*>(a.q_out) + t * a.qo_tok + h * a.qo_head;
-    } else if (u < q_units + k_units) {
-      const int h = (u - q_units) / head_units;
-      at = u - q_units - h * head_units;
-      src = static_cast<const X*>(a.k) + t * a.k_tok + h * a.k_head;
-      if (page >= 0) dst = static_cast<C*>(a.kv.k) + page * a.kv.k_page + slot * a.kv.k_slot + h * a.kv.k_head;
-    } else {
-      const int h = (u - q_units - k_units) / p.v_units;
-      at = u - q_units - k_units - h * p.v_units;
-      src = static_cast<const X*>(a.v) + t * a.v_tok + h * a.v_head;
-      if (page >= 0) dst = static_cast<C*>(a.kv.v) + page * a.kv.v_page + slot * a.kv.v_slot + h * a.kv.v_head;
-      is_v = true;
-    }
-    if (!is_v && at < p.rot_units) {
-      // VEC pairs: (i, i + half), or two neighbours.
-      const int e0 = by_half ? at * VEC : 2 * at * VEC, e1 = by_half ? e0 + half : e0 + VEC;
-      float x[VEC], y[VEC], c[VEC], s[VEC];
-      load_vec<X, VEC>(src + e0, x);
-      load_vec<X, VEC>(src + e1, y);
-      const float* cs = a.rope + ((int64_t)pos * half + at * VEC) * 2;
-#pragma unroll
-      for (int i = 0; i < VEC; i++) {
-        const float2 w = *reinterpret_cast<const float2*>(cs + 2 * i);
-        c[i] = w.x;
-        s[i] = w.y;
-      }
-      float r0[VEC], r1[VEC];
-      if (by_half) {
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-          r0[i] = x[i] * c[i] - y[i] * s[i];
-          r1[i] = x[i] * s[i] + y[i] * c[i];
-        }
+  const int64_t end = TOK == 1 ? blockIdx.x + 1 : a.tokens * (blockIdx.x + 1) / gridDim.x;
+  for (int64_t t0 = TOK == 1 ? blockIdx.x : a.tokens * blockIdx.x / gridDim.x; t0 < end; t0 += TOK) {
+    const int tokens = TOK == 1 ? 1 : (int)min((int64_t)TOK, end - t0);
+    for (int u0 = 0; u0 < p.units; u0 += blockDim.x) {
+      const int u = min(u0 + (int)threadIdx.x, p.units - 1);
+      const X* src;
+      C* out;
+      int64_t src_tok;
+      int at, h;  // unit within the head, head
+      int kind;   // 0 q, 1 k, 2 v
+      if (u < q_units) {
+        kind = 0, h = u / head_units, at = u - h * head_units;
+        src = static_cast<const X*>(a.q) + h * a.q_head, src_tok = a.q_tok;
+        out = static_cast<C*>(a.q_out) + t0 * a.qo_tok + h * a.qo_head;
+      } else if (u < q_units + k_units) {
+        kind = 1, h = (u - q_units) / head_units, at = u - q_units - h * head_units;
+        src = static_cast<const X*>(a.k) + h * a.k_head, src_tok = a.k_tok;
+        out = static_cast<C*>(a.kv.k) + h * a.kv.k_head;
       } else {
-        float z[2 * VEC], r[2 * VEC];
+        kind = 2, h = (u - q_units - k_units) / p.v_units, at = u - q_units - k_units - h * p.v_units;
+        src = static_cast<const X*>(a.v) + h * a.v_head, src_tok = a.v_tok;
+        out = static_cast<C*>(a.kv.v) + h * a.kv.v_head;
+      }
+      const bool mine = u0 + (int)threadIdx.x < p.units, turn = kind < 2 && at < p.rot_units;
+      const int e = turn || kind == 2 ? at * W : (int)a.rot_dim + (at - p.rot_units) * W;
+      src += t0 * src_tok + e;
+      out += e;
+      const float* cs = a.rope + at * P * 2;
+      Raw<X, W, WIDE> x[U], y[HALF ? U : 1];
+      auto load = [&](int i0) {
 #pragma unroll
-        for (int i = 0; i < VEC; i++) z[i] = x[i], z[VEC + i] = y[i];
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-          r[2 * i] = z[2 * i] * c[i] - z[2 * i + 1] * s[i];
-          r[2 * i + 1] = z[2 * i] * s[i] + z[2 * i + 1] * c[i];
+        for (int i = 0; i < U; i++) {
+          const int t = min(i0 + i, tokens - 1);
+          x[i] = load_raw<X, W, WIDE>(src + t * src_tok);
+          if (HALF && turn) y[HALF ? i : 0] = load_raw<X, W, WIDE>(src + t * src_tok + half);
         }
+      };
+      load(0);
+      Place only{};  // one token: every thread finds its place itself, rather than wait for one that does
+      if constexpr (TOK == 1) {
+        only = place_of(a, t0);
+      } else if (u0 == 0) {
+        __syncthreads();  // the places before have been used
+        if (threadIdx.x < tokens) s_place[threadIdx.x] = place_of(a, t0 + threadIdx.x);
+        __syncthreads();
+      }
+      for (int i0 = 0; i0 < tokens; i0 += U) {
+        Raw<X, W, WIDE> x0[U], y0[HALF ? U : 1];
+        float c[U][P], s[U][P];
 #pragma unroll
-        for (int i = 0; i < VEC; i++) r0[i] = r[i], r1[i] = r[VEC + i];
+        for (int i = 0; i < U; i++) {
+          x0[i] = x[i];
+          if (HALF) y0[HALF ? i : 0] = y[HALF ? i : 0];
+          const int pos = TOK == 1 ? only.pos : s_place[min(i0 + i, tokens - 1)].pos;
+          if (turn) load_turn<P, WIDE>(cs + (int64_t)max(pos, 0) * half * 2, c[i], s[i]);
+        }
+        if (i0 + U < tokens) load(i0 + U);
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+          if (!mine || i0 + i >= tokens) continue;
+          const Place& w = TOK == 1 ? only : s_place[i0 + i];
+          const int64_t to = kind == 0 ? (w.pos < 0 ? -1 : (i0 + i) * a.qo_tok) : kind == 1 ? w.k : w.v;
+          if (to < 0) continue;
+          float r[W];
+#pragma unroll
+          for (int k = 0; k < W; k++) r[k] = to_f32(x0[i].v[k]);
+          if (turn) {
+            if constexpr (HALF) {
+              float o[W];
+#pragma unroll
+              for (int k = 0; k < W; k++) {
+                const float b = to_f32(y0[i].v[k]);
+                o[k] = r[k] * s[i][k] + b * c[i][k];
+                r[k] = r[k] * c[i][k] - b * s[i][k];
+              }
+              store<C, W, WIDE>(out + to + half, o);
+            } else {
+#pragma unroll
+              for (int k = 0; k < P; k++) {
+                const float b = r[2 * k + 1];
+                r[2 * k + 1] = r[2 * k] * s[i][k] + b * c[i][k];
+                r[2 * k] = r[2 * k] * c[i][k] - b * s[i][k];
+              }
+            }
+          }
+          store<C, W, WIDE>(out + to, r);
+        }
       }
-      if (dst) {
-        store_vec<C, VEC>(dst + e0, r0);
-        store_vec<C, VEC>(dst + e1, r1);
-      }
-    } else {
-      const int e0 = is_v ? at * VEC : (int)a.rot_dim + (at - p.rot_units) * VEC;
-      float x[VEC];
-      load_vec<X, VEC>(src + e0, x);
-      if (dst) store_vec<C, VEC>(dst + e0, x);
     }
   }
+}
+
+template <typename X, typename C, int W, bool HALF, bool WIDE>
+cudaError_t run(const vtq_append_kv_args& a, cudaStream_t st) {
+  const int dim = (int)a.kv.head_dim, rot = (int)a.rot_dim;
+  AppendParams p;
+  p.a = a;
+  p.rot_units = rot / (HALF ? 2 * W : W);
+  p.rest_units = (dim - rot) / W;
+  p.v_units = dim / W;
+  p.units = (int)((a.q ? a.heads : 0) + a.kv.kv_heads) * (p.rot_units + p.rest_units) + (int)a.kv.kv_heads * p.v_units;
+  // Even passes over a token's units: of 512 threads for one token (latency), of 256 where several CTAs have
+  // to fit an SM.
+  const bool many = a.tokens > 4 * num_sms();
+  const int most = many ? 256 : 512, passes = (p.units + most - 1) / most;
+  const int threads = ((p.units + passes - 1) / passes + 31) / 32 * 32;
+  // A decode step's few tokens go one to a CTA, for latency; many in even shares to as many as fit at once.
+  kernel_launch_count()++;
+  if (many)
+    append_kernel<X, C, W, 32, HALF, WIDE><<<(unsigned)(num_sms() * std::max(1, 1024 / threads)), threads, 0, st>>>(p);
+  else
+    append_kernel<X, C, W, 1, HALF, WIDE><<<(unsigned)a.tokens, threads, 0, st>>>(p);
+  return cudaGetLastError();
 }
 
 template <typename X, typename C>
 cudaError_t launch(const vtq_append_kv_args& a, cudaStream_t st) {
+  constexpr int W = 16 / sizeof(X);
+  const bool by_half = a.flags & VTQ_ROPE_HALF;
   const int dim = (int)a.kv.head_dim, rot = (int)a.rot_dim;
-  // 16-byte accesses where every head begins on one and the pairs come in whole units.
-  constexpr int kX = 16 / sizeof(X);
-  auto strides_ok = [](int64_t s0, int64_t s1, int64_t m) { return s0 % m == 0 && s1 % m == 0; };
-  const bool wide = ((a.flags & VTQ_ROPE_HALF) ? rot % 16 == 0 : rot % 16 == 0) && (dim - rot) % 8 == 0 &&
-                    aligned16(a.k) && aligned16(a.v) && strides_ok(a.k_tok, a.k_head, kX) &&
-                    strides_ok(a.v_tok, a.v_head, kX) &&
-                    (!a.q || (aligned16(a.q) && aligned16(a.q_out) && strides_ok(a.q_tok, a.q_head, kX) &&
-                              strides_ok(a.qo_tok, a.qo_head, 8)));
-  const int vec = wide ? 8 : 1;
-  AppendParams p;
-  p.a = a;
-  p.rot_units = rot / (2 * vec);
-  p.rest_units = (dim - rot) / vec;
-  p.v_units = dim / vec;
-  p.units = (int)((a.q ? a.heads : 0) + a.kv.kv_heads) * (p.rot_units + p.rest_units) +
-            (int)a.kv.kv_heads * p.v_units;
-  const int threads = std::min(512, (p.units + 31) / 32 * 32);
-  kernel_launch_count()++;
-  if (wide) append_kernel<X, C, 8><<<(unsigned)a.tokens, threads, 0, st>>>(p);
-  else append_kernel<X, C, 1><<<(unsigned)a.tokens, threads, 0, st>>>(p);
-  return cudaGetLastError();
+  // 16-byte loads where every head begins on one and units come whole.
+  auto fits = [](const void* p, int64_t s0, int64_t s1, int64_t m) { return aligned16(p) && s0 % m == 0 && s1 % m == 0; };
+  const bool wide = rot % (by_half ? 2 * W : W) == 0 && (dim - rot) % W == 0 && aligned16(a.rope) &&
+                    fits(a.k, a.k_tok, a.k_head, W) && fits(a.v, a.v_tok, a.v_head, W) &&
+                    (!a.q || (fits(a.q, a.q_tok, a.q_head, W) && fits(a.q_out, a.qo_tok, a.qo_head, W)));
+  if (by_half) return wide ? run<X, C, W, true, true>(a, st) : run<X, C, 1, true, false>(a, st);
+  return wide ? run<X, C, W, false, true>(a, st) : run<X, C, 2, false, false>(a, st);
 }
 
 }  // namespace
