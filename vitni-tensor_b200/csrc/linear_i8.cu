@@ -124,7 +124,10 @@ cudaError_t launch_quantize(const X* x, int64_t ldx, int64_t tokens, int64_t n, 
                             float* scale, cudaStream_t st) {
   const bool wide = aligned16(x) && ldx % (16 / (int)sizeof(X)) == 0;
   const bool wide_q = (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && ldq % 8 == 0;
-  const int threads = (int)std::min<int64_t>(kQThreads, std::max<int64_t>(32, ((n + 7) / 8 + 31) / 32 * 32));
+  // Few tokens: a row over as many threads as it has 16 bytes for, for latency. Many: 32 values a thread, so
+  // that more rows are in flight.
+  const int64_t each = tokens <= 2 * num_sms() ? 8 : 32;
+  const int threads = (int)std::min<int64_t>(kQThreads, std::max<int64_t>(32, ((n + each - 1) / each + 31) / 32 * 32));
   kernel_launch_count()++;
   quantize_kernel<X><<<(unsigned)tokens, threads, 0, st>>>(x, ldx, n, wide, q, ldq, wide_q, scale);
   return cudaGetLastError();
@@ -285,17 +288,196 @@ __global__ void __launch_bounds__(kThreads)
   }
   if (splits > 1) {
     cl.sync();
-    if (warp >= 2) {
-      const int row = 32 * (warp & 3) + lane, o = o0 + row;
-      const float wsc = o < p.N ? p.ws[o] : 0.0f, b = p.bias && o < p.N ? p.bias[o] : 0.0f;
-      for (int c = rank; c < NT && t0 + c < p.T; c += splits) {
-        int acc = 0;
-        for (int s = 0; s < splits; s++) acc += cl.map_shared_rank(part, s)[c * BM + row];
-        if (o < p.N && !*abort_flag) store_y<Y>(p, t0 + c, o, acc, wsc, b);
+    // Token c of the tile is added up by CTA c mod splits: a warp a token, a lane four channels, two tokens'
+    // parts from all CTAs in flight at once (one 4-byte load after the other: 60 us at 256 tokens).
+    const int o = o0 + 4 * lane;
+    float wsc[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      wsc[i] = o + i < p.N ? p.ws[o + i] : 0.0f;
+      b[i] = p.bias && o + i < p.N ? p.bias[o + i] : 0.0f;
+    }
+    const int last = min(NT, p.T - t0);
+    for (int c0 = rank + splits * warp; c0 < last; c0 += 2 * splits * (kThreads / 32)) {
+      int4 v[2][8];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int c = c0 + h * splits * (kThreads / 32);
+#pragma unroll
+        for (int s = 0; s < 8; s++)
+          if (s < splits && c < last) v[h][s] = reinterpret_cast<const int4*>(cl.map_shared_rank(part, s) + c * BM)[lane];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int c = c0 + h * splits * (kThreads / 32);
+        if (c >= last || *abort_flag) continue;
+        int acc[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < 8; s++)
+          if (s < splits) acc[0] += v[h][s].x, acc[1] += v[h][s].y, acc[2] += v[h][s].z, acc[3] += v[h][s].w;
+        const float xs = p.xs[t0 + c];
+        Y* y = static_cast<Y*>(p.y) + (int64_t)(t0 + c) * p.ldy + o;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          float r = __int2float_rn(acc[i]) * (xs * wsc[i]);
+          if (p.bias) r += b[i];
+          if (o + i < p.N) y[i] = from_f32<Y>(r);
+        }
       }
     }
     cl.sync();  // no CTA leaves while another still reads its part
   }
+}
+
+// Many tokens: persistent CTAs, each walking tiles of 128 channels x 256 tokens. Two accumulators of 256
+// columns in TMEM, so that one tile is stored while the next one is summed; the operand ring runs on across
+// tiles.
+constexpr int PN = 256, kPStages = 4, kPEpiWarps = 8, kPThreads = 64 + 32 * kPEpiWarps;
+constexpr uint32_t kPStage = A_STAGE + PN * 128;
+
+template <typename Y>
+__global__ void __launch_bounds__(kPThreads, 1)
+    i8_wide_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx,
+                   const __grid_constant__ I8Params p, int tiles, int token_tiles) {
+  constexpr uint32_t kIdesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(PN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t s_bar[2 * kPStages + 4];
+  __shared__ uint32_t s_slot;
+  __shared__ int s_abort;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  auto FULL = [&](int i) { return smem_u32(&s_bar[i]); };
+  auto EMPTY = [&](int i) { return smem_u32(&s_bar[kPStages + i]); };
+  auto ACC_FULL = [&](int i) { return smem_u32(&s_bar[2 * kPStages + i]); };
+  auto ACC_EMPTY = [&](int i) { return smem_u32(&s_bar[2 * kPStages + 2 + i]); };
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nk = p.kblocks;
+  volatile int* abort_flag = &s_abort;
+  if (tid == 0) {
+    for (int i = 0; i < kPStages; i++) {
+      tc5::bar_init(FULL(i), 1);
+      tc5::bar_init(EMPTY(i), 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      tc5::bar_init(ACC_FULL(i), 1);
+      tc5::bar_init(ACC_EMPTY(i), kPEpiWarps);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tc5::alloc(smem_u32(&s_slot), 512);
+  tc5::fence_before();
+  __syncthreads();
+  tc5::fence_after();
+  const uint32_t tmem = s_slot;
+  auto fail = [&]() {
+    record_error(p.status, KERR_TIMEOUT);
+    *abort_flag = 1;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tc5::grid_wait();  // the codes
+      int g = 0;
+      for (int u = blockIdx.x; u < tiles && !*abort_flag; u += gridDim.x) {
+        const int o0 = u / token_tiles * BM, t0 = u % token_tiles * PN;
+        for (int k = 0; k < nk; k++, g++) {
+          const int s = g % kPStages;
+          if (g >= kPStages && !tc5::bar_wait(EMPTY(s), tc5::phase(g, kPStages, true))) {
+            fail();
+            break;
+          }
+          tc5::bar_expect(FULL(s), kPStage);
+          tc5::tma_2d(base + s * kPStage, &tmw, k * 128, o0, FULL(s));
+          tc5::tma_2d(base + s * kPStage + A_STAGE, &tmx, k * 128, t0, FULL(s));
+        }
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t one = tc5::elect();
+    int g = 0, n = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; u < tiles && ok; u += gridDim.x, n++) {
+      const int acc = n & 1;
+      ok = n < 2 || tc5::bar_wait(ACC_EMPTY(acc), tc5::phase(n, 2, true));
+      for (int k = 0; k < nk && ok; k++, g++) {
+        const int s = g % kPStages;
+        ok = tc5::bar_wait(FULL(s), tc5::phase(g, kPStages));
+        if (!ok) break;
+        tc5::fence_after();
+        const uint32_t sa = base + s * kPStage, sb = sa + A_STAGE;
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+          mma_i8(tmem + acc * PN, tc5::desc_sw128(sa + 32 * c), tc5::desc_sw128(sb + 32 * c), kIdesc, (k | c) ? 1u : 0u, one);
+        tc5::commit(EMPTY(s), one);
+      }
+      if (ok) tc5::commit(ACC_FULL(acc), one);
+    }
+    if (!ok && lane == 0) fail();
+  } else {
+    tc5::grid_wait();  // the token scales
+    const int quad = warp & 3, half = (warp - 2) >> 2, row = 32 * quad + lane;
+    int n = 0;
+    for (int u = blockIdx.x; u < tiles; u += gridDim.x, n++) {
+      const int acc = n & 1, o = u / token_tiles * BM + row, t0 = u % token_tiles * PN + half * (PN / 2);
+      if (!tc5::bar_wait(ACC_FULL(acc), tc5::phase(n, 2))) {
+        if (lane == 0) fail();
+        break;
+      }
+      tc5::fence_after();
+      const float wsc = o < p.N ? p.ws[o] : 0.0f, b = p.bias && o < p.N ? p.bias[o] : 0.0f;
+      Y* y = static_cast<Y*>(p.y) + (int64_t)t0 * p.ldy + o;
+      const uint32_t at = tmem + ((uint32_t)(32 * quad) << 16) + acc * PN + half * (PN / 2);
+#pragma unroll 1
+      for (int c = 0; c < PN / 2; c += 32) {
+        uint32_t r[32];
+        float xs[32];
+        tc5::ld16(at + c, *reinterpret_cast<uint32_t(*)[16]>(r));
+        tc5::ld16(at + c + 16, *reinterpret_cast<uint32_t(*)[16]>(r + 16));
+        const bool all = t0 + c + 32 <= p.T;
+        // Each lane reads one token's scale; they are passed round below.
+        const float mine = t0 + c + lane < p.T ? p.xs[t0 + c + lane] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; i++) xs[i] = __shfl_sync(0xffffffffu, mine, i);
+        tc5::wait_ld();
+        if (o < p.N) {
+#pragma unroll
+          for (int i = 0; i < 32; i++) {
+            float v = __int2float_rn((int)r[i]) * (xs[i] * wsc);
+            if (p.bias) v += b;
+            if (all || t0 + c + i < p.T) y[(int64_t)(c + i) * p.ldy] = from_f32<Y>(v);
+          }
+        }
+      }
+      tc5::fence_before();
+      __syncwarp();
+      if (lane == 0) tc5::bar_arrive(ACC_EMPTY(acc));
+    }
+  }
+  tc5::fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc5::fence_after();
+    tc5::dealloc(tmem, 512);
+  }
+}
+
+template <typename Y>
+cudaError_t launch_wide(const CUtensorMap& tmw, const CUtensorMap& tmx, const I8Params& p, bool pdl, cudaStream_t st) {
+  constexpr size_t smem = (size_t)kPStages * kPStage + 1024;
+  cudaError_t e = cudaFuncSetAttribute(i8_wide_kernel<Y>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  const int token_tiles = (p.T + PN - 1) / PN, tiles = (p.N + BM - 1) / BM * token_tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min(tiles, num_sms()));
+  cfg.blockDim = dim3(kPThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl && pdl_enabled() ? 1 : 0;
+  kernel_launch_count()++;
+  return cudaLaunchKernelEx(&cfg, i8_wide_kernel<Y>, tmw, tmx, p, tiles, token_tiles);
 }
 
 template <int NT, int STAGES, typename Y>
@@ -329,7 +511,7 @@ cudaError_t product(const CUtensorMap& tmw, const CUtensorMap& tmx, const I8Para
     case 32: return launch_tile<32, 5, Y>(tmw, tmx, p, splits, pdl, st);
     case 64: return launch_tile<64, 4, Y>(tmw, tmx, p, splits, pdl, st);
     case 128: return launch_tile<128, 3, Y>(tmw, tmx, p, splits, pdl, st);
-    default: return launch_tile<256, 4, Y>(tmw, tmx, p, splits, pdl, st);
+    default: return splits > 1 ? launch_tile<256, 4, Y>(tmw, tmx, p, splits, pdl, st) : launch_wide<Y>(tmw, tmx, p, pdl, st);
   }
 }
 
@@ -399,8 +581,9 @@ vtq_status vtq_linear_i8(const vtq_linear_i8_args* a, void* ws, size_t ws_bytes,
   const int T = (int)a->tokens, kb = (int)((a->in_feat + 127) / 128);
   const int nt = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
   const int64_t tiles = (a->out_feat + BM - 1) / BM * ((T + nt - 1) / nt);
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= 2 * num_sms() && kb >= splits * 4) splits *= 2;
+  // Two CTAs of a tile of up to 128 tokens fit an SM, one of 256.
+  const int64_t room = (nt == 256 ? 1 : 2) * num_sms();
+  const int splits = (int)std::max<int64_t>(1, std::min<int64_t>({8, room / tiles, kb / 2}));
   CUtensorMap tmw, tmx;
   cudaError_t e = tma_byte_map(&tmw, a->w, a->out_feat, a->in_feat, a->ldw, 128, BM, CU_TENSOR_MAP_SWIZZLE_128B);
   if (e == cudaSuccess) e = tma_byte_map(&tmx, q, T, a->in_feat, ldq, 128, (uint32_t)nt, CU_TENSOR_MAP_SWIZZLE_128B);
