@@ -26,16 +26,23 @@ namespace {
 
 constexpr int kQThreads = 512, kQKeep = 4;  // values kept in registers: 4 x 8 a thread
 
-// Round-half-even of the real quotient x / s. The product with 1 / s is at most one off; the
-// remainder x - q s is exact in 32 bits (both are multiples of a common power of two and it is
-// no larger than s), so comparing it with s / 2 decides.
-__device__ __forceinline__ int code(float x, float s, float inv) {
-  float q = rintf(x * inv);
-  const float rem = fmaf(-q, s, x), h = 0.5f * s;
-  const bool odd = ((int)q) & 1;
-  if (rem > h || (rem == h && odd)) q += 1.0f;
-  else if (rem < -h || (rem == -h && odd)) q -= 1.0f;
-  return max(-127, min(127, (int)q));
+// Round-half-even of the real quotient x / s, as the low byte of a word. x / s is first rounded as the
+// product with 1 / s, by adding 1.5 * 2^23, whose last bits are then the whole number: at most one off. The
+// remainder x - q s is exact in 32 bits (both are multiples of a common power of two and it is no larger
+// than s), so comparing it with s / 2 tells whether q was right; only quotients next to a half get there.
+__device__ __forceinline__ uint32_t code(float x, float s, float inv, float look) {
+  constexpr float kMagic = 12582912.0f;
+  float t = fmaf(x, inv, kMagic);
+  const float q = __fsub_rn(t, kMagic), rem = fmaf(-q, s, x);
+  if (fabsf(rem) >= look) {
+    const float h = 0.5f * s;
+    const bool odd = ((int)q) & 1;
+    if (rem > h || (rem == h && odd)) t = __fadd_rn(t, 1.0f);
+    else if (rem < -h || (rem == -h && odd)) t = __fsub_rn(t, 1.0f);
+    // A scale rounded down in the subnormals leaves quotients over 127.
+    t = fminf(fmaxf(t, kMagic - 127.0f), kMagic + 127.0f);
+  }
+  return __float_as_uint(t);
 }
 
 template <typename X>
@@ -91,15 +98,19 @@ __global__ void __launch_bounds__(kQThreads)
   float s = finite ? __fdiv_rn(__uint_as_float(m), 127.0f) : __uint_as_float(0x7fc00000u);
   if (threadIdx.x == 0) scale[blockIdx.x] = s;
   const bool some = finite && s > 0.0f;
-  const float up = s < 1e-30f ? 18446744073709551616.0f : 1.0f;  // keeps 1 / s finite; exact on both
+  const bool tiny = s < 1e-30f;
+  const float up = tiny ? 18446744073709551616.0f : 1.0f;  // keeps 1 / s finite; exact on both
   s = s * up;
+  const float look = tiny ? 0.0f : 0.5f * s;  // 0: every quotient is looked at, for those over 127
   const float inv = some ? __fdiv_rn(1.0f, s) : 0.0f;
   auto put = [&](int64_t i, const float (&v)[8]) {
-    uint32_t w[2] = {0, 0};
+    uint32_t c[8], w[2] = {0, 0};
+    if (some) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const int c = some ? code(v[e] * up, s, inv) : 0;
-      w[e >> 2] |= (uint32_t)(c & 0xff) << (8 * (e & 3));
+      for (int e = 0; e < 8; e++) c[e] = code(tiny ? v[e] * up : v[e], s, inv, look);
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+        w[e] = __byte_perm(__byte_perm(c[4 * e], c[4 * e + 1], 0x0040), __byte_perm(c[4 * e + 2], c[4 * e + 3], 0x0040), 0x5410);
     }
     if (wide_q && i + 8 <= n) {
       *reinterpret_cast<uint2*>(out + i) = make_uint2(w[0], w[1]);
@@ -329,26 +340,63 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// Many tokens: persistent CTAs, each walking tiles of 128 channels x 256 tokens. Two accumulators of 256
-// columns in TMEM, so that one tile is stored while the next one is summed; the operand ring runs on across
-// tiles.
-constexpr int PN = 256, kPStages = 4, kPEpiWarps = 8, kPThreads = 64 + 32 * kPEpiWarps;
-constexpr uint32_t kPStage = A_STAGE + PN * 128;
+// Many tokens: persistent pairs of CTAs (cta_group::2), each walking tiles of 256 channels x 256 tokens. A
+// CTA brings 128 channels and 128 tokens, 32 KB for 2^22 products: at the 62 bytes a cycle that L2 gives an
+// SM here this feeds the tensor cores, where a CTA by itself (128 x 256, 48 KB) waits: 93 us against 65 on
+// 2048 x 4096 x 14336. The leader (rank 0) issues the products for both; barriers that only it waits for are
+// its own, signalled from the peer. Two accumulators of 256 columns in TMEM, so that one tile is stored while
+// the next one is summed; the operand ring runs on across tiles.
+constexpr int PM = 256, PN = 256, kPStages = 6, kPEpiWarps = 8, kPThreads = 64 + 32 * kPEpiWarps;
+constexpr uint32_t kPHalf = 128 * 128, kPStage = 2 * kPHalf;
+
+__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one));
+}
+// Arrives at the barrier of this offset in both CTAs once the products so far are done.
+__device__ __forceinline__ void commit_pair(uint32_t bar, uint32_t one) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t.reg .b16 m;\n\tsetp.ne.b32 q, %1, 0;\n\tmov.b16 m, 3;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}" ::"r"(bar),
+      "r"(one)
+      : "memory");
+}
+// The address of a shared location of this CTA's in the pair's leader.
+__device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+// A load into this CTA that completes on a barrier of the leader's.
+__device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap* tm, int x, int y, uint32_t leader_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, "
+      "{%2, %3}], [%4];" ::"r"(dst),
+      "l"(tm), "r"(x), "r"(y), "r"(leader_bar)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 
 template <typename Y>
-__global__ void __launch_bounds__(kPThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
     i8_wide_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx,
                    const __grid_constant__ I8Params p, int tiles, int token_tiles) {
-  constexpr uint32_t kIdesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(PN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+  constexpr uint32_t kIdesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(PN >> 3) << 17) | ((uint32_t)(PM >> 4) << 24);
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_bar[2 * kPStages + 4];
   __shared__ uint32_t s_slot;
   __shared__ int s_abort;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  auto FULL = [&](int i) { return smem_u32(&s_bar[i]); };
-  auto EMPTY = [&](int i) { return smem_u32(&s_bar[kPStages + i]); };
+  auto FULL = [&](int i) { return smem_u32(&s_bar[i]); };                 // the leader's: both CTAs' operands are there
+  auto EMPTY = [&](int i) { return smem_u32(&s_bar[kPStages + i]); };     // each CTA's own
   auto ACC_FULL = [&](int i) { return smem_u32(&s_bar[2 * kPStages + i]); };
-  auto ACC_EMPTY = [&](int i) { return smem_u32(&s_bar[2 * kPStages + 2 + i]); };
+  auto ACC_EMPTY = [&](int i) { return smem_u32(&s_bar[2 * kPStages + 2 + i]); };  // the leader's
+  cg::cluster_group cl = cg::this_cluster();
+  const int rank = (int)cl.block_rank(), first = (int)blockIdx.x / 2, step = (int)gridDim.x / 2;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nk = p.kblocks;
   volatile int* abort_flag = &s_abort;
   if (tid == 0) {
@@ -358,14 +406,17 @@ __global__ void __launch_bounds__(kPThreads, 1)
     }
     for (int i = 0; i < 2; i++) {
       tc5::bar_init(ACC_FULL(i), 1);
-      tc5::bar_init(ACC_EMPTY(i), kPEpiWarps);
+      tc5::bar_init(ACC_EMPTY(i), 2 * kPEpiWarps);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tc5::alloc(smem_u32(&s_slot), 512);
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_slot)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
   tc5::fence_before();
-  __syncthreads();
+  cl.sync();
   tc5::fence_after();
   const uint32_t tmem = s_slot;
   auto fail = [&]() {
@@ -377,47 +428,50 @@ __global__ void __launch_bounds__(kPThreads, 1)
     if (lane == 0) {
       tc5::grid_wait();  // the codes
       int g = 0;
-      for (int u = blockIdx.x; u < tiles && !*abort_flag; u += gridDim.x) {
-        const int o0 = u / token_tiles * BM, t0 = u % token_tiles * PN;
+      for (int u = first; u < tiles && !*abort_flag; u += step) {
+        const int o0 = u / token_tiles * PM + rank * 128, t0 = u % token_tiles * PN + rank * 128;
         for (int k = 0; k < nk; k++, g++) {
           const int s = g % kPStages;
           if (g >= kPStages && !tc5::bar_wait(EMPTY(s), tc5::phase(g, kPStages, true))) {
             fail();
             break;
           }
-          tc5::bar_expect(FULL(s), kPStage);
-          tc5::tma_2d(base + s * kPStage, &tmw, k * 128, o0, FULL(s));
-          tc5::tma_2d(base + s * kPStage + A_STAGE, &tmx, k * 128, t0, FULL(s));
+          const uint32_t full = in_leader(FULL(s)), at = base + s * kPStage;
+          if (rank == 0) tc5::bar_expect(FULL(s), 2 * kPStage);
+          tma_2d_pair(at, &tmw, k * 128, o0, full);
+          tma_2d_pair(at + kPHalf, &tmx, k * 128, t0, full);
         }
       }
     }
   } else if (warp == 1) {
-    const uint32_t one = tc5::elect();
-    int g = 0, n = 0;
-    bool ok = true;
-    for (int u = blockIdx.x; u < tiles && ok; u += gridDim.x, n++) {
-      const int acc = n & 1;
-      ok = n < 2 || tc5::bar_wait(ACC_EMPTY(acc), tc5::phase(n, 2, true));
-      for (int k = 0; k < nk && ok; k++, g++) {
-        const int s = g % kPStages;
-        ok = tc5::bar_wait(FULL(s), tc5::phase(g, kPStages));
-        if (!ok) break;
-        tc5::fence_after();
-        const uint32_t sa = base + s * kPStage, sb = sa + A_STAGE;
+    if (rank == 0) {
+      const uint32_t one = tc5::elect();
+      int g = 0, n = 0;
+      bool ok = true;
+      for (int u = first; u < tiles && ok; u += step, n++) {
+        const int acc = n & 1;
+        ok = n < 2 || tc5::bar_wait(ACC_EMPTY(acc), tc5::phase(n, 2, true));
+        for (int k = 0; k < nk && ok; k++, g++) {
+          const int s = g % kPStages;
+          ok = tc5::bar_wait(FULL(s), tc5::phase(g, kPStages));
+          if (!ok) break;
+          tc5::fence_after();
+          const uint32_t sa = base + s * kPStage, sb = sa + kPHalf;
 #pragma unroll
-        for (int c = 0; c < 4; c++)
-          mma_i8(tmem + acc * PN, tc5::desc_sw128(sa + 32 * c), tc5::desc_sw128(sb + 32 * c), kIdesc, (k | c) ? 1u : 0u, one);
-        tc5::commit(EMPTY(s), one);
+          for (int c = 0; c < 4; c++)
+            mma_i8_pair(tmem + acc * PN, tc5::desc_sw128(sa + 32 * c), tc5::desc_sw128(sb + 32 * c), kIdesc, (k | c) ? 1u : 0u, one);
+          commit_pair(EMPTY(s), one);
+        }
+        if (ok) commit_pair(ACC_FULL(acc), one);
       }
-      if (ok) tc5::commit(ACC_FULL(acc), one);
+      if (!ok && lane == 0) fail();
     }
-    if (!ok && lane == 0) fail();
   } else {
     tc5::grid_wait();  // the token scales
     const int quad = warp & 3, half = (warp - 2) >> 2, row = 32 * quad + lane;
     int n = 0;
-    for (int u = blockIdx.x; u < tiles; u += gridDim.x, n++) {
-      const int acc = n & 1, o = u / token_tiles * BM + row, t0 = u % token_tiles * PN + half * (PN / 2);
+    for (int u = first; u < tiles; u += step, n++) {
+      const int acc = n & 1, o = u / token_tiles * PM + rank * 128 + row, t0 = u % token_tiles * PN + half * (PN / 2);
       if (!tc5::bar_wait(ACC_FULL(acc), tc5::phase(n, 2))) {
         if (lane == 0) fail();
         break;
@@ -449,14 +503,14 @@ __global__ void __launch_bounds__(kPThreads, 1)
       }
       tc5::fence_before();
       __syncwarp();
-      if (lane == 0) tc5::bar_arrive(ACC_EMPTY(acc));
+      if (lane == 0) arrive_remote(in_leader(ACC_EMPTY(acc)));
     }
   }
   tc5::fence_before();
-  __syncthreads();
+  cl.sync();  // the leader's products read the peer's operands and write its accumulators
   if (warp == 1) {
     tc5::fence_after();
-    tc5::dealloc(tmem, 512);
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }
 }
 
@@ -465,9 +519,9 @@ cudaError_t launch_wide(const CUtensorMap& tmw, const CUtensorMap& tmx, const I8
   constexpr size_t smem = (size_t)kPStages * kPStage + 1024;
   cudaError_t e = cudaFuncSetAttribute(i8_wide_kernel<Y>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  const int token_tiles = (p.T + PN - 1) / PN, tiles = (p.N + BM - 1) / BM * token_tiles;
+  const int token_tiles = (p.T + PN - 1) / PN, tiles = (p.N + PM - 1) / PM * token_tiles;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min(tiles, num_sms()));
+  cfg.gridDim = dim3((unsigned)(2 * std::min(tiles, num_sms() / 2)));
   cfg.blockDim = dim3(kPThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -586,7 +640,9 @@ vtq_status vtq_linear_i8(const vtq_linear_i8_args* a, void* ws, size_t ws_bytes,
   const int splits = (int)std::max<int64_t>(1, std::min<int64_t>({8, room / tiles, kb / 2}));
   CUtensorMap tmw, tmx;
   cudaError_t e = tma_byte_map(&tmw, a->w, a->out_feat, a->in_feat, a->ldw, 128, BM, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (e == cudaSuccess) e = tma_byte_map(&tmx, q, T, a->in_feat, ldq, 128, (uint32_t)nt, CU_TENSOR_MAP_SWIZZLE_128B);
+  // The wide kernel's CTAs bring 128 tokens each.
+  const uint32_t token_box = nt == 256 && splits == 1 ? 128 : (uint32_t)nt;
+  if (e == cudaSuccess) e = tma_byte_map(&tmx, q, T, a->in_feat, ldq, 128, token_box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (e != cudaSuccess) return serve_cuda(e, fn);
   const I8Params p{T, (int)a->in_feat, (int)a->out_feat, kb, xs, a->w_scale, a->bias, a->y, a->ldy, a->status};
   if (a->y_dtype == VTQ_F32) e = product<float>(tmw, tmx, p, nt, splits, !codes, st);
