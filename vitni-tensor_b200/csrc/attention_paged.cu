@@ -37,9 +37,9 @@ struct Part<T, 256> { static constexpr int KT = 16, WARPS = 8; };
 template <typename T, int DP, int RT>
 struct Tile;
 template <typename T, int RT>
-struct Tile<T, 64, RT> { static constexpr int KT = 64, STREAMS = 2, NSLOT = 14; };
+struct Tile<T, 64, RT> { static constexpr int KT = 128, STREAMS = 2, NSLOT = 8; };
 template <typename T, int RT>
-struct Tile<T, 128, RT> { static constexpr int KT = 64, STREAMS = 2, NSLOT = RT == 2 ? 10 : 12; };
+struct Tile<T, 128, RT> { static constexpr int KT = 128, STREAMS = 2, NSLOT = RT == 2 ? 5 : 6; };
 template <typename T>
 struct Tile<T, 256, 1> { static constexpr int KT = 64, STREAMS = 1, NSLOT = 5; };
 
@@ -205,7 +205,7 @@ TileCut tile_cut(const vtq_attention_args& a) {
   const int64_t rows = a.tokens * (a.heads / a.kv.kv_heads), prefix = std::min(a.shared_len, a.kv.table_width * a.kv.page_size);
   c.on = rows > 16 && prefix >= 512;
   const bool wide = a.kv.head_dim > 128;
-  c.keys = 64;
+  c.keys = wide ? 64 : 128;
   c.streams = wide ? 1 : 2;
   c.rt = !wide && rows > kTileRows ? 2 : 1;
   c.segs = (int)((rows + kTileRows * c.rt - 1) / (kTileRows * c.rt));
@@ -354,9 +354,9 @@ vtq_status vtq_attention_paged(const vtq_attention_args* a, void* ws, size_t ws_
     p.tile_segs = c.segs;
     p.tiles_each = c.each;
     p.tiles_total = (int)c.total;
-    // Cycles of an SM, measured (head_dim 128: a step of 64 keys and 256 rows; a part's tile of 32 keys).
-    p.step_cost = 1700;
-    p.part_cost = 400;
+    // Cycles of an SM, measured (head_dim 128: a step of 128 keys and 256 rows; a part's tile of 32 keys).
+    p.step_cost = 4200;
+    p.part_cost = 520;
     p.tile_part = reinterpret_cast<float*>(at + part_bytes(*a));
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);

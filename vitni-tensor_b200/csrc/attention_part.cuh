@@ -136,7 +136,7 @@ __device__ __forceinline__ void part_role(const AttnParams& p, const CUtensorMap
   };
 
   Cursor c = seek(p, pl, B, tile0), in = c;
-  Tile now, next = find(in, ask(in));
+  Tile next = find(in, ask(in));
   load(next, false);
   load(next, true);
   int page = -1;
@@ -199,8 +199,7 @@ __device__ __forceinline__ void part_role(const AttnParams& p, const CUtensorMap
       l0 = l1 = 0.0f;
     }
     const uint32_t parity = (uint32_t)(tile - tile0) & 1u;
-    now = next;
-    const uint32_t valid = now.valid;
+    const uint32_t valid = next.valid;
     if (!landed(k_full, parity)) break;
     const int key0 = c.first + c.t * KT;
     float sc[KT / 8][4];

@@ -2,14 +2,13 @@
 //
 // A CTA runs STREAMS streams of one softmax warpgroup each over a run of key tiles. With RT = 2 the
 // streams are two blocks of 128 query rows that share every key tile; with RT = 1 they are the even and
-// the odd key tiles of one block (two parts of the same rows, joined later). Each stream's S is
-// double-buffered in TMEM, so that its softmax finds the next tile's scores ready, and runs beside the
-// products of this one and of the other stream.
+// the odd key tiles of one block (two parts of the same rows, joined later), so that a stream's softmax
+// runs beside the other's products. (S twice for each stream, with tiles of 64 keys for TMEM's sake, is
+// slower: an MMA of 64 columns takes as long as one of 128, 5600 cycles a 256 x 128 step.)
 //   softmax warpgroups  a thread a row: S from TMEM, the weights back into TMEM as the second product's A
-//   3 loader warps      pages into a ring of swizzled K and V tiles, by TMA where a page holds 4 positions
-//                       or more (gathering rows with 16-byte copies takes three warps 5700 cycles a tile,
-//                       twice what the softmax needs)
-//   1 warp              one thread issues S = Q K^T (N = KT keys) and O += P V (V as it lies: N-major)
+//   2 loader warps      pages into a ring of swizzled K and V tiles, by TMA where a page holds 4 positions
+//                       or more (gathering rows with 16-byte copies took three warps 5700 cycles a tile)
+//   a warp a stream     one thread issues S = Q K^T (N = KT keys) and O += P V (V as it lies: N-major)
 // O stays in TMEM; it is scaled again only where a row's maximum has grown by more than 2^8 since the
 // last time, until then the weights are taken relative to the old one (at most 256, and l with them).
 // Head dims over 128 have room in TMEM for one stream.
@@ -88,7 +87,7 @@ struct TileShape {
   static constexpr int THREADS = STREAMS * 128 + 128;
   static constexpr size_t SMEM = Q_BYTES + NSLOT * SLOT;
 };
-constexpr int kLoaders = 3, kMasks = 8;
+constexpr int kLoaders = 2, kMasks = 8;
 static_assert(2 * kMasks > 14 + 1, "a mask's place must not come round before its tile's V slot has");
 
 // The role of CTA `cta` of `ctas`.
@@ -100,9 +99,9 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
   constexpr uint32_t kIdescS = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((uint32_t)(KT >> 3) << 17) | (8u << 24);
   constexpr uint32_t kIdescO = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | (8u << 24);
   constexpr int TPS = STREAMS / RT;   // key tiles of a step: 2 where the streams are the tiles
-  constexpr uint32_t kColO = 2 * STREAMS * KT;  // columns: each stream's S / P twice, then each stream's O
+  constexpr uint32_t kColO = STREAMS * KT;  // columns: each stream's S / P, then each stream's O
   constexpr int kGroups = KT / 4;     // of 4 keys: loader lw copies groups lw, lw + 3, ..
-  static_assert(STREAMS * (2 * KT + DP) <= 512 && NSLOT <= 14 && RT <= STREAMS, "TMEM, masks");
+  static_assert(STREAMS * (KT + DP) <= 512 && NSLOT <= 14 && RT <= STREAMS, "TMEM, masks");
   __shared__ __align__(8) uint64_t s_bar[2 * NSLOT + 12 + kMasks];
   __shared__ uint32_t s_valid[kMasks][kLoaders][2];
   __shared__ uint32_t s_slot;
@@ -111,10 +110,11 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
   auto bar = [&](int i) { return smem_u32(&s_bar[i]); };
   auto FULL = [&](int s) { return bar(s); };
   auto EMPTY = [&](int s) { return bar(NSLOT + s); };
-  auto S_FULL = [&](int r, int u) { return bar(2 * NSLOT + 2 * r + (u & 1)); };  // of a stream's tile u
-  auto P_FULL = [&](int r, int u) { return bar(2 * NSLOT + 4 + 2 * r + (u & 1)); };
-  auto PV_DONE = [&](int r) { return bar(2 * NSLOT + 8 + r); };  // of a stream
-  const uint32_t Q_FULL = bar(2 * NSLOT + 10), Q_EMPTY = bar(2 * NSLOT + 11);
+  auto S_FULL = [&](int r) { return bar(2 * NSLOT + r); };              // of a stream
+  auto P_FULL = [&](int r, int h) { return bar(2 * NSLOT + 2 + 2 * r + h); };  // of its P's two halves
+  auto PV_DONE = [&](int r) { return bar(2 * NSLOT + 6 + r); };
+  const uint32_t Q_FULL = bar(2 * NSLOT + 8), Q_EMPTY = bar(2 * NSLOT + 9);
+  auto TURN = [&](int r) { return bar(2 * NSLOT + 10 + r); };  // stream r may take its exponentials
   auto MASK = [&](int i) { return bar(2 * NSLOT + 12 + i); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int D = (int)p.a.kv.head_dim;
@@ -123,22 +123,21 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
   if (tid == 0) {
     for (int s = 0; s < NSLOT; s++) {
       tc5::bar_init(FULL(s), 32 * kLoaders);
-      tc5::bar_init(EMPTY(s), 1);
+      tc5::bar_init(EMPTY(s), STREAMS / TPS);  // the streams that share a tile
     }
     for (int r = 0; r < 2; r++) {
-      for (int u = 0; u < 2; u++) {
-        tc5::bar_init(S_FULL(r, u), 1);
-        tc5::bar_init(P_FULL(r, u), 128);
-      }
+      tc5::bar_init(S_FULL(r), 1);
+      for (int h = 0; h < 2; h++) tc5::bar_init(P_FULL(r, h), 128);
       tc5::bar_init(PV_DONE(r), 1);
+      tc5::bar_init(TURN(r), 128);
     }
     tc5::bar_init(Q_FULL, 32 * kLoaders);
-    tc5::bar_init(Q_EMPTY, 1);
+    tc5::bar_init(Q_EMPTY, STREAMS);
     for (int i = 0; i < kMasks; i++) tc5::bar_init(MASK(i), kLoaders);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  constexpr int kMmaWarp = 4 * STREAMS + kLoaders;
+  constexpr int kMmaWarp = 4 * STREAMS + kLoaders;  // of stream 0
   if (warp == kMmaWarp) tc5::alloc(smem_u32(&s_slot), 512);
   tc5::fence_before();
   __syncthreads();
@@ -153,6 +152,11 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
   };
   // Whether stream r has rows in a segment.
   auto live = [&](int seg, int r) { return RT == 1 || ((seg % p.tile_segs) * RT + r) * kTileRows < rows; };
+  // Word w of loader lw's part of s_valid where every key is there.
+  auto full_word = [](int lw, int w) {
+    const int keys = 4 * ((kGroups - lw + kLoaders - 1) / kLoaders) - 32 * w;
+    return keys >= 32 ? 0xffffffffu : keys > 0 ? (1u << keys) - 1u : 0u;
+  };
   // Bytes into a K, V or Q tile of `n` rows: blocks of 64 values, 128-byte rows, 16-byte chunks swizzled.
   auto place = [](int n, int row, int chunk) {
     return (uint32_t)((chunk >> 3) * n * 128 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
@@ -264,8 +268,7 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
             if (h == 0 && lane == 0) {
 #pragma unroll
               for (int w = 0; w < 2; w++) {
-                const int keys = 4 * ((kGroups - lw + kLoaders - 1) / kLoaders) - 32 * w;
-                s_valid[n % kMasks][lw][w] = keys >= 32 ? 0xffffffffu : keys > 0 ? (1u << keys) - 1u : 0u;
+                s_valid[n % kMasks][lw][w] = full_word(lw, w);
               }
               tc5::bar_arrive(MASK(n % kMasks));
             }
@@ -343,77 +346,69 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
       if (ok && !*abort_flag) tell(2 * tiles);
       else if (lane == 0) fail();
     } else {
-      // ---- products ----
-      const uint32_t one = tc5::elect();
-      int segs_seen = 0;
-      bool ok = true;
-      // S of step i for stream r: its key tile is n. `seg_of` and `in_of`: the segment of a step and the
-      // step's place in it, for this step and the next (divisions are slow next to an MMA).
-      int seg_of[2], in_of[2];
-      seg_of[0] = step0 / each;
-      in_of[0] = step0 - seg_of[0] * each;
-      auto follow = [&]() {
-        in_of[1] = in_of[0] + 1 == each ? 0 : in_of[0] + 1;
-        seg_of[1] = seg_of[0] + (in_of[1] == 0);
-      };
-      follow();
-      int sent[2] = {0, 0}, used[2] = {0, 0};  // tiles of each stream so far: S asked for, P used
-      auto first = [&](int i, int r, int k_) {
-        const int n = i * TPS + (TPS == 2 ? r : 0), at = 2 * n % NSLOT, u = sent[r];
-        const int in = in_of[k_];
-        if (r == 0 && (i == 0 || in == 0)) {
-          if (!tc5::bar_wait(Q_FULL, tc5::phase(segs_seen, 1))) return false;
-          segs_seen++;
+      // ---- products of stream r ----
+      // (One warp that looks after both streams finds each barrier some 500 cycles late; 6600 cycles a step.)
+      const int r = warp - kMmaWarp;
+      const uint32_t one = tc5::elect(), S = tmem + r * KT, O = tmem + kColO + r * DP;
+      int k_at = TPS == 2 ? 2 * r : 0, v_at = k_at + 1;  // ring places of this step's K and V, and their phases
+      uint32_t k_ph = 0, v_ph = 0, q_ph = 0, used = 0;   // used: of the stream's own barriers
+      int in = step0 % each, mt = step0 / each % p.tile_segs;
+      bool ok = true, used_before = false;
+      for (int i = 0; i < steps && r < STREAMS; i++) {
+        const bool fresh = i == 0 || in == 0, last_of_q = i + 1 == steps || in + 1 == each;
+        const bool on = RT == 1 || (mt * RT + r) * kTileRows < rows;
+        if (fresh) {
+          ok = tc5::bar_wait(Q_FULL, q_ph);
+          q_ph ^= 1;
         }
-        if ((TPS == 2 || r == 0) && !tc5::bar_wait(FULL(at), tc5::phase(2 * n, NSLOT))) return false;
-        tc5::fence_after();
-        const bool on = live(seg_of[k_], r);
-        // The buffer holds the P of the tile before the last: MMAs of different shapes need not run in the
-        // order of their issue, so its product has to be done, not only asked for.
-        if (on && u >= 2 && !tc5::bar_wait(PV_DONE(r), u & 1)) return false;
-        const uint32_t qs = base + (RT == 2 ? r : 0) * L::Q_TILE, ks = ring + at * L::SLOT;
-        if (on) {
+        ok = ok && tc5::bar_wait(FULL(k_at), k_ph);
+        if (!on) {
+          // No rows: it only takes its part in the releases, each place once it has been filled.
+          if (lane == 0 && ok) {
+            tc5::bar_arrive(EMPTY(k_at));
+            if (last_of_q) tc5::bar_arrive(Q_EMPTY);
+          }
+          ok = ok && tc5::bar_wait(FULL(v_at), v_ph);
+          if (lane == 0 && ok) tc5::bar_arrive(EMPTY(v_at));
+        } else {
+          // S takes the place of the P before it, whose product has to be done by then, not only asked for:
+          // MMAs with other accumulators need not run in the order of their issue.
+          if (used_before) ok = ok && tc5::bar_wait(PV_DONE(r), used ^ 1);
+          if (!ok) break;
+          __syncwarp();
+          tc5::fence_after();
+          const uint32_t q_s = base + (RT == 2 ? r : 0) * L::Q_TILE, k_s = ring + k_at * L::SLOT, v_s = ring + v_at * L::SLOT;
 #pragma unroll
           for (int k = 0; k < DP / 16; k++)
-            mma_ss(tmem + (2 * r + (u & 1)) * KT, tc5::desc_sw128(qs + (k >> 2) * (kTileRows * 128) + (k & 3) * 32),
-                   tc5::desc_sw128(ks + (k >> 2) * (KT * 128) + (k & 3) * 32), kIdescS, k > 0, one);
-          tc5::commit(S_FULL(r, u), one);
-          sent[r]++;
-        }
-        if (TPS == 2 || r == RT - 1) tc5::commit(EMPTY(at), one);
-        if (r == STREAMS - 1 && (i + 1 == steps || in + 1 == each)) tc5::commit(Q_EMPTY, one);
-        return true;
-      };
-      // O of stream r += P V at step i.
-      auto second = [&](int i, int r) {
-        const int n = i * TPS + (TPS == 2 ? r : 0), at = (2 * n + 1) % NSLOT, u = used[r];
-        const bool on = live(seg_of[0], r);
-        if (on && !tc5::bar_wait(P_FULL(r, u), (u >> 1) & 1)) return false;
-        if ((TPS == 2 || r == 0) && !tc5::bar_wait(FULL(at), tc5::phase(2 * n + 1, NSLOT))) return false;
-        tc5::fence_after();
-        const bool start = i == 0 || in_of[0] == 0;
-        const uint32_t vs = ring + at * L::SLOT;
-        if (on) {
+            mma_ss(S, tc5::desc_sw128(q_s + (k >> 2) * (kTileRows * 128) + (k & 3) * 32),
+                   tc5::desc_sw128(k_s + (k >> 2) * (KT * 128) + (k & 3) * 32), kIdescS, k > 0, one);
+          tc5::commit(S_FULL(r), one);
+          tc5::commit(EMPTY(k_at), one);
+          if (last_of_q) tc5::commit(Q_EMPTY, one);
+          ok = tc5::bar_wait(FULL(v_at), v_ph);
 #pragma unroll
-          for (int k = 0; k < KT / 16; k++)
-            mma_ts(tmem + kColO + r * DP, tmem + (2 * r + (u & 1)) * KT + 8 * k, desc_n_major(vs + k * 2048, KT * 128), kIdescO, !start || k > 0, one);
+          for (int h = 0; h < 2; h++) {
+            ok = ok && tc5::bar_wait(P_FULL(r, h), used);
+            if (!ok) break;
+            __syncwarp();
+            tc5::fence_after();
+#pragma unroll
+            for (int k = 0; k < KT / 32; k++)
+              mma_ts(O, S + 8 * (h * (KT / 32) + k), desc_n_major(v_s + (h * (KT / 32) + k) * 2048, KT * 128), kIdescO,
+                     !(fresh && h == 0 && k == 0), one);
+          }
+          if (!ok) break;
           tc5::commit(PV_DONE(r), one);
-          used[r]++;
+          tc5::commit(EMPTY(v_at), one);
+          used ^= 1;
+          used_before = true;
         }
-        if (TPS == 2 || r == RT - 1) tc5::commit(EMPTY(at), one);
-        return true;
-      };
-      if (steps) {
-        for (int r = 0; r < STREAMS && ok; r++) ok = first(0, r, 0);
-        for (int i = 0; i < steps && ok; i++) {
-          // The next tiles' S before this one's P is waited for: the softmax finds it ready.
-#pragma unroll
-          for (int r = 0; r < STREAMS; r++) ok = ok && (i + 1 == steps || first(i + 1, r, 1));
-#pragma unroll
-          for (int r = 0; r < STREAMS; r++) ok = ok && second(i, r);
-          seg_of[0] = seg_of[1];
-          in_of[0] = in_of[1];
-          follow();
+        if (!ok) break;
+        if ((k_at += 2 * TPS) >= NSLOT) k_at -= NSLOT, k_ph ^= 1;
+        if ((v_at += 2 * TPS) >= NSLOT) v_at -= NSLOT, v_ph ^= 1;
+        if (++in == each) {
+          in = 0;
+          if (++mt == p.tile_segs) mt = 0;
         }
       }
       if (!ok && lane == 0) fail();
@@ -429,22 +424,33 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
       const bool start = i == 0 || in == 0, last = i + 1 == steps || in + 1 == each;
       const int this_seg = seg;
       if (++in == each) in = 0, seg++;
-      if (!live(this_seg, r)) continue;
+      // The streams take turns at their exponentials, stream 0 first, one beginning when the other is half
+      // through: left alone they fall into step, and both wait for the exponential unit, then both for the
+      // tensor cores (4700 cycles a step).
+      const uint32_t turn = (uint32_t)(i - (r == 0)) & 1u;
+      const bool wait_turn = STREAMS == 2 && (r == 1 || i > 0);
+      if (!live(this_seg, r)) {
+        if (wait_turn && !tc5::bar_wait(TURN(r), turn)) {
+          if (lane == 0) fail();
+          break;
+        }
+        if (STREAMS == 2) tc5::bar_arrive(TURN(1 - r));
+        continue;
+      }
       const int n = i * TPS + (TPS == 2 ? r : 0);
-      const uint32_t sp = tmem + lanes + (2 * r + (used & 1)) * KT;
+      const uint32_t sp = tmem + lanes + r * KT;
       bool whole = tc5::bar_wait(MASK(n % kMasks), tc5::phase(n, kMasks));
-      if (!whole || !tc5::bar_wait(S_FULL(r, used), (used >> 1) & 1)) {
+      if (!whole || !tc5::bar_wait(S_FULL(r), used & 1)) {
         if (lane == 0) fail();
         break;
       }
       tc5::fence_after();
-      // The row is read twice, 32 columns at a time, in loops that stay in the instruction cache: the same
+      // The row is read twice, a half at a time, in loops that stay in the instruction cache: the same
       // arithmetic unrolled over a whole row waits more for instructions than for anything else (2.4 of
-      // 4 cycles an instruction, 86 us on 64 sequences behind 32768 keys).
+      // 4 cycles an instruction).
 #pragma unroll
       for (int w = 0; w < kLoaders; w++) {
-        const int keys = 4 * ((kGroups - w + kLoaders - 1) / kLoaders);
-        const uint32_t lo = keys >= 32 ? 0xffffffffu : (1u << (keys & 31)) - 1u, hi = keys > 32 ? (1u << (keys - 32)) - 1u : 0u;
+        const uint32_t lo = full_word(w, 0), hi = full_word(w, 1);
         whole = whole && s_valid[n % kMasks][w][0] == lo && s_valid[n % kMasks][w][1] == hi;
       }
       if (!whole) {
@@ -464,34 +470,33 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
         }
         tmem_wait_st();
       }
+      constexpr int HALF = KT / 2;  // columns at a time: a half of P
       float top;
-      if (p.scale_log2 > 0.0f) {
+      {
         float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll 1
-        for (int c = 0; c < KT / 64; c++) {
-          float x[64];
-          tmem_ld32(sp + 64 * c, x);
-          tmem_ld32(sp + 64 * c + 32, x + 32);
-          tc5::wait_ld();
-          float a = fmaxf(x[0], x[1]), b = fmaxf(x[2], x[3]);
+        for (int c = 0; c < 2; c++) {
+          float x[HALF];
 #pragma unroll
-          for (int j = 4; j < 64; j += 4) {
+          for (int j = 0; j < HALF; j += 32) tmem_ld32(sp + c * HALF + j, x + j);
+          tc5::wait_ld();
+#pragma unroll
+          for (int j = 0; j < HALF; j += 4) {
             t0 = fmaxf(fmaxf(x[j], x[j + 1]), t0);
             t1 = fmaxf(fmaxf(x[j + 2], x[j + 3]), t1);
           }
-          t0 = fmaxf(t0, a);
-          t1 = fmaxf(t1, b);
         }
         top = fmaxf(t0, t1) * p.scale_log2;
-      } else {  // the largest score is that of the smallest product
+      }
+      if (p.scale_log2 < 0.0f) {  // the largest score is that of the smallest product
         float low = INFINITY;
 #pragma unroll 1
         for (int c = 0; c < KT / 32; c++) {
-          float x[32];
-          tmem_ld32(sp + 32 * c, x);
+          float z[32];
+          tmem_ld32(sp + 32 * c, z);
           tc5::wait_ld();
 #pragma unroll
-          for (int j = 0; j < 32; j++) low = fminf(low, x[j]);
+          for (int j = 0; j < 32; j++) low = fminf(low, z[j]);
         }
         top = low * p.scale_log2;
       }
@@ -503,11 +508,7 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
         if (__any_sync(0xffffffffu, grow)) {
           const float to = grow ? top : m;
           const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : exp2_fast(m - to);
-          if (!tc5::bar_wait(PV_DONE(r), (used - 1) & 1)) {
-            if (lane == 0) fail();
-            break;
-          }
-          tc5::fence_after();
+          // (This S was asked for when the product before it was done.)
 #pragma unroll 1
           for (int c = 0; c < DP / 32; c++) {
             float o[32];
@@ -523,38 +524,47 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
         }
       }
       const float u = m == -INFINITY ? 0.0f : m;
+      if (wait_turn && !tc5::bar_wait(TURN(r), turn)) {
+        if (lane == 0) fail();
+        break;
+      }
       // P in the place of S: 16 columns for 32, so that a chunk never lands on columns not read yet.
       const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), u2 = make_float2(-u, -u);
       float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
-      float x[32];
-      tmem_ld32(sp, x);
+      float x[HALF];
+#pragma unroll
+      for (int j = 0; j < HALF; j += 32) tmem_ld32(sp + j, x + j);
 #pragma unroll 1
-      for (int c = 0; c < KT / 32; c++) {
+      for (int c = 0; c < 2; c++) {
         tc5::wait_ld();
-        float2 e[16];
+        float2 e[HALF / 2];
 #pragma unroll
-        for (int j = 0; j < 16; j++) e[j] = fma2(make_float2(x[2 * j], x[2 * j + 1]), scale2, u2);
-        if (c + 1 < KT / 32) tmem_ld32(sp + 32 * (c + 1), x);
-        uint32_t w[16];
+        for (int j = 0; j < HALF / 2; j++) e[j] = fma2(make_float2(x[2 * j], x[2 * j + 1]), scale2, u2);
+        if (c == 0) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
+          for (int j = 0; j < HALF; j += 32) tmem_ld32(sp + HALF + j, x + j);
+        }
+        uint32_t w[HALF / 2];
+#pragma unroll
+        for (int j = 0; j < HALF / 2; j++) {
           e[j].x = exp2_fast(e[j].x);
           e[j].y = exp2_fast(e[j].y);
           if (j & 1) sum1 = add2(sum1, e[j]);
           else sum0 = add2(sum0, e[j]);
           w[j] = pack2<T>(e[j].x, e[j].y);
         }
-        tmem_st16(sp + 16 * c, w);
+#pragma unroll
+        for (int j = 0; j < HALF / 2; j += 16) tmem_st16(sp + c * (HALF / 2) + j, w + j);
+        // This half's product can start.
+        tmem_wait_st();
+        tc5::fence_before();
+        tc5::bar_arrive(P_FULL(r, c));
+        if (STREAMS == 2 && c == 0) tc5::bar_arrive(TURN(1 - r));
       }
       l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
-      tmem_wait_st();
-      tc5::fence_before();
-      tc5::bar_arrive(P_FULL(r, used));
       used++;
       if (last) {
-        // The product of the tile before may still be out: a wait for this one's alone would take the end of
-        // the phase before that for it.
-        if ((used >= 2 && !tc5::bar_wait(PV_DONE(r), used & 1)) || !tc5::bar_wait(PV_DONE(r), (used - 1) & 1)) {
+        if (!tc5::bar_wait(PV_DONE(r), (used - 1) & 1)) {
           if (lane == 0) fail();
           break;
         }

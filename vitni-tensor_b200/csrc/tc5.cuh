@@ -33,6 +33,18 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// Whether a phase is over, without waiting.
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Bounded by the SM's own clock (cheaper to read than %globaltimer): 2^32 cycles, about 2 s.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
   if (bar_try(bar, parity)) return true;
