@@ -10,7 +10,7 @@
 #include <algorithm>
 
 #include "serve.h"
-#include "vtq_internal.h"
+#include "tc5.cuh"
 
 namespace vtq {
 namespace {
@@ -106,6 +106,7 @@ __device__ __forceinline__ Place place_of(const vtq_append_kv_args& a, int64_t t
 // their W partners; otherwise W values, pairs of neighbours.
 template <typename X, typename C, int W, int TOK, bool HALF, bool WIDE>
 __global__ void __launch_bounds__(TOK > 1 ? 256 : 512, TOK > 1 ? 4 : 1) append_kernel(const __grid_constant__ AppendParams p) {
+  tc5::grid_wait();
   constexpr int P = HALF ? W : W / 2;  // pairs of a rotated unit
   constexpr int U = TOK < 4 ? TOK : HALF ? (W == 8 ? 1 : 2) : W == 8 ? 2 : 4;
   __shared__ Place s_place[TOK];
@@ -220,12 +221,10 @@ cudaError_t run(const vtq_append_kv_args& a, cudaStream_t st) {
   const int most = many ? 256 : 512, passes = (p.units + most - 1) / most;
   const int threads = ((p.units + passes - 1) / passes + 31) / 32 * 32;
   // A decode step's few tokens go one to a CTA, for latency; many in even shares to as many as fit at once.
-  kernel_launch_count()++;
   if (many)
-    append_kernel<X, C, W, 32, HALF, WIDE><<<(unsigned)(num_sms() * std::max(1, 1024 / threads)), threads, 0, st>>>(p);
-  else
-    append_kernel<X, C, W, 1, HALF, WIDE><<<(unsigned)a.tokens, threads, 0, st>>>(p);
-  return cudaGetLastError();
+    return launch_after(append_kernel<X, C, W, 32, HALF, WIDE>, dim3((unsigned)(num_sms() * std::max(1, 1024 / threads))),
+                        threads, 0, 1, st, p);
+  return launch_after(append_kernel<X, C, W, 1, HALF, WIDE>, dim3((unsigned)a.tokens), threads, 0, 1, st, p);
 }
 
 template <typename X, typename C>

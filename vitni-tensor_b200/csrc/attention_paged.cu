@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(attention_threads<T, DP, RT>(), 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   int* base = reinterpret_cast<int*>(smem + PS::STAGES_BYTES);
+  tc5::grid_wait();
   tc5::grid_release();
   build_plan(p, base);
   const int cta = (int)blockIdx.x, x = base[2];
@@ -90,104 +91,116 @@ __global__ void __launch_bounds__(attention_threads<T, DP, RT>(), 1)
   part_role<T, DP, P::KT, P::WARPS>(p, tmk, tmv, smem, base, cta - x, p.ctas - x);
 }
 
-// Adds the parts of each row (query head of a token): one warp a row.
+// Adds the parts of each row (query head of a token): one warp a row. The kernel before lets it start early;
+// until it is done the warp goes through its own code once, on made-up places and with nothing stored, so
+// that the instructions are there when the parts are (they are most of its time otherwise: 8 us for 128 rows).
 template <typename T, int DP>
 __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttnParams p) {
-  tc5::grid_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int row = (int)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int heads = (int)p.a.heads, H = (int)p.a.kv.kv_heads, D = (int)p.a.kv.head_dim;
-  if (row >= p.a.tokens * heads) return;
-  const int token = (int)row / heads, head = (int)row - token * heads, g = head / p.group;
-  const int4 of = p.rows[token];
-  if (!of.w) return;  // no sequence owns the row
-  // The parts of the row's place among the sequence's own rows, and among all rows for the prefix.
-  int count[2] = {0, 0}, rr[2] = {0, 0};
-  const float* slot0[2] = {nullptr, nullptr};
-  if (of.x >= 0) {
-    const int r = of.y + head - g * p.group, seg = of.x + r / kRows * H + g;
-    const int2 w = p.seg_parts[seg];
-    rr[0] = r % kRows;
-    count[0] = w.y - w.x + 1;
-    slot0[0] = p.part + (int64_t)(w.x + seg) * (kRows * (DP + 2));
-  }
-  if (of.z >= 0) {
-    const int r = token * p.group + head - g * p.group;
-    if (p.on_tiles) {
-      // A CTA leaves a part for each stream: of other rows, or of the same rows' other keys.
-      const int stream = p.tile_rt == 2 ? r / kTileRows % 2 : 0, seg = g * p.tile_segs + r / (kTileRows * p.tile_rt);
-      const int2 w = p.seg_ctas[seg];
-      rr[1] = r % kTileRows;
-      count[1] = (w.y - w.x + 1) * (p.tile_rt == 2 ? 1 : p.tile_streams);
-      slot0[1] = p.tile_part + ((int64_t)(w.x + seg) * p.tile_streams + stream) * (kTileRows * (DP + 2));
-    } else {
-      const int seg = of.z + r / kRows * H + g;
-      const int2 w = p.seg_parts[seg];
-      rr[1] = r % kRows;
-      count[1] = w.y - w.x + 1;
-      slot0[1] = p.part + (int64_t)(w.x + seg) * (kRows * (DP + 2));
+  if (row >= (int)p.a.tokens * heads) return;
+  const int token = row / heads, head = row - token * heads, g = head / p.group;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; pass++) {
+    if (pass) tc5::grid_wait();
+    int4 of = make_int4(0, 0, p.prefix ? 0 : -1, 1);
+    if (pass) of = p.rows[token];
+    if (!of.w) return;  // no sequence owns the row
+    // The parts of the row's place among the sequence's own rows, and among all rows for the prefix.
+    int count[2] = {0, 0}, rr[2] = {0, 0};
+    const float* slot0[2] = {p.part, p.part};
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const int seg0 = k ? of.z : of.x;
+      if (seg0 < 0) continue;
+      const int r = (k ? token * p.group : of.y) + head - g * p.group;
+      const bool tiles = k && p.on_tiles;
+      // A CTA of the prefix's own tiles leaves a part for each stream: of other rows, or of the same rows'
+      // other keys.
+      const int seg = tiles ? g * p.tile_segs + r / (kTileRows * p.tile_rt) : seg0 + r / kRows * H + g;
+      int2 w = make_int2(0, 0);
+      if (pass) w = (tiles ? p.seg_ctas : p.seg_parts)[seg];
+      rr[k] = r % (tiles ? kTileRows : kRows);
+      count[k] = (w.y - w.x + 1) * (tiles && p.tile_rt == 1 ? p.tile_streams : 1);
+      if (!pass) continue;
+      slot0[k] = tiles ? p.tile_part + ((int64_t)(w.x + seg) * p.tile_streams + (p.tile_rt == 2 ? r / kTileRows % 2 : 0)) * (kTileRows * (DP + 2))
+                       : p.part + (int64_t)(w.x + seg) * (kRows * (DP + 2));
     }
-  }
-  const int parts = count[0] + count[1];
-  // Part i's (m, l) of the row, and its o.
-  auto at = [&](int i, const float*& o) {
-    const int k = i >= count[0], rows = k && p.on_tiles ? kTileRows : kRows;
-    const int step = rows * (DP + 2) * (k && p.on_tiles && p.tile_rt == 2 ? 2 : 1);
-    const float* s = slot0[k] + (int64_t)(i - (k ? count[0] : 0)) * step;
-    o = s + 2 * rows + rr[k] * DP;
-    return s + 2 * rr[k];
-  };
-  float m = -INFINITY;
-  for (int i = lane; i < parts; i += 32) {
-    const float* o;
-    m = fmaxf(m, *at(i, o));
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  const float um = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, acc[DP / 32];
-#pragma unroll
-  for (int e = 0; e < DP / 32; e++) acc[e] = 0.0f;
-  for (int i0 = 0; i0 < parts; i0 += 32) {
-    float f = 0.0f;
-    if (i0 + lane < parts) {
+    if (!pass) rr[0] = rr[1] = 0;
+    const int parts = count[0] + count[1];
+    // Part i's (m, l) of the row, and its o.
+    auto at = [&](int i, const float*& o) {
+      const bool k = i >= count[0], tiles = k && p.on_tiles;
+      const int rows = tiles ? kTileRows : kRows, step = rows * (DP + 2) * (tiles && p.tile_rt == 2 ? 2 : 1);
+      const float* s = (k ? slot0[1] : slot0[0]) + (pass ? (int64_t)(i - (k ? count[0] : 0)) * step : 0);
+      const int r = k ? rr[1] : rr[0];
+      o = s + (pass ? 2 * rows : 0) + r * DP;
+      return s + 2 * r;
+    };
+    float m = -INFINITY;
+    for (int i = lane; i < parts; i += 32) {
       const float* o;
-      const float2 ml = *reinterpret_cast<const float2*>(at(i0 + lane, o));
-      f = exp2_fast(ml.x - um);
-      l += f * ml.y;
+      m = fmaxf(m, *at(i, o));
     }
-    const int n = min(32, parts - i0);
-#pragma unroll 4
-    for (int i = 0; i < n; i++) {
-      const float* s;
-      at(i0 + i, s);
-      const float fi = __shfl_sync(0xffffffffu, f, i);
-      if (fi == 0.0f) continue;  // nothing of it, or nothing in it
 #pragma unroll
-      for (int e = 0; e < DP / 64; e++) {
-        const float2 v = *reinterpret_cast<const float2*>(s + 64 * e + 2 * lane);
-        acc[2 * e] = fmaf(fi, v.x, acc[2 * e]);
-        acc[2 * e + 1] = fmaf(fi, v.y, acc[2 * e + 1]);
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const float um = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, acc[DP / 32];
+#pragma unroll
+    for (int e = 0; e < DP / 32; e++) acc[e] = 0.0f;
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+      float f = 0.0f;
+      if (i0 + lane < parts) {
+        const float* o;
+        const float2 ml = *reinterpret_cast<const float2*>(at(i0 + lane, o));
+        f = exp2_fast(ml.x - um);
+        l += f * ml.y;
+        if (ml.y == 0.0f) f = 0.0f;  // nothing in it, whatever its o holds
+      }
+      const int n = min(32, parts - i0);
+      // Several parts' loads at once.
+      constexpr int kAtOnce = DP > 64 ? 4 : 8;
+      for (int i = 0; i < n; i += kAtOnce) {
+        float2 v[kAtOnce][DP / 64];
+        float fi[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++) {
+          fi[k] = __shfl_sync(0xffffffffu, f, (i + k) & 31);
+          if (i + k >= n) fi[k] = 0.0f;
+          const float* s;
+          at(min(i0 + i + k, parts - 1), s);
+#pragma unroll
+          for (int e = 0; e < DP / 64; e++)
+            v[k][e] = fi[k] != 0.0f ? *reinterpret_cast<const float2*>(s + 64 * e + 2 * lane) : make_float2(0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++)
+#pragma unroll
+          for (int e = 0; e < DP / 64; e++) {
+            acc[2 * e] = fmaf(fi[k], v[k][e].x, acc[2 * e]);
+            acc[2 * e + 1] = fmaf(fi[k], v[k][e].y, acc[2 * e + 1]);
+          }
       }
     }
-  }
 #pragma unroll
-  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
-  T* out = static_cast<T*>(p.a.out) + token * p.a.o_tok + head * p.a.o_head;
+    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
+    T* out = static_cast<T*>(p.a.out) + token * p.a.o_tok + head * p.a.o_head;
 #pragma unroll
-  for (int e = 0; e < DP / 64; e++) {
-    const int d = 64 * e + 2 * lane;
-    if (d >= D) continue;
-    if (p.o_wide) {
-      *reinterpret_cast<uint32_t*>(out + d) = pack2<T>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-    } else {
-      out[d] = from_f32<T>(acc[2 * e] * inv);
-      out[d + 1] = from_f32<T>(acc[2 * e + 1] * inv);
+    for (int e = 0; e < DP / 64; e++) {
+      const int d = 64 * e + 2 * lane;
+      if (!pass || d >= D) continue;
+      if (p.o_wide) {
+        *reinterpret_cast<uint32_t*>(out + d) = pack2<T>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+      } else {
+        out[d] = from_f32<T>(acc[2 * e] * inv);
+        out[d + 1] = from_f32<T>(acc[2 * e + 1] * inv);
+      }
     }
+    if (pass && p.a.lse && lane == 0)
+      p.a.lse[token * p.a.lse_tok + head] = l == 0.0f ? -INFINITY : (um + log2f(l)) * 0.69314718055994531f;
   }
-  if (p.a.lse && lane == 0)
-    p.a.lse[token * p.a.lse_tok + head] = l == 0.0f ? -INFINITY : (um + log2f(l)) * 0.69314718055994531f;
 }
 
 int padded_dim(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
@@ -247,7 +260,7 @@ vtq_status check(const char* fn, const vtq_attention_args* a) {
     return serve_fail(VTQ_ERR_INTERNAL, "%s: bad shape (heads not a multiple of kv_heads, or a negative size)", fn);
   if (a->kv.seqs > kMaxSeqs)
     return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "%s: not implemented (over %d sequences in one call)", fn, kMaxSeqs);
-  if (a->tokens > (1 << 20) || a->heads > 65536 || a->kv.table_width * a->kv.page_size > INT32_MAX / 2)
+  if (a->tokens > (1 << 20) || a->heads > 65536 || a->tokens * a->heads > INT32_MAX / 2 || a->kv.table_width * a->kv.page_size > INT32_MAX / 2)
     return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "%s: not implemented (over 2^20 tokens, 2^16 heads or 2^30 positions)", fn);
   const int64_t tiles = (a->kv.table_width * a->kv.page_size + 15) / 16 + 1;
   if (most_segments(*a) * tiles > INT32_MAX || tile_cut(*a).total > INT32_MAX)
@@ -267,7 +280,8 @@ cudaError_t launch(AttnParams p, cudaStream_t st) {
   p.warps = P::WARPS;
   p.tile = P::KT;
   auto kernel = attention_kernel<T, DP, RT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_smem((const void*)kernel, smem, allowed);
   if (e != cudaSuccess) return e;
   // A box is the largest power of two of positions that pages are made of.
   CUtensorMap tmk = {}, tmv = {};
@@ -284,19 +298,9 @@ cudaError_t launch(AttnParams p, cudaStream_t st) {
         tma_half_map(&tmv, kv.v, dim, vs, 64, (uint32_t)p.box) != cudaSuccess)
       p.box = 0;  // strides that TMA does not take: rows are gathered
   }
-  kernel_launch_count() += 2;
-  kernel<<<(unsigned)p.ctas, attention_threads<T, DP, RT>(), smem, st>>>(p, tmk, tmv);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.a.tokens * p.a.heads + 3) / 4));
-  cfg.blockDim = dim3(128);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, attention_join_kernel<T, DP>, p);
+  e = launch_after(kernel, dim3((unsigned)p.ctas), attention_threads<T, DP, RT>(), smem, 1, st, p, tmk, tmv);
+  if (e != cudaSuccess) return e;
+  return launch_after(attention_join_kernel<T, DP>, dim3((unsigned)((p.a.tokens * p.a.heads + 3) / 4)), 128, 0, 1, st, p);
 }
 
 template <typename T>

@@ -69,6 +69,7 @@ __global__ void __launch_bounds__(kQThreads)
     quantize_kernel(const X* __restrict__ x, int64_t ldx, int64_t n, bool wide, int8_t* __restrict__ q,
                     int64_t ldq, bool wide_q, float* __restrict__ scale) {
   __shared__ uint32_t s_max[kQThreads / 32];
+  tc5::grid_wait();
   tc5::grid_release();
   const X* row = x + (int64_t)blockIdx.x * ldx;
   int8_t* out = q + (int64_t)blockIdx.x * ldq;
@@ -139,9 +140,7 @@ cudaError_t launch_quantize(const X* x, int64_t ldx, int64_t tokens, int64_t n, 
   // that more rows are in flight.
   const int64_t each = tokens <= 2 * num_sms() ? 8 : 32;
   const int threads = (int)std::min<int64_t>(kQThreads, std::max<int64_t>(32, ((n + each - 1) / each + 31) / 32 * 32));
-  kernel_launch_count()++;
-  quantize_kernel<X><<<(unsigned)tokens, threads, 0, st>>>(x, ldx, n, wide, q, ldq, wide_q, scale);
-  return cudaGetLastError();
+  return launch_after(quantize_kernel<X>, dim3((unsigned)tokens), threads, 0, 1, st, x, ldx, n, wide, q, ldq, wide_q, scale);
 }
 
 cudaError_t quantize(int dtype, const void* x, int64_t ldx, int64_t tokens, int64_t n, int8_t* q, int64_t ldq,
@@ -156,6 +155,7 @@ cudaError_t quantize(int dtype, const void* x, int64_t ldx, int64_t tokens, int6
 struct I8Params {
   int T, K, N;
   int kblocks;  // of 128 inputs
+  bool early;   // the kernel before is this call's own: whatever wrote the weights has ended
   const float* xs;
   const float* ws;
   const float* bias;
@@ -230,8 +230,10 @@ __global__ void __launch_bounds__(kThreads)
 
   if (warp == 0) {
     if (lane == 0) {
-      // The weights do not depend on the kernel before: as many as fit are on their way before its
-      // codes are waited for.
+      // The call's own codes kernel lets this one begin only when all before it have ended: as many weights
+      // as fit are on their way before its codes are waited for. With the caller's codes the kernel
+      // before may be the one that writes the weights.
+      if (!p.early) tc5::grid_wait();
       const int ahead = min(nk, STAGES);
       for (int k = 0; k < ahead; k++) {
         tc5::bar_expect(FULL(k), STAGE);
@@ -342,8 +344,8 @@ __global__ void __launch_bounds__(kThreads)
 
 // Many tokens: persistent pairs of CTAs (cta_group::2), each walking tiles of 256 channels x 256 tokens. A
 // CTA brings 128 channels and 128 tokens, 32 KB for 2^22 products: at the 62 bytes a cycle that L2 gives an
-// SM here this feeds the tensor cores, where a CTA by itself (128 x 256, 48 KB) waits: 93 us against 65 on
-// 2048 x 4096 x 14336. The leader (rank 0) issues the products for both; barriers that only it waits for are
+// SM here this feeds the tensor cores, where a CTA by itself (128 x 256, 48 KB) waits: 101 us against 92 on
+// 2048 x 4096 x 14336, the codes' kernel of 9 us included. The leader (rank 0) issues the products for both; barriers that only it waits for are
 // its own, signalled from the peer. Two accumulators of 256 columns in TMEM, so that one tile is stored while
 // the next one is summed; the operand ring runs on across tiles.
 constexpr int PM = 256, PN = 256, kPStages = 6, kPEpiWarps = 8, kPThreads = 64 + 32 * kPEpiWarps;
@@ -382,7 +384,7 @@ __device__ __forceinline__ void arrive_remote(uint32_t bar) {
 }
 
 template <typename Y>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
+__global__ void __launch_bounds__(kPThreads, 1)
     i8_wide_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx,
                    const __grid_constant__ I8Params p, int tiles, int token_tiles) {
   constexpr uint32_t kIdesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(PN >> 3) << 17) | ((uint32_t)(PM >> 4) << 24);
@@ -515,57 +517,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
 }
 
 template <typename Y>
-cudaError_t launch_wide(const CUtensorMap& tmw, const CUtensorMap& tmx, const I8Params& p, bool pdl, cudaStream_t st) {
+cudaError_t launch_wide(const CUtensorMap& tmw, const CUtensorMap& tmx, const I8Params& p, cudaStream_t st) {
   constexpr size_t smem = (size_t)kPStages * kPStage + 1024;
-  cudaError_t e = cudaFuncSetAttribute(i8_wide_kernel<Y>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_smem((const void*)i8_wide_kernel<Y>, smem, allowed);
   if (e != cudaSuccess) return e;
   const int token_tiles = (p.T + PN - 1) / PN, tiles = (p.N + PM - 1) / PM * token_tiles;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * std::min(tiles, num_sms() / 2)));
-  cfg.blockDim = dim3(kPThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl && pdl_enabled() ? 1 : 0;
-  kernel_launch_count()++;
-  return cudaLaunchKernelEx(&cfg, i8_wide_kernel<Y>, tmw, tmx, p, tiles, token_tiles);
+  return launch_after(i8_wide_kernel<Y>, dim3((unsigned)(2 * std::min(tiles, num_sms() / 2))), kPThreads, smem, 2, st, tmw, tmx, p,
+                      tiles, token_tiles);
 }
 
 template <int NT, int STAGES, typename Y>
-cudaError_t launch_tile(const CUtensorMap& tmw, const CUtensorMap& tmx, const I8Params& p, int splits, bool pdl,
-                        cudaStream_t st) {
+cudaError_t launch_tile(const CUtensorMap& tmw, const CUtensorMap& tmx, const I8Params& p, int splits, cudaStream_t st) {
   constexpr size_t smem = (size_t)STAGES * (A_STAGE + NT * 128) + 1024;
-  cudaError_t e = cudaFuncSetAttribute(i8_tile_kernel<NT, STAGES, Y>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_smem((const void*)i8_tile_kernel<NT, STAGES, Y>, smem, allowed);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.N + BM - 1) / BM * splits), (unsigned)((p.T + NT - 1) / NT));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)splits;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl && pdl_enabled() ? 2 : 1;
-  kernel_launch_count()++;
-  return cudaLaunchKernelEx(&cfg, i8_tile_kernel<NT, STAGES, Y>, tmw, tmx, p);
+  return launch_after(i8_tile_kernel<NT, STAGES, Y>, dim3((unsigned)((p.N + BM - 1) / BM * splits), (unsigned)((p.T + NT - 1) / NT)),
+                      kThreads, smem, splits, st, tmw, tmx, p);
 }
 
 template <typename Y>
-cudaError_t product(const CUtensorMap& tmw, const CUtensorMap& tmx, const I8Params& p, int nt, int splits, bool pdl,
-                    cudaStream_t st) {
+cudaError_t product(const CUtensorMap& tmw, const CUtensorMap& tmx, const I8Params& p, int nt, int splits, cudaStream_t st) {
   switch (nt) {
-    case 16: return launch_tile<16, 5, Y>(tmw, tmx, p, splits, pdl, st);
-    case 32: return launch_tile<32, 5, Y>(tmw, tmx, p, splits, pdl, st);
-    case 64: return launch_tile<64, 4, Y>(tmw, tmx, p, splits, pdl, st);
-    case 128: return launch_tile<128, 3, Y>(tmw, tmx, p, splits, pdl, st);
-    default: return splits > 1 ? launch_tile<256, 4, Y>(tmw, tmx, p, splits, pdl, st) : launch_wide<Y>(tmw, tmx, p, pdl, st);
+    case 16: return launch_tile<16, 5, Y>(tmw, tmx, p, splits, st);
+    case 32: return launch_tile<32, 5, Y>(tmw, tmx, p, splits, st);
+    case 64: return launch_tile<64, 4, Y>(tmw, tmx, p, splits, st);
+    case 128: return launch_tile<128, 3, Y>(tmw, tmx, p, splits, st);
+    default: return splits > 1 ? launch_tile<256, 4, Y>(tmw, tmx, p, splits, st) : launch_wide<Y>(tmw, tmx, p, st);
   }
 }
 
@@ -644,10 +623,10 @@ vtq_status vtq_linear_i8(const vtq_linear_i8_args* a, void* ws, size_t ws_bytes,
   const uint32_t token_box = nt == 256 && splits == 1 ? 128 : (uint32_t)nt;
   if (e == cudaSuccess) e = tma_byte_map(&tmx, q, T, a->in_feat, ldq, 128, token_box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (e != cudaSuccess) return serve_cuda(e, fn);
-  const I8Params p{T, (int)a->in_feat, (int)a->out_feat, kb, xs, a->w_scale, a->bias, a->y, a->ldy, a->status};
-  if (a->y_dtype == VTQ_F32) e = product<float>(tmw, tmx, p, nt, splits, !codes, st);
-  else if (a->y_dtype == VTQ_F16) e = product<__half>(tmw, tmx, p, nt, splits, !codes, st);
-  else e = product<__nv_bfloat16>(tmw, tmx, p, nt, splits, !codes, st);
+  const I8Params p{T, (int)a->in_feat, (int)a->out_feat, kb, !codes, xs, a->w_scale, a->bias, a->y, a->ldy, a->status};
+  if (a->y_dtype == VTQ_F32) e = product<float>(tmw, tmx, p, nt, splits, st);
+  else if (a->y_dtype == VTQ_F16) e = product<__half>(tmw, tmx, p, nt, splits, st);
+  else e = product<__nv_bfloat16>(tmw, tmx, p, nt, splits, st);
   return serve_cuda(e, fn);
 }
 

@@ -22,14 +22,14 @@
 #include <algorithm>
 
 #include "serve.h"
-#include "vtq_internal.h"
+#include "tc5.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace vtq {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;  // four CTAs an SM
 constexpr int kStrips = 8, kBlock = 32 * kStrips;  // elements summed by one warp at a time
 static_assert(kWarps >= 4 && kWarps <= 32, "the joins below take one warp a row and one lane a warp");
 
@@ -70,23 +70,22 @@ __device__ __forceinline__ Left left(float p, float q) {
   w.e = __fsub_rn(__fsub_rn(p, __fsub_rn(w.r, t)), __fadd_rn(q, t));
   return w;
 }
-// The kStrips values at e0, e0 + 32, ..: nothing behind v1.
+// The kStrips values of both rows at e0, e0 + 32, ..: nothing behind v1.
 template <typename T>
-__device__ __forceinline__ void left_strips(const T* p, const T* q, int64_t e0, int64_t v1, int64_t only, bool sub,
-                                            Left (&r)[kStrips]) {
-  float a[kStrips], b[kStrips];
+struct Strips {
+  T a[kStrips], b[kStrips];
+  __device__ __forceinline__ void load(const T* p, const T* q, int64_t e0, int64_t v1, bool sub) {
 #pragma unroll
-  for (int k = 0; k < kStrips; k++) {
-    const bool in = e0 + 32 * k < v1;
-    a[k] = in ? to_f32(p[e0 + 32 * k]) : 0.0f;
-    b[k] = in && sub && q ? to_f32(q[e0 + 32 * k]) : 0.0f;
+    for (int k = 0; k < kStrips; k++) {
+      const bool in = e0 + 32 * k < v1;
+      a[k] = in ? p[e0 + 32 * k] : from_f32<T>(0.0f);
+      b[k] = in && sub && q ? q[e0 + 32 * k] : from_f32<T>(0.0f);
+    }
   }
-#pragma unroll
-  for (int k = 0; k < kStrips; k++) {
-    if (sub && e0 + 32 * k == only) b[k] = 1.0f;
-    r[k] = left<T>(a[k], b[k]);
+  __device__ __forceinline__ Left left_at(int k, int64_t e0, int64_t only, bool sub) const {
+    return left<T>(to_f32(a[k]), sub && e0 + 32 * k == only ? 1.0f : to_f32(b[k]));
   }
-}
+};
 
 __device__ __forceinline__ double warp_sum(double s) {
 #pragma unroll
@@ -105,11 +104,12 @@ __device__ __forceinline__ double warp_scan(double s, int lane) {
 // One cluster a sequence. CTA c of the cluster owns the blocks of kBlock
 // tokens [c nb, (c + 1) nb).
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) verify_draft_kernel(const VerifyParams a, int nb) {
+__global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const VerifyParams a, int nb) {
   extern __shared__ double sums[];  // nb: block sums, then their inclusive scan
   __shared__ int s_acc;
   __shared__ double s_total, s_warp[kWarps];
   __shared__ int64_t s_last, s_lastw[kWarps];
+  tc5::grid_wait();
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), size = (int)cl.num_blocks();
   const int b = blockIdx.x / size;
@@ -155,16 +155,17 @@ __global__ void __launch_bounds__(kThreads, 2) verify_draft_kernel(const VerifyP
     int64_t last = -1;  // the last token that has any weight
     for (int j = warp; j < mine; j += kWarps) {
       const int64_t e0 = v0 + (int64_t)j * kBlock + lane;
-      Left r[kStrips];
-      left_strips(p, q, e0, v1, only, sub, r);
+      Strips<T> now;
+      now.load(p, q, e0, v1, sub);
       // This lane's sum as a 32-bit value and what its roundings lost: 2^-48 of it.
       float hi = 0.0f, lo = 0.0f;
 #pragma unroll
       for (int k = 0; k < kStrips; k++) {
-        const float s = __fadd_rn(hi, r[k].r), t = __fsub_rn(s, hi);
-        lo = __fadd_rn(lo, __fadd_rn(__fadd_rn(__fsub_rn(hi, __fsub_rn(s, t)), __fsub_rn(r[k].r, t)), r[k].e));
+        const Left r = now.left_at(k, e0, only, sub);
+        const float s = __fadd_rn(hi, r.r), t = __fsub_rn(s, hi);
+        lo = __fadd_rn(lo, __fadd_rn(__fadd_rn(__fsub_rn(hi, __fsub_rn(s, t)), __fsub_rn(r.r, t)), r.e));
         hi = s;
-        if (r[k].r > 0.0f) last = e0 + 32 * k;
+        if (r.r > 0.0f) last = e0 + 32 * k;
       }
       const double s = warp_sum((double)hi + (double)lo);
       if (lane == 0) sums[j] = s;
@@ -239,13 +240,14 @@ __global__ void __launch_bounds__(kThreads, 2) verify_draft_kernel(const VerifyP
         for (int j = lo; j >= 0 && tail < 0; j--) {
           double cum = j ? sums[j - 1] : 0.0;
           const int64_t e0 = v0 + (int64_t)j * kBlock + lane;
-          Left r[kStrips];
-          left_strips(p, q, e0, v1, only, sub, r);
+          Strips<T> now;
+          now.load(p, q, e0, v1, sub);
 #pragma unroll
           for (int k = 0; k < kStrips; k++) {
-            const double c = warp_scan((double)r[k].r + (double)r[k].e, lane);
-            const unsigned over = __ballot_sync(0xffffffffu, r[k].r > 0.0f && start + (cum + c) > cut);
-            const unsigned some = __ballot_sync(0xffffffffu, r[k].r > 0.0f);
+            const Left r = now.left_at(k, e0, only, sub);
+            const double c = warp_scan((double)r.r + (double)r.e, lane);
+            const unsigned over = __ballot_sync(0xffffffffu, r.r > 0.0f && start + (cum + c) > cut);
+            const unsigned some = __ballot_sync(0xffffffffu, r.r > 0.0f);
             if (found < 0 && over) found = e0 - lane + 32 * k + __ffs(over) - 1;
             if (some) tail = e0 - lane + 32 * k + 31 - __clz(some);
             cum += __shfl_sync(0xffffffffu, c, 31);
@@ -272,10 +274,12 @@ __device__ __forceinline__ void take(float x, uint32_t v, uint32_t& hi, uint32_t
 
 constexpr int kGroup = 4;  // rows looked at together: a chain of drafts waits for two groups, not eight rows
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_greedy_kernel(const VerifyParams a) {
+// VEC: rows of whole 16-byte pieces.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads, 4) verify_greedy_kernel(const VerifyParams a) {
   __shared__ uint2 s_warp[kGroup][kWarps];
   __shared__ uint2 s_key[2][kGroup];  // two sets: a CTA may be one group ahead of another's reads
+  tc5::grid_wait();
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), size = (int)cl.num_blocks();
   const int b = blockIdx.x / size;
@@ -293,22 +297,44 @@ __global__ void __launch_bounds__(kThreads) verify_greedy_kernel(const VerifyPar
 #pragma unroll
     for (int r = 0; r < kGroup; r++) hi[r] = lo[r] = 0;
     const T* p = P + acc * a.p_row;
-    for (uint32_t v0 = (uint32_t)(rank * kThreads + tid); v0 < V; v0 += step * 4) {
-      float x[kGroup][4];
+    if constexpr (VEC) {
+      constexpr uint32_t W = 16 / sizeof(T);
+      const uint32_t chunks = V / W;
+      for (uint32_t c0 = (uint32_t)(rank * kThreads + tid); c0 < chunks; c0 += step * 2) {
+        uint4 x[kGroup][2];
 #pragma unroll
-      for (int r = 0; r < kGroup; r++)
+        for (int r = 0; r < kGroup; r++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const uint32_t v = v0 + k * step;
-          x[r][k] = r < rows && v < V ? to_f32(p[r * a.p_row + v]) : __uint_as_float(0x7fc00000u);
-        }
+          for (int k = 0; k < 2; k++)
+            if (r < rows && c0 + k * step < chunks) x[r][k] = reinterpret_cast<const uint4*>(p + r * a.p_row)[c0 + k * step];
 #pragma unroll
-      for (int r = 0; r < kGroup; r++)
+        for (int r = 0; r < kGroup; r++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const uint32_t v = v0 + k * step;
-          if (v < V) take(x[r][k], v, hi[r], lo[r]);
-        }
+          for (int k = 0; k < 2; k++) {
+            if (r >= rows || c0 + k * step >= chunks) continue;
+            const T* e = reinterpret_cast<const T*>(&x[r][k]);
+#pragma unroll
+            for (uint32_t i = 0; i < W; i++) take(to_f32(e[i]), (c0 + k * step) * W + i, hi[r], lo[r]);
+          }
+      }
+    } else {
+      for (uint32_t v0 = (uint32_t)(rank * kThreads + tid); v0 < V; v0 += step * 4) {
+        float x[kGroup][4];
+#pragma unroll
+        for (int r = 0; r < kGroup; r++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const uint32_t v = v0 + k * step;
+            x[r][k] = r < rows && v < V ? to_f32(p[r * a.p_row + v]) : __uint_as_float(0x7fc00000u);
+          }
+#pragma unroll
+        for (int r = 0; r < kGroup; r++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const uint32_t v = v0 + k * step;
+            if (v < V) take(x[r][k], v, hi[r], lo[r]);
+          }
+      }
     }
 #pragma unroll
     for (int r = 0; r < kGroup; r++) {
@@ -358,27 +384,24 @@ int cluster_size(int64_t seqs, int64_t V) {
   return c;
 }
 
-template <typename Kernel, typename... Args>
-cudaError_t launch_clusters(Kernel kernel, int64_t seqs, int cluster, size_t smem, cudaStream_t st,
-                            Args... args) {
-  if (smem > 48 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+template <typename T>
+cudaError_t launch_draft(const VerifyParams& p, int64_t seqs, int cluster, int nb, cudaStream_t st) {
+  static std::atomic<uint64_t> allowed{0};
+  const size_t smem = (size_t)nb * sizeof(double);
+  if (smem > 48 * 1024 - 1024) {
+    const cudaError_t e = allow_smem((const void*)verify_draft_kernel<T>, smem, allowed);
     if (e != cudaSuccess) return e;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(seqs * cluster));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  kernel_launch_count()++;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
+  return launch_after(verify_draft_kernel<T>, dim3((unsigned)(seqs * cluster)), kThreads, smem, cluster, st, p, nb);
+}
+
+template <typename T>
+cudaError_t launch_greedy(const VerifyParams& p, int64_t seqs, int cluster, cudaStream_t st) {
+  constexpr int64_t W = 16 / sizeof(T);
+  const dim3 grid((unsigned)(seqs * cluster));
+  if (aligned16(p.p) && p.V % W == 0 && p.p_row % W == 0 && p.p_seq % W == 0)
+    return launch_after(verify_greedy_kernel<T, true>, grid, kThreads, 0, cluster, st, p);
+  return launch_after(verify_greedy_kernel<T, false>, grid, kThreads, 0, cluster, st, p);
 }
 
 vtq_status check(const char* fn, const vtq_verify_args* a, bool greedy) {
@@ -419,13 +442,11 @@ vtq_status vtq_verify_draft(const vtq_verify_args* a, void* stream) {
   const int64_t blocks = (a->vocab + kBlock - 1) / kBlock;
   const int nb = (int)((blocks + c - 1) / c);
   const VerifyParams p = params(a);
-  const size_t smem = (size_t)nb * sizeof(double);
-  if (smem > 200 * 1024)
+  if ((size_t)nb * sizeof(double) > 200 * 1024)
     return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "vtq_verify_draft: not implemented (vocab too large)");
-  cudaError_t e = a->dtype == VTQ_F32 ? launch_clusters(verify_draft_kernel<float>, a->seqs, c, smem, st, p, nb)
-                  : a->dtype == VTQ_F16
-                      ? launch_clusters(verify_draft_kernel<__half>, a->seqs, c, smem, st, p, nb)
-                      : launch_clusters(verify_draft_kernel<__nv_bfloat16>, a->seqs, c, smem, st, p, nb);
+  const cudaError_t e = a->dtype == VTQ_F32   ? launch_draft<float>(p, a->seqs, c, nb, st)
+                        : a->dtype == VTQ_F16 ? launch_draft<__half>(p, a->seqs, c, nb, st)
+                                              : launch_draft<__nv_bfloat16>(p, a->seqs, c, nb, st);
   return serve_cuda(e, "vtq_verify_draft");
 }
 
@@ -435,9 +456,9 @@ vtq_status vtq_verify_greedy(const vtq_verify_args* a, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int c = cluster_size(a->seqs, a->vocab);
   const VerifyParams p = params(a);
-  cudaError_t e = a->dtype == VTQ_F32 ? launch_clusters(verify_greedy_kernel<float>, a->seqs, c, 0, st, p)
-                  : a->dtype == VTQ_F16 ? launch_clusters(verify_greedy_kernel<__half>, a->seqs, c, 0, st, p)
-                                        : launch_clusters(verify_greedy_kernel<__nv_bfloat16>, a->seqs, c, 0, st, p);
+  const cudaError_t e = a->dtype == VTQ_F32   ? launch_greedy<float>(p, a->seqs, c, st)
+                        : a->dtype == VTQ_F16 ? launch_greedy<__half>(p, a->seqs, c, st)
+                                              : launch_greedy<__nv_bfloat16>(p, a->seqs, c, st);
   return serve_cuda(e, "vtq_verify_greedy");
 }
 
