@@ -88,12 +88,14 @@ __global__ void __launch_bounds__(attention_threads<T, DP, RT>(), 1)
       return;
     }
   }
-  part_role<T, DP, P::KT, P::WARPS>(p, tmk, tmv, smem, base, cta - x, p.ctas - x);
+  part_role<T, DP, P::KT, P::WARPS, RT == 0>(p, tmk, tmv, smem, base, cta - x, p.ctas - x);
 }
 
-// Adds the parts of each row (query head of a token): one warp a row. The kernel before lets it start early;
-// until it is done the warp goes through its own code once, on made-up places and with nothing stored, so
-// that the instructions are there when the parts are (they are most of its time otherwise: 8 us for 128 rows).
+// Adds the parts of each row (query head of a token): one warp a row. A row whose keys one part took alone is
+// there already. The kernel before lets this one start early; until it is done the warps of the first wave go
+// through their own code once, on made-up places and with nothing stored, so that the instructions are there
+// when the parts are (8 us for 128 rows without). What is left is a chain of four reads from L2: a row's entry, its
+// parts' numbers, their (m, l) and first values at once, and their further values.
 template <typename T, int DP>
 __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttnParams p) {
   const int lane = threadIdx.x & 31;
@@ -102,7 +104,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
   if (row >= (int)p.a.tokens * heads) return;
   const int token = row / heads, head = row - token * heads, g = head / p.group;
 #pragma unroll 1
-  for (int pass = 0; pass < 2; pass++) {
+  for (int pass = (int)blockIdx.x < 8 * p.ctas ? 0 : 1; pass < 2; pass++) {
     if (pass) tc5::grid_wait();
     int4 of = make_int4(0, 0, p.prefix ? 0 : -1, 1);
     if (pass) of = p.rows[token];
@@ -129,6 +131,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     }
     if (!pass) rr[0] = rr[1] = 0;
     const int parts = count[0] + count[1];
+    if (pass && !p.on_tiles && count[0] == 1 && of.z < 0) return;  // written by the part
     // Part i's (m, l) of the row, and its o.
     auto at = [&](int i, const float*& o) {
       const bool k = i >= count[0], tiles = k && p.on_tiles;
@@ -138,49 +141,51 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
       o = s + (pass ? 2 * rows : 0) + r * DP;
       return s + 2 * r;
     };
-    float m = -INFINITY;
-    for (int i = lane; i < parts; i += 32) {
-      const float* o;
-      m = fmaxf(m, *at(i, o));
-    }
+    constexpr int kAtOnce = DP > 128 ? 4 : 8, V = DP / 32;  // parts read together; values a lane
+    float v[kAtOnce][V];
+    auto load = [&](int i) {
+#pragma unroll
+      for (int k = 0; k < kAtOnce; k++) {
+        const float* s;
+        at(max(min(i + k, parts - 1), 0), s);
+        if constexpr (V == 2) {
+          const float2 x = *reinterpret_cast<const float2*>(s + 2 * lane);
+          v[k][0] = x.x, v[k][1] = x.y;
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; e += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(s + 32 * e + 4 * lane);
+            v[k][e] = x.x, v[k][e + 1] = x.y, v[k][e + 2] = x.z, v[k][e + 3] = x.w;
+          }
+        }
+      }
+    };
+    const float* unused;
+    float2 ml = lane < parts ? *reinterpret_cast<const float2*>(at(lane, unused)) : make_float2(-INFINITY, 0.0f);
+    load(0);
+    float m = ml.x;
+    for (int i = lane + 32; i < parts; i += 32) m = fmaxf(m, *at(i, unused));
 #pragma unroll
     for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     const float um = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, acc[DP / 32];
+    float l = 0.0f, f = 0.0f, acc[V];
 #pragma unroll
-    for (int e = 0; e < DP / 32; e++) acc[e] = 0.0f;
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-      float f = 0.0f;
-      if (i0 + lane < parts) {
-        const float* o;
-        const float2 ml = *reinterpret_cast<const float2*>(at(i0 + lane, o));
+    for (int e = 0; e < V; e++) acc[e] = 0.0f;
+#pragma unroll 1
+    for (int i = 0; i < parts; i += kAtOnce) {
+      if (i) load(i);
+      if (i % 32 == 0) {
+        if (i) ml = i + lane < parts ? *reinterpret_cast<const float2*>(at(i + lane, unused)) : make_float2(-INFINITY, 0.0f);
         f = exp2_fast(ml.x - um);
         l += f * ml.y;
         if (ml.y == 0.0f) f = 0.0f;  // nothing in it, whatever its o holds
       }
-      const int n = min(32, parts - i0);
-      // Several parts' loads at once.
-      constexpr int kAtOnce = DP > 64 ? 4 : 8;
-      for (int i = 0; i < n; i += kAtOnce) {
-        float2 v[kAtOnce][DP / 64];
-        float fi[kAtOnce];
 #pragma unroll
-        for (int k = 0; k < kAtOnce; k++) {
-          fi[k] = __shfl_sync(0xffffffffu, f, (i + k) & 31);
-          if (i + k >= n) fi[k] = 0.0f;
-          const float* s;
-          at(min(i0 + i + k, parts - 1), s);
+      for (int k = 0; k < kAtOnce; k++) {
+        const float fk = __shfl_sync(0xffffffffu, f, (i + k) & 31);
 #pragma unroll
-          for (int e = 0; e < DP / 64; e++)
-            v[k][e] = fi[k] != 0.0f ? *reinterpret_cast<const float2*>(s + 64 * e + 2 * lane) : make_float2(0.0f, 0.0f);
-        }
-#pragma unroll
-        for (int k = 0; k < kAtOnce; k++)
-#pragma unroll
-          for (int e = 0; e < DP / 64; e++) {
-            acc[2 * e] = fmaf(fi[k], v[k][e].x, acc[2 * e]);
-            acc[2 * e + 1] = fmaf(fi[k], v[k][e].y, acc[2 * e + 1]);
-          }
+        for (int e = 0; e < V; e++)
+          if (i + k < parts && fk != 0.0f) acc[e] = fmaf(fk, v[k][e], acc[e]);
       }
     }
 #pragma unroll
@@ -188,18 +193,11 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
     T* out = static_cast<T*>(p.a.out) + token * p.a.o_tok + head * p.a.o_head;
 #pragma unroll
-    for (int e = 0; e < DP / 64; e++) {
-      const int d = 64 * e + 2 * lane;
-      if (!pass || d >= D) continue;
-      if (p.o_wide) {
-        *reinterpret_cast<uint32_t*>(out + d) = pack2<T>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-      } else {
-        out[d] = from_f32<T>(acc[2 * e] * inv);
-        out[d + 1] = from_f32<T>(acc[2 * e + 1] * inv);
-      }
+    for (int e = 0; e < V; e += 2) {
+      const int d = V == 2 ? 2 * lane : 32 * (e & ~3) + 4 * lane + (e & 2);
+      if (pass && d < D) store_pair<T>(p, out + d, acc[e] * inv, acc[e + 1] * inv);
     }
-    if (pass && p.a.lse && lane == 0)
-      p.a.lse[token * p.a.lse_tok + head] = l == 0.0f ? -INFINITY : (um + log2f(l)) * 0.69314718055994531f;
+    if (pass && p.a.lse && lane == 0) p.a.lse[token * p.a.lse_tok + head] = lse_of(m, l);
   }
 }
 
@@ -279,6 +277,7 @@ cudaError_t launch(AttnParams p, cudaStream_t st) {
   smem += 1024;  // alignment
   p.warps = P::WARPS;
   p.tile = P::KT;
+  p.tile_shift = P::KT == 32 ? 5 : 4;
   auto kernel = attention_kernel<T, DP, RT>;
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem((const void*)kernel, smem, allowed);
@@ -336,6 +335,8 @@ vtq_status vtq_attention_paged(const vtq_attention_args* a, void* ws, size_t ws_
   AttnParams p = {};
   p.a = *a;
   p.group = (int)(a->heads / a->kv.kv_heads);
+  p.by_group = divisor(p.group);
+  p.by_page = divisor(a->kv.page_size);
   p.dim_padded = padded_dim(a->kv.head_dim);
   p.ctas = num_sms();
   p.keys_max = (int)(a->kv.table_width * a->kv.page_size);

@@ -15,10 +15,24 @@ constexpr int kRows = 16;      // query rows of a segment: M of the MMA
 constexpr int kTileRows = 128; // of a segment of the prefix on tcgen05
 constexpr int kMaxSeqs = 1024;
 
+// n / d for 0 <= n < 2^31, d >= 1: with 2^s >= d, m = floor(2^32 (2^s - d) / d) + 1 and (mulhi(m, n) + n) >> s.
+struct Divisor {
+  uint32_t mul;
+  int shift;
+  __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi(mul, (uint32_t)n) + (uint32_t)n) >> shift); }
+};
+inline Divisor divisor(int64_t d) {
+  int s = 0;
+  while ((1ll << s) < d) s++;
+  return Divisor{(uint32_t)((((uint64_t)((1ll << s) - d)) << 32) / (uint64_t)d + 1), s};
+}
+
 struct AttnParams {
   vtq_attention_args a;
   int group;        // query heads of a kv head
-  int tile;         // keys of a part's tile
+  int tile;         // keys of a part's tile, a power of two,
+  int tile_shift;   // and which
+  Divisor by_page, by_group;
   int ctas, warps;  // of the grid; warps of a CTA that take parts
   int box;          // positions of a TMA box: a page, or an even part of it; 0: none, rows are gathered
   int keys_max;     // positions that the table can hold
@@ -35,7 +49,7 @@ struct AttnParams {
   int tile_rt, tile_streams;         // blocks of kTileRows rows of a segment; softmax warpgroups of a CTA
   int tile_segs, tiles_each;         // segments of a kv head, steps (of tile_streams / tile_rt key tiles) of each
   int tiles_total;                   // steps in all
-  int step_cost, part_cost;          // what a CTA takes for a step, and for a part's tile
+  int step_cost, part_cost, seg_cost;  // what a CTA takes for a step, for a part's tile, and to begin a segment
   float* tile_part;                  // slots of kTileRows (m, l) and o
 };
 
@@ -63,6 +77,25 @@ __device__ __forceinline__ bool sees_prefix(const AttnParams& p, const Plan& pl,
   const int n = seq_rows(pl, b);
   return n > 0 && pl.len[b] - n + 1 >= p.prefix;
 }
+
+// The list's entry b: its query rows, and the keys of its tiles.
+struct Entry {
+  int rows, keys;
+};
+__device__ __forceinline__ Entry entry_of(const AttnParams& p, const Plan& pl, int b, int B) {
+  Entry e;
+  if (b < B) {
+    e.rows = seq_rows(pl, b) * p.group;
+    e.keys = min(pl.len[b], p.keys_max);
+    if (sees_prefix(p, pl, b)) e.keys = e.keys > p.prefix ? e.keys - (p.prefix & -p.tile) : 0;
+  } else {
+    e.rows = p.on_tiles ? 0 : (int)p.a.tokens * p.group;  // the prefix has a list of its own then
+    e.keys = pl.len[B];
+  }
+  return e;
+}
+__device__ __forceinline__ int blocks_of(const Entry& e) { return (e.rows + kRows - 1) / kRows; }
+__device__ __forceinline__ int tiles_of(const AttnParams& p, const Entry& e) { return (e.keys + p.tile - 1) >> p.tile_shift; }
 
 // Built by all threads of a CTA in its shared memory; base[0] = the parts' tiles in all, base[1] = parts in
 // use, base[2] = CTAs that work on the prefix's own tiles (the first ones), by the two sides' cost.
@@ -94,18 +127,10 @@ __device__ void build_plan(const AttnParams& p, int* base) {
   int st = 0, ss = 0;
   for (int pass = 0; pass < 2; pass++) {
     for (int b = b0; b < b1; b++) {
-      int rows, keys;
-      if (b < B) {
-        rows = seq_rows(pl, b) * p.group;
-        keys = min(pl.len[b], p.keys_max);
-        if (sees_prefix(p, pl, b)) keys = keys > p.prefix ? keys - p.prefix / p.tile * p.tile : 0;
-      } else {
-        rows = p.on_tiles ? 0 : T * p.group;  // the prefix has a kernel of its own then
-        keys = pl.len[B];
-      }
-      const int segs = (rows + kRows - 1) / kRows * H;
+      const Entry e = entry_of(p, pl, b, B);
+      const int segs = blocks_of(e) * H;
       if (pass) pl.tiles[b] = st, pl.segs[b] = ss;
-      st += segs * ((keys + p.tile - 1) / p.tile);
+      st += segs * tiles_of(p, e);
       ss += segs;
     }
     if (pass == 0) {
@@ -126,7 +151,7 @@ __device__ void build_plan(const AttnParams& p, int* base) {
   __syncthreads();
   if (tid == 0) {
     const int64_t steps = p.on_tiles && pl.len[B] ? p.tiles_total : 0, tiles = pl.tiles[n];
-    const int64_t a = steps * p.step_cost, b = tiles * p.part_cost;
+    const int64_t a = steps * p.step_cost, b = tiles * p.part_cost + pl.segs[n] * (int64_t)p.seg_cost;
     int x = 0;
     if (steps) x = tiles ? (int)min(max((p.ctas * a + (a + b) / 2) / (a + b), (int64_t)1), (int64_t)p.ctas - 1) : p.ctas;
     x = (int)min((int64_t)x, steps);
@@ -138,29 +163,22 @@ __device__ void build_plan(const AttnParams& p, int* base) {
   __syncthreads();
 }
 
-// Part w of W covers tiles [first(w), first(w + 1)) of `total`; part_of is its inverse.
+// Part w of W covers tiles [first(w), first(w + 1)) of `total`.
 __device__ __forceinline__ int first_tile(int total, int W, int w) { return (int)((int64_t)total * w / W); }
-__device__ __forceinline__ int part_of(int total, int W, int t) { return (int)((((int64_t)t + 1) * W - 1) / total); }
 
 // Where a part stands: sequence, row block, head, tile. Tiles lie on multiples of their size, so that pages
 // and boxes do not straddle them: the first one of a sequence behind the prefix may begin inside it.
-struct Cursor {
+struct __align__(16) Cursor {
   int b, mb, g, t, nt;  // nt tiles in a segment of b
   int mbs;              // row blocks of b
-  int first, lo, end;   // of b: its first tile's position; its keys are lo .. end
+  int lo, end;          // of b: its keys; the first tile lies at lo, rounded down
 };
 
-__device__ __forceinline__ int seq_tiles(const AttnParams& p, const Plan& pl, int b, int B, int* mbs) {
-  const int H = (int)p.a.kv.kv_heads;
-  *mbs = (pl.segs[b + 1] - pl.segs[b]) / H;
-  const int segs = *mbs * H;
-  return segs ? (pl.tiles[b + 1] - pl.tiles[b]) / segs : 0;
-}
-
 __device__ __forceinline__ void enter(const AttnParams& p, const Plan& pl, int B, Cursor& c) {
-  c.nt = seq_tiles(p, pl, c.b, B, &c.mbs);
+  const Entry e = entry_of(p, pl, c.b, B);
+  c.mbs = blocks_of(e);
+  c.nt = c.mbs ? tiles_of(p, e) : 0;
   c.lo = c.b < B && sees_prefix(p, pl, c.b) ? p.prefix : 0;
-  c.first = c.lo / p.tile * p.tile;
   c.end = c.b < B ? min(pl.len[c.b], p.keys_max) : pl.len[B];
 }
 
@@ -181,9 +199,9 @@ __device__ Cursor seek(const AttnParams& p, const Plan& pl, int B, int tile) {
   return c;
 }
 
-// The next tile; true where it begins another segment. Never called behind the last tile.
-__device__ __forceinline__ bool advance(const AttnParams& p, const Plan& pl, int B, Cursor& c) {
-  if (++c.t < c.nt) return false;
+// The next tile; t = 0 where it begins another segment. Never called behind the last tile.
+__device__ __forceinline__ void advance(const AttnParams& p, const Plan& pl, int B, Cursor& c) {
+  if (++c.t < c.nt) return;
   c.t = 0;
   if (++c.g == (int)p.a.kv.kv_heads) {
     c.g = 0;
@@ -194,7 +212,6 @@ __device__ __forceinline__ bool advance(const AttnParams& p, const Plan& pl, int
       } while (c.b <= B && c.nt == 0);
     }
   }
-  return true;
 }
 
 // The sequence that owns a row of q, or -1.
@@ -252,11 +269,24 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
-// Whether either half of a word is an infinity or a NaN.
 template <typename T>
-__device__ __forceinline__ bool odd_word(uint32_t w) {
-  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  return (w & e) == e || ((w >> 16) & e) == e;
+__device__ __forceinline__ void store_pair(const AttnParams& p, T* out, float a, float b) {
+  if (p.o_wide) {
+    *reinterpret_cast<uint32_t*>(out) = pack2<T>(a, b);
+  } else {
+    out[0] = from_f32<T>(a);
+    out[1] = from_f32<T>(b);
+  }
+}
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) + log2f(l)) * 0.69314718055994531f;
+}
+// Whether either half of a word is an infinity or a NaN (an exponent of ones carries into the sign's place): not 0.
+template <typename T>
+__device__ __forceinline__ uint32_t odd_word(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  constexpr uint32_t one = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+  return ((w & e) + one) & 0x80008000u;
 }
 
 }  // namespace
