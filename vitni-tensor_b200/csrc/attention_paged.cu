@@ -225,6 +225,19 @@ TileCut tile_cut(const vtq_attention_args& a) {
   c.total = a.kv.kv_heads * (int64_t)c.segs * c.each;
   return c;
 }
+// Fitted to when the two kinds of CTA end, on batches of 16 .. 256 sequences behind 8199 .. 32768 keys. A step is 128
+// keys and 256 rows, 64 keys and 128 rows at head_dim 256; a part's tile 32 keys, 16 there.
+Costs costs(int dp) {
+  Costs c;
+  c.tile = dp == 64 ? 315 : dp == 128 ? 560 : 660;
+  c.segment = 300;
+  c.begin = 27000;  // until the last of the parts is done: a warp by itself is slow
+  c.step = dp == 64 ? 4000 : dp == 128 ? 4900 : 3050;
+  c.tile_segment = 20000;
+  c.tile_bytes = (dp == 256 ? 16 : 32) * dp * 4;
+  return c;
+}
+
 size_t tile_bytes(const vtq_attention_args& a) {
   const TileCut c = tile_cut(a);
   if (!c.on) return 0;
@@ -359,9 +372,7 @@ vtq_status vtq_attention_paged(const vtq_attention_args* a, void* ws, size_t ws_
     p.tile_segs = c.segs;
     p.tiles_each = c.each;
     p.tiles_total = (int)c.total;
-    // Cycles of an SM, measured (head_dim 128: a step of 128 keys and 256 rows; a part's tile of 32 keys).
-    p.step_cost = 4200;
-    p.part_cost = 520;
+    p.cost = costs(p.dim_padded);
     p.tile_part = reinterpret_cast<float*>(at + part_bytes(*a));
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -14,6 +14,7 @@ namespace {
 constexpr int kRows = 16;      // query rows of a segment: M of the MMA
 constexpr int kTileRows = 128; // of a segment of the prefix on tcgen05
 constexpr int kMaxSeqs = 1024;
+constexpr int kBytesPerCycle = 3500;  // from HBM, of all SMs
 
 // n / d for 0 <= n < 2^31, d >= 1: with 2^s >= d, m = floor(2^32 (2^s - d) / d) + 1 and (mulhi(m, n) + n) >> s.
 struct Divisor {
@@ -26,6 +27,13 @@ inline Divisor divisor(int64_t d) {
   while ((1ll << s) < d) s++;
   return Divisor{(uint32_t)((((uint64_t)((1ll << s) - d)) << 32) / (uint64_t)d + 1), s};
 }
+
+// What the two kinds of work take of an SM, in cycles (measured; attention_paged.cu).
+struct Costs {
+  int tile, segment, begin;   // a part's tile, a segment of parts, and what passes before and behind them
+  int step, tile_segment;     // a step of the prefix's own tiles, and a segment of them
+  int tile_bytes;             // of a part's tile, from HBM
+};
 
 struct AttnParams {
   vtq_attention_args a;
@@ -49,7 +57,7 @@ struct AttnParams {
   int tile_rt, tile_streams;         // blocks of kTileRows rows of a segment; softmax warpgroups of a CTA
   int tile_segs, tiles_each;         // segments of a kv head, steps (of tile_streams / tile_rt key tiles) of each
   int tiles_total;                   // steps in all
-  int step_cost, part_cost, seg_cost;  // what a CTA takes for a step, for a part's tile, and to begin a segment
+  Costs cost;
   float* tile_part;                  // slots of kTileRows (m, l) and o
 };
 
@@ -103,8 +111,9 @@ __device__ void build_plan(const AttnParams& p, int* base) {
   const int B = (int)p.a.kv.seqs, T = (int)p.a.tokens, H = (int)p.a.kv.kv_heads;
   const Plan pl = plan_of(base, B);
   __shared__ int s_any, s_bad, s_warp_t[32], s_warp_s[32];
+  __shared__ unsigned long long s_best;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid == 0) s_any = s_bad = 0;
+  if (tid == 0) s_any = s_bad = 0, s_best = ~0ull;
   __syncthreads();
   for (int b = tid; b <= B; b += blockDim.x) {
     pl.q0[b] = p.a.q_start ? min(max(p.a.q_start[b], 0), T) : min(b, T);
@@ -149,14 +158,29 @@ __device__ void build_plan(const AttnParams& p, int* base) {
   }
   if (b0 < n && b1 == n) pl.tiles[n] = st, pl.segs[n] = ss;
   __syncthreads();
+  // CTAs for the prefix: as many as end soonest. The worst of them begins as many segments as its share can touch,
+  // one where the CTAs are a multiple of the segments; the others are bound by HBM where there are many.
+  const int steps = p.on_tiles && pl.len[B] ? p.tiles_total : 0, tiles = pl.tiles[n];
+  if (steps) {
+    const int segments = H * p.tile_segs;
+    unsigned long long best = ~0ull;
+    for (int x = tid + 1; x <= min(p.ctas, steps); x += blockDim.x) {
+      if (x == p.ctas && tiles) break;
+      const int share = (steps + x - 1) / x;
+      const int touched = x % segments == 0 ? 1 : segments % x == 0 ? segments / x : (share - 2) / p.tiles_each + 2;
+      const int64_t mine = (int64_t)share * p.cost.step + (int64_t)touched * p.cost.tile_segment;
+      int64_t others = 0;
+      if (tiles)
+        others = max(((int64_t)tiles * p.cost.tile + (int64_t)pl.segs[n] * p.cost.segment) / (p.ctas - x), (int64_t)tiles * p.cost.tile_bytes / kBytesPerCycle) + p.cost.begin;
+      best = min(best, (unsigned long long)max(mine, others) << 16 | (unsigned)x);
+    }
+    if (best != ~0ull) atomicMin(&s_best, best);
+  }
+  __syncthreads();
   if (tid == 0) {
-    const int64_t steps = p.on_tiles && pl.len[B] ? p.tiles_total : 0, tiles = pl.tiles[n];
-    const int64_t a = steps * p.step_cost, b = tiles * p.part_cost + pl.segs[n] * (int64_t)p.seg_cost;
-    int x = 0;
-    if (steps) x = tiles ? (int)min(max((p.ctas * a + (a + b) / 2) / (a + b), (int64_t)1), (int64_t)p.ctas - 1) : p.ctas;
-    x = (int)min((int64_t)x, steps);
-    base[0] = (int)tiles;
-    base[1] = (int)min(tiles, (int64_t)(p.ctas - x) * p.warps);
+    const int x = steps ? (int)(s_best & 0xffffu) : 0;
+    base[0] = tiles;
+    base[1] = (int)min((int64_t)tiles, (int64_t)(p.ctas - x) * p.warps);
     base[2] = x;
     base[3] = pl.segs[B];
   }
