@@ -91,20 +91,24 @@ __global__ void __launch_bounds__(attention_threads<T, DP, RT>(), 1)
   part_role<T, DP, P::KT, P::WARPS, RT == 0>(p, tmk, tmv, smem, base, cta - x, p.ctas - x);
 }
 
-// Adds the parts of each row (query head of a token): one warp a row. A row whose keys one part took alone is
+// Adds the parts of each row (query head of a token): p.join_warps warps a row, one where the rows fill the SMs, more
+// where they are few and their parts many (one sequence of 4096 keys, 32 rows: 38 us with one). A row whose keys one part took alone is
 // there already. The kernel before lets this one start early; until it is done the warps of the first wave go
 // through their own code once, on made-up places and with nothing stored, so that the instructions are there
 // when the parts are (8 us for 128 rows without). What is left is a chain of four reads from L2: a row's entry, its
 // parts' numbers, their (m, l) and first values at once, and their further values.
+constexpr int kJoinWarps = 8;  // of a block
 template <typename T, int DP>
-__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(32 * kJoinWarps, DP > 128 ? 2 : 3) attention_join_kernel(const __grid_constant__ AttnParams p) {
   const int lane = threadIdx.x & 31;
-  const int row = (int)blockIdx.x * 4 + (threadIdx.x >> 5);
+  __shared__ float s_acc[kJoinWarps][DP];
+  const int warp = threadIdx.x >> 5, split = p.join_warps, sub = warp % split;
+  const int row = ((int)blockIdx.x * kJoinWarps + warp) / split;
   const int heads = (int)p.a.heads, H = (int)p.a.kv.kv_heads, D = (int)p.a.kv.head_dim;
   if (row >= (int)p.a.tokens * heads) return;
   const int token = row / heads, head = row - token * heads, g = head / p.group;
 #pragma unroll 1
-  for (int pass = (int)blockIdx.x < 8 * p.ctas ? 0 : 1; pass < 2; pass++) {
+  for (int pass = (int)blockIdx.x < 4 * p.ctas ? 0 : 1; pass < 2; pass++) {
     if (pass) tc5::grid_wait();
     int4 of = make_int4(0, 0, p.prefix ? 0 : -1, 1);
     if (pass) of = p.rows[token];
@@ -143,11 +147,13 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     };
     constexpr int kAtOnce = DP > 128 ? 4 : 8, V = DP / 32;  // parts read together; values a lane
     float v[kAtOnce][V];
+    // Each lane finds one part's place, which all load from together.
+    const float* place;
+    auto find = [&](int i) { return *reinterpret_cast<const float2*>(at(max(min(i, parts - 1), 0), place)); };
     auto load = [&](int i) {
 #pragma unroll
       for (int k = 0; k < kAtOnce; k++) {
-        const float* s;
-        at(max(min(i + k, parts - 1), 0), s);
+        const float* s = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(place), (i + k) & 31));
         if constexpr (V == 2) {
           const float2 x = *reinterpret_cast<const float2*>(s + 2 * lane);
           v[k][0] = x.x, v[k][1] = x.y;
@@ -160,36 +166,64 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
         }
       }
     };
+    // This warp's parts, and all parts' (m, l).
+    const int lo = parts * sub / split, hi = parts * (sub + 1) / split;
     const float* unused;
-    float2 ml = lane < parts ? *reinterpret_cast<const float2*>(at(lane, unused)) : make_float2(-INFINITY, 0.0f);
+    const float2 none = make_float2(-INFINITY, 0.0f);
+    constexpr int kMl = 4;
+    float2 ml[kMl];
+#pragma unroll
+    for (int j = 0; j < kMl; j++)
+      ml[j] = lane + 32 * j < parts ? *reinterpret_cast<const float2*>(at(lane + 32 * j, unused)) : none;
+    float2 mine = find(lo + lane);
     load(0);
-    float m = ml.x;
-    for (int i = lane + 32; i < parts; i += 32) m = fmaxf(m, *at(i, unused));
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kMl; j++) m = fmaxf(m, ml[j].x);
+#pragma unroll 1
+    for (int i = lane + 32 * kMl; i < parts; i += 32) m = fmaxf(m, *at(i, unused));
 #pragma unroll
     for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     const float um = m == -INFINITY ? 0.0f : m;
     float l = 0.0f, f = 0.0f, acc[V];
 #pragma unroll
+    for (int j = 0; j < kMl; j++) l += exp2_fast(ml[j].x - um) * ml[j].y;
+#pragma unroll 1
+    for (int i = lane + 32 * kMl; i < parts; i += 32) {
+      const float2 x = *reinterpret_cast<const float2*>(at(i, unused));
+      l += exp2_fast(x.x - um) * x.y;
+    }
+#pragma unroll
     for (int e = 0; e < V; e++) acc[e] = 0.0f;
 #pragma unroll 1
-    for (int i = 0; i < parts; i += kAtOnce) {
-      if (i) load(i);
-      if (i % 32 == 0) {
-        if (i) ml = i + lane < parts ? *reinterpret_cast<const float2*>(at(i + lane, unused)) : make_float2(-INFINITY, 0.0f);
-        f = exp2_fast(ml.x - um);
-        l += f * ml.y;
-        if (ml.y == 0.0f) f = 0.0f;  // nothing in it, whatever its o holds
+    for (int i = lo; i < hi; i += kAtOnce) {
+      if ((i - lo) % 32 == 0) {
+        if (i > lo) mine = find(i + lane);
+        f = mine.y == 0.0f ? 0.0f : exp2_fast(mine.x - um);  // nothing in it, whatever its o holds
       }
+      if (i > lo) load(i - lo);
 #pragma unroll
       for (int k = 0; k < kAtOnce; k++) {
-        const float fk = __shfl_sync(0xffffffffu, f, (i + k) & 31);
+        const float fk = __shfl_sync(0xffffffffu, f, (i - lo + k) & 31);
 #pragma unroll
         for (int e = 0; e < V; e++)
-          if (i + k < parts && fk != 0.0f) acc[e] = fmaf(fk, v[k][e], acc[e]);
+          if (i + k < hi && fk != 0.0f) acc[e] = fmaf(fk, v[k][e], acc[e]);
       }
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    if (split > 1) {
+      // The row's warps add theirs in order; a barrier of their own, as other rows of the block may have left.
+#pragma unroll
+      for (int e = 0; e < V; e++) s_acc[warp][e * 32 + lane] = acc[e];
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / split), "r"(32 * split) : "memory");
+      if (sub == 0)
+        for (int w = 1; w < split; w++)
+#pragma unroll
+          for (int e = 0; e < V; e++) acc[e] += s_acc[warp + w][e * 32 + lane];
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / split), "r"(32 * split) : "memory");
+      if (sub) continue;
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
     T* out = static_cast<T*>(p.a.out) + token * p.a.o_tok + head * p.a.o_head;
 #pragma unroll
@@ -204,27 +238,6 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
 int padded_dim(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 int part_warps(int dp) { return dp == 64 ? Part<__half, 64>::WARPS : dp == 128 ? Part<__half, 128>::WARPS : Part<__half, 256>::WARPS; }
 
-// How the prefix goes to the tensor cores' own tiles, and where: more rows than the 16 that one read of
-// a key serves in the part kernel, and keys enough to pay for another launch.
-struct TileCut {
-  bool on;
-  int keys, rt, streams, segs, each;  // keys of a tile; see AttnParams
-  int64_t total;
-};
-TileCut tile_cut(const vtq_attention_args& a) {
-  TileCut c = {};
-  const int64_t rows = a.tokens * (a.heads / a.kv.kv_heads), prefix = std::min(a.shared_len, a.kv.table_width * a.kv.page_size);
-  c.on = rows > 16 && prefix >= 512;
-  const bool wide = a.kv.head_dim > 128;
-  c.keys = wide ? 64 : 128;
-  c.streams = wide ? 1 : 2;
-  c.rt = !wide && rows > kTileRows ? 2 : 1;
-  c.segs = (int)((rows + kTileRows * c.rt - 1) / (kTileRows * c.rt));
-  const int step = c.keys * c.streams / c.rt;
-  c.each = (int)((prefix + step - 1) / step);
-  c.total = a.kv.kv_heads * (int64_t)c.segs * c.each;
-  return c;
-}
 // Fitted to when the two kinds of CTA end, on batches of 16 .. 256 sequences behind 8199 .. 32768 keys. A step is 128
 // keys and 256 rows, 64 keys and 128 rows at head_dim 256; a part's tile 32 keys, 16 there.
 Costs costs(int dp) {
@@ -238,6 +251,31 @@ Costs costs(int dp) {
   return c;
 }
 
+// How the prefix goes to the tensor cores' own tiles, and where: more rows than the 16 that one read of
+// a key serves in the part kernel, and work enough that they end sooner than parts would, by the same costs.
+struct TileCut {
+  bool on;
+  int keys, rt, streams, segs, each;  // keys of a tile; see AttnParams
+  int64_t total;
+};
+TileCut tile_cut(const vtq_attention_args& a) {
+  TileCut c = {};
+  const int64_t rows = a.tokens * (a.heads / a.kv.kv_heads), prefix = std::min(a.shared_len, a.kv.table_width * a.kv.page_size);
+  const bool wide = a.kv.head_dim > 128;
+  c.keys = wide ? 64 : 128;
+  c.streams = wide ? 1 : 2;
+  c.rt = !wide && rows > kTileRows ? 2 : 1;
+  c.segs = (int)((rows + kTileRows * c.rt - 1) / (kTileRows * c.rt));
+  const int step = c.keys * c.streams / c.rt;
+  c.each = (int)((prefix + step - 1) / step);
+  c.total = a.kv.kv_heads * (int64_t)c.segs * c.each;
+  if (rows <= kRows || !prefix) return c;
+  const Costs cost = costs(padded_dim(a.kv.head_dim));
+  const int64_t sms = num_sms(), share = (c.total + sms - 1) / sms, key_tiles = (prefix + (wide ? 15 : 31)) / (wide ? 16 : 32);
+  const int64_t parts = (rows + kRows - 1) / kRows * a.kv.kv_heads * key_tiles * cost.tile / sms + cost.begin / 2;
+  c.on = share * cost.step + ((share + c.each - 1) / c.each) * cost.tile_segment < parts;
+  return c;
+}
 size_t tile_bytes(const vtq_attention_args& a) {
   const TileCut c = tile_cut(a);
   if (!c.on) return 0;
@@ -312,7 +350,11 @@ cudaError_t launch(AttnParams p, cudaStream_t st) {
   }
   e = launch_after(kernel, dim3((unsigned)p.ctas), attention_threads<T, DP, RT>(), smem, 1, st, p, tmk, tmv);
   if (e != cudaSuccess) return e;
-  return launch_after(attention_join_kernel<T, DP>, dim3((unsigned)((p.a.tokens * p.a.heads + 3) / 4)), 128, 0, 1, st, p);
+  const int64_t rows = p.a.tokens * p.a.heads;
+  p.join_warps = 1;
+  while (p.join_warps < kJoinWarps && rows * p.join_warps * 2 <= 16 * p.ctas) p.join_warps *= 2;
+  const int64_t blocks = (rows * p.join_warps + kJoinWarps - 1) / kJoinWarps;
+  return launch_after(attention_join_kernel<T, DP>, dim3((unsigned)blocks), 32 * kJoinWarps, 0, 1, st, p);
 }
 
 template <typename T>

@@ -292,16 +292,27 @@ __device__ __forceinline__ void part_role(const AttnParams& p, const CUtensorMap
     if (tile + 1 < tile1 && at[turn ^ 1].t == 0) queries(at[turn ^ 1]);
     if (!landed(v_full, parity)) break;
     if (!whole) {
-      // A weight of 0 times an infinity or a NaN is no 0: values that some rows must not see (or nobody:
-      // what lies behind a sequence's end in its last page) are taken out of the tile, and added to the
-      // rows that do see them.
+      // A weight of 0 times an infinity or a NaN is no 0: keys that are not there (what lies behind a sequence's end
+      // in its last page, or was in the stage before) become zeros; values that only some rows must not see are
+      // taken out of the tile, and added to the rows that do see them.
+      uint4* const chunks = reinterpret_cast<uint4*>(smem + (v_s - smem_u32(smem)));
+      auto odd_chunk = [](const uint4& v) { return odd_word<T>(v.x) | odd_word<T>(v.y) | odd_word<T>(v.z) | odd_word<T>(v.w); };
       uint32_t odd = 0;
 #pragma unroll 8
-      for (int i = lane; i < KT * CH; i += 32) {
-        const uint4 v = *reinterpret_cast<const uint4*>(smem + (v_s - smem_u32(smem)) + i * 16);
-        odd |= odd_word<T>(v.x) | odd_word<T>(v.y) | odd_word<T>(v.z) | odd_word<T>(v.w);
+      for (int i = lane; i < KT * CH; i += 32) odd |= odd_chunk(chunks[i]);
+      bool any = __any_sync(0xffffffffu, odd != 0);
+      if (any) {
+        odd = 0;
+#pragma unroll 1
+        for (int i = lane; i < KT * CH; i += 32) {
+          if ((valid >> ((i >> 3) & (KT - 1))) & 1) odd |= odd_chunk(chunks[i]);
+          else chunks[i] = make_uint4(0, 0, 0, 0);
+        }
+        any = __any_sync(0xffffffffu, odd != 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // TMA writes the stage next
+        __syncwarp();
       }
-      if (__any_sync(0xffffffffu, odd != 0)) {
+      if (any) {
         T* vt = reinterpret_cast<T*>(smem + (v_s - smem_u32(smem)));
 #pragma unroll
         for (int i = 0; i < DP / 8; i++)

@@ -42,6 +42,7 @@ struct AttnParams {
   int tile_shift;   // and which
   Divisor by_page, by_group;
   int ctas, warps;  // of the grid; warps of a CTA that take parts
+  int join_warps;   // of a row in the joining kernel
   int box;          // positions of a TMA box: a page, or an even part of it; 0: none, rows are gathered
   int keys_max;     // positions that the table can hold
   int prefix;       // min(shared_len, keys_max)
