@@ -359,7 +359,13 @@ def test_attention(S, dtype, counts, lens, heads, kv, dim, page, shared, hnd):
     ([1] * 64, 70, 32, 8, 128, 16, 2048, True),
     ([3] * 11, 5, 16, 2, 256, 32, 777, False),
     ([1] * 130, 3, 4, 4, 72, 128, 6000, True),
-    ([4] * 5, 20, 64, 4, 96, 24, 20000, False)])
+    ([4] * 5, 20, 64, 4, 96, 24, 20000, False),
+    ([1] * 17, 30, 8, 8, 128, 16, 6100, False),
+    ([1] * 24, 40, 40, 8, 64, 7, 4100, True),
+    ([2, 0, 5, 1] * 12, 12, 16, 2, 64, 64, 5000, False),
+    ([1] * 130, 3, 12, 4, 80, 1, 1500, False),
+    ([3] * 11, 5, 16, 2, 256, 32, 3001, False),
+    ([8] * 100, 30, 32, 2, 128, 16, 90, True)])             # a short prefix, of 12800 rows
 def test_attention_long_prefix(S, dtype, counts, own, heads, kv, dim, page, shared, hnd):
     g = gen(shared + dim)
     lens = [shared + n + int(e) for n, e in zip(counts, torch.randint(0, own, (len(counts),), generator=g, device="cuda"))]
@@ -378,12 +384,13 @@ def test_attention_long_prefix(S, dtype, counts, own, heads, kv, dim, page, shar
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-def test_attention_growing_and_negative_scores(S, dtype):
+@pytest.mark.parametrize("heads,kv,shared", [(8, 2, 1500), (32, 8, 6000)])
+def test_attention_growing_and_negative_scores(S, dtype, heads, kv, shared):
     """Scores that rise along the prefix by hundreds, so that what was summed before is scaled down again and again;
     and a scale below 0."""
-    counts, shared = [1] * 20, 1500
+    counts = [1] * 20
     lens = [shared + 1 + i for i in range(20)]
-    q, kp, vp, table, kv_len, start = attention_case(gen(12), counts, lens, 8, 2, 64, 16, shared, dtype, False)
+    q, kp, vp, table, kv_len, start = attention_case(gen(12), counts, lens, heads, kv, 64, 16, shared, dtype, False)
     kp[table[0, :shared // 16].long()] *= torch.linspace(0, 6, shared // 16, device="cuda").to(dtype)[:, None, None, None]
     q *= 4
     for scale in (1.0, -0.125, 0.0):
@@ -394,13 +401,13 @@ def test_attention_growing_and_negative_scores(S, dtype):
         assert ((out.double() - want).abs() <= (half_step(dtype) + 2 ** -11) * size + half_step(dtype) * want.abs() + 2 ** -24).all()
 
 
-@pytest.mark.parametrize("shared", [40, 1024])
-def test_attention_padded_batch(S, shared):
+@pytest.mark.parametrize("shared,heads,dim", [(40, 8, 64), (1024, 8, 64), (4096, 16, 128), (3000, 32, 256)])
+def test_attention_padded_batch(S, shared, heads, dim):
     """Empty sequences, one that ends inside the prefix and one at its end, next to ordinary ones; NaN all over the
     slots that nobody reaches, and in keys of the prefix that only the longer ones reach."""
     lens = [0, shared + 3, shared // 2, 0, shared, shared + 50, 1] + [shared + 9] * 20 + [0] * 5
     counts = [1] * len(lens)
-    q, kp, vp, table, kv_len, start = attention_case(gen(13), counts, lens, 8, 4, 64, 16, shared, F16, False, math.nan)
+    q, kp, vp, table, kv_len, start = attention_case(gen(13), counts, lens, heads, 4, dim, 16, shared, F16, False, math.nan)
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     out, lse = S.attention_paged(q, kp, vp, table, kv_len, shared_len=shared, return_lse=True, status=status)
     want, size, want_lse = attention64(q, kp, vp, table, lens, counts, shared)
@@ -412,26 +419,27 @@ def test_attention_padded_batch(S, shared):
     vp[table[0, j // 16].long(), j % 16, 2, 7] = math.inf
     again = S.attention_paged(q, kp, vp, table, kv_len, shared_len=shared)
     see = torch.tensor([n > j for n in lens], device="cuda")
-    assert torch.equal(again[~see], out[~see]) and torch.isposinf(again[see][:, 4:6, 7]).all()
+    assert torch.equal(again[~see], out[~see]) and torch.isposinf(again[see][:, 2 * heads // 4:3 * heads // 4, 7]).all()
     # all of them empty: a table without any page
     none = torch.full_like(table, -1)
     out = S.attention_paged(q, kp, vp, none, torch.zeros_like(kv_len), shared_len=shared, status=status)
     assert (out == 0).all() and status.item() == 0
 
 
-def test_attention_bad_page_of_a_long_prefix(S):
-    counts, shared = [1] * 24, 600
+@pytest.mark.parametrize("heads,kv,shared", [(2, 2, 600), (16, 8, 8000)])
+def test_attention_bad_page_of_a_long_prefix(S, heads, kv, shared):
+    counts, group = [1] * 24, heads // kv
     lens = [shared + 4] * 24
-    q, kp, vp, table, kv_len, start = attention_case(gen(14), counts, lens, 2, 2, 64, 8, shared, BF16, False)
+    q, kp, vp, table, kv_len, start = attention_case(gen(14), counts, lens, heads, kv, 64, 8, shared, BF16, False)
     bad = table.clone()
     bad[0, 30], bad[0, 70] = 10 ** 8, -1
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     out = S.attention_paged(q, kp, vp, bad, kv_len, shared_len=shared, status=status)
     assert status.item() == 2
-    keep = torch.tensor([j for j in range(604) if j // 8 not in (30, 70)], device="cuda")
+    keep = torch.tensor([j for j in range(shared + 4) if j // 8 not in (30, 70)], device="cuda")
     for b in (0, 23):
         rows = torch.where(keep < shared, 0, b)
-        k, v = (c[table[rows, keep // 8].long(), keep % 8].double() for c in (kp, vp))
+        k, v = (c[table[rows, keep // 8].long(), keep % 8].double().repeat_interleave(group, 1) for c in (kp, vp))
         p = torch.softmax(torch.einsum("hd,lhd->hl", q[b].double(), k) / 8, 1)
         assert attention_close(out[b], torch.einsum("hl,lhd->hd", p, v), torch.einsum("hl,lhd->hd", p, v.abs()), BF16)
 
