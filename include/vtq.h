@@ -406,7 +406,8 @@ vtq_status vtq_append_kv(const vtq_append_kv_args* args, void* stream);
  * query that sees no key gives zeros. Query head h reads kv head
  * h / (heads / kv_heads). lse (optional, [tokens][heads] F32): the logarithm of
  * the sum of exp(scale q k), -inf without a key. Rows of q that no sequence
- * owns, and theirs of out, are left alone; what cached positions at or behind
+ * owns, and theirs of out, are left alone unless `clear` has the bit 1 (out:
+ * zeros) or 2 (lse: -inf); what cached positions at or behind
  * kv_len hold has no effect, whatever it is.
  * Keys behind the table's width, and pages that do not exist, count as unseen
  * and set the status word; row starts that decrease leave no sequence a row.
@@ -421,6 +422,7 @@ typedef struct vtq_attention_args {
   const int32_t* kv_len;
   int64_t tokens, heads, shared_len;
   float scale;
+  uint32_t clear;
   uint32_t* status; /* or NULL */
 } vtq_attention_args;
 size_t vtq_attention_paged_workspace_bytes(const vtq_attention_args* args);

@@ -487,6 +487,32 @@ def test_attention_rows_without_owner_strides_and_scale(S):
     assert (out[3:] == 9).all() and (out[..., :3] == 9).all() and (out[..., 67:] == 9).all()
 
 
+@pytest.mark.parametrize("shared", [0, 16])
+def test_attention_allocated_rows_without_owner(S, shared):
+    """In what the function allocates, rows that no sequence owns are zeros and -inf, whatever the memory held."""
+    counts, lens = [1, 2], [20, 45]
+    q, kp, vp, table, kv_len, start = attention_case(gen(7), counts, lens, 4, 2, 64, 8, shared, BF16, False)
+    q = torch.cat([q, torch.full((4, 4, 64), math.nan, dtype=BF16, device="cuda")])
+    want, size, want_lse = attention64(q[:3], kp, vp, table, lens, counts, shared)
+    for _ in range(3):
+        used = [torch.full((7, 4, 64), 8.0, dtype=BF16, device="cuda"), torch.full((7, 4), 8.0, device="cuda")]
+        del used
+        out, lse = S.attention_paged(q, kp, vp, table, kv_len, q_start=start, shared_len=shared, return_lse=True)
+        assert attention_close(out[:3], want, size, BF16)
+        assert (out[3:] == 0).all() and torch.isneginf(lse[3:]).all() and torch.isfinite(lse[:3]).all()
+    mine = torch.full((7, 4, 64), 8.0, dtype=BF16, device="cuda")
+    lse = S.attention_paged(q, kp, vp, table, kv_len, q_start=start, shared_len=shared, out=mine, return_lse=True)[1]
+    assert (mine[3:] == 8).all() and torch.isneginf(lse[3:]).all() and torch.equal(mine[:3], out[:3])
+    # without q_start: row s alone
+    out = S.attention_paged(q, kp, vp, table, kv_len, shared_len=shared)
+    assert (out[2:] == 0).all() and not (out[:2] == 0).all(2).any()
+    # starts that decrease: no owner at all; no sequences at all
+    wrong = torch.tensor([0, 2, 1], dtype=torch.int32, device="cuda")
+    assert (S.attention_paged(q, kp, vp, table, kv_len, q_start=wrong, shared_len=shared) == 0).all()
+    out, lse = S.attention_paged(q, kp, vp, table[:0], kv_len[:0], q_start=start[:1], return_lse=True)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+
+
 def test_attention_bad_pages_and_starts(S):
     """Pages that do not exist count as unseen keys and are reported; starts that decrease own nothing."""
     counts, lens = [1, 1], [40, 40]

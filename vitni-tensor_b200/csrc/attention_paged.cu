@@ -112,7 +112,12 @@ __global__ void __launch_bounds__(32 * kJoinWarps, DP > 128 ? 2 : 3) attention_j
     if (pass) tc5::grid_wait();
     int4 of = make_int4(0, 0, p.prefix ? 0 : -1, 1);
     if (pass) of = p.rows[token];
-    if (!of.w) return;  // no sequence owns the row
+    if (!of.w) {  // no sequence owns the row
+      if ((p.a.clear & 1u) && !sub)
+        for (int d = lane; d < D; d += 32) static_cast<T*>(p.a.out)[token * p.a.o_tok + head * p.a.o_head + d] = from_f32<T>(0.0f);
+      if ((p.a.clear & 2u) && p.a.lse && !sub && !lane) p.a.lse[token * p.a.lse_tok + head] = -INFINITY;
+      return;
+    }
     // The parts of the row's place among the sequence's own rows, and among all rows for the prefix.
     int count[2] = {0, 0}, rr[2] = {0, 0};
     const float* slot0[2] = {p.part, p.part};

@@ -281,12 +281,14 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     g.scale = given(a[7]) ? (float)PyFloat_AsDouble(a[7]) : 1.0f / std::sqrt((float)g.kv.head_dim);
     if (given(a[7]) && PyErr_Occurred()) return nullptr;
     at::Tensor out, lse;
-    // Rows that no sequence owns are the caller's, or zeros.
-    const bool all = !starts && t == g.kv.seqs;
+    // Rows that no sequence owns: left alone in the caller's out, zeros (and -inf) in what is allocated here.
     if (given(a[8])) out = distinct("out", want("out", a[8], 3, {type}, &dev, {t, heads, g.kv.head_dim}));
-    else out = all ? at::empty(q.sizes(), q.options()) : at::zeros(q.sizes(), q.options());
+    else out = g.kv.seqs ? at::empty(q.sizes(), q.options()) : at::zeros(q.sizes(), q.options());
+    if (!given(a[8])) g.clear |= 1;
     if (PyObject_IsTrue(a[9])) {
-      lse = at::full({t, heads}, -std::numeric_limits<float>::infinity(), q.options().dtype(at::kFloat));
+      g.clear |= 2;
+      lse = g.kv.seqs ? at::empty({t, heads}, q.options().dtype(at::kFloat))
+                      : at::full({t, heads}, -std::numeric_limits<float>::infinity(), q.options().dtype(at::kFloat));
       g.lse = static_cast<float*>(ptr(lse));
     }
     g.q = ptr(q), g.q_tok = q.stride(0), g.q_head = q.stride(1);
