@@ -84,7 +84,7 @@ def test_append_refuses_caches(kv, want, text):
     (dict(x_dtype=A.I8), vtq.ERR_NOT_IMPLEMENTED, "k / v"), (dict(tokens=-2), vtq.ERR_INTERNAL, "shape"),
     (dict(rot_dim=63), vtq.ERR_INTERNAL, "rot_dim"), (dict(rot_dim=66), vtq.ERR_INTERNAL, "rot_dim"),
     (dict(rot_dim=0), vtq.ERR_INTERNAL, "rot_dim"), (dict(rope=None), vtq.ERR_INTERNAL, "rot_dim"),
-    (dict(rope=FAKE + 4), vtq.ERR_INTERNAL, "rope"), (dict(k=None), vtq.ERR_INVALID_ARG, "null"),
+    (dict(rope=FAKE + 4), vtq.ERR_INTERNAL, "rope"), (dict(max_pos=0), vtq.ERR_INTERNAL, "rope"), (dict(k=None), vtq.ERR_INVALID_ARG, "null"),
     (dict(q=FAKE, heads=0), vtq.ERR_INTERNAL, "shape"), (dict(q=FAKE, heads=4), vtq.ERR_INVALID_ARG, "null")])
 def test_append(kw, want, text):
     refused(A.function("vtq_append_kv"), want, text, ctypes.byref(append_args(**kw)), None)
