@@ -402,8 +402,8 @@ vtq_status vtq_append_kv(const vtq_append_kv_args* args, void* stream);
  * kv_len[s] cached positions, those of its query tokens the last of them: its
  * query i of n sees the keys 0 .. kv_len[s] - n + i. Positions below shared_len
  * are read through row 0 of the table for every sequence, once for all of them.
- * out = softmax(scale q k) v, [tokens][heads][head_dim] in the cache's type; a
- * query that sees no key gives zeros. Query head h reads kv head
+ * out = softmax(scale q k) v, [tokens][heads][head_dim] in the cache's type, not
+ * over q; a query that sees no key gives zeros. Query head h reads kv head
  * h / (heads / kv_heads). lse (optional, [tokens][heads] F32): the logarithm of
  * the sum of exp(scale q k), -inf without a key. Rows of q that no sequence
  * owns, and theirs of out, are left alone unless `clear` has the bit 1 (out:

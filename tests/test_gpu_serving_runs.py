@@ -7,7 +7,7 @@ import torch
 
 from tests.test_gpu_serving import (BF16, F16, F32, attention64, attention_case, attention_close, codes64, gen, half_step, i8_check,
                               make_cache, turned, verify64)
-from vtq import NotImplementedOp
+from vtq import Internal, NotImplementedOp
 
 pytestmark = pytest.mark.gpu
 
@@ -112,6 +112,34 @@ def test_attention_pages_of_odd_sizes(S, page, dim, hnd):
         out = S.attention_paged(q, kp, vp, table, kv_len, q_start=start, shared_len=cut)
         want, size, _ = attention64(q, kp, vp, table, lens, counts, cut)
         assert attention_close(out, want, size, BF16)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [8, 24, 40, 72, 136, 200, 248])
+@pytest.mark.parametrize("counts,lens,heads,kv,page,shared", [
+    ([1, 3], [50, 70], 4, 2, 16, 32), ([1], [33], 3, 1, 5, 0), ([2] * 40, [2600 + i for i in range(40)], 16, 4, 32, 2555)])
+def test_attention_head_dims(S, dtype, dim, counts, lens, heads, kv, page, shared):
+    q, kp, vp, table, kv_len, start = attention_case(gen(dim), counts, lens, heads, kv, dim, page, shared, dtype, False)
+    out = S.attention_paged(q, kp, vp, table, kv_len, q_start=start, shared_len=shared)
+    want, size, _ = attention64(q, kp, vp, table, lens, counts, shared)
+    assert attention_close(out, want, size, dtype)
+
+
+def test_outputs_over_inputs(S):
+    """Attention refuses to write over its queries; the append takes q itself, but nothing that overlaps it otherwise."""
+    q, kp, vp, table, kv_len, _ = attention_case(gen(5), [1, 1], [20, 9], 4, 2, 64, 8, 0, BF16, False)
+    with pytest.raises(Internal, match="shares memory"):
+        S.attention_paged(q, kp, vp, table, kv_len, out=q)
+    two = torch.zeros(4, 4, 64, dtype=BF16, device="cuda")
+    two[:2] = q
+    with pytest.raises(Internal, match="shares memory"):
+        S.attention_paged(two[:2], kp, vp, table, kv_len, out=two[1:3])
+    assert torch.equal(S.attention_paged(two[:2], kp, vp, table, kv_len, out=two[2:]), S.attention_paged(q, kp, vp, table, kv_len))
+    k = torch.randn(3, 2, 64, generator=gen(6), device="cuda").to(BF16)
+    seq, pos = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.arange(3, dtype=torch.int32, device="cuda")
+    with pytest.raises(Internal, match="shares memory"):
+        S.append_kv(k, k, kp, vp, table, seq, pos, q=two[:3], q_out=two[1:])
+    S.append_kv(k, k, kp, vp, table, seq, pos, q=two[:3], q_out=two[:3])
 
 
 def test_attention_of_the_most_sequences(S):

@@ -5,6 +5,7 @@
 // Errors are C++ exceptions inside and Python exceptions (the package's classes, by status) at the border.
 #include <Python.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/full.h>
@@ -76,6 +77,16 @@ const at::Tensor& distinct(const char* name, const at::Tensor& t) {
   for (int64_t i = 0; i < t.dim(); i++)
     if (t.size(i) > 1 && t.stride(i) == 0) refuse(VTQ_ERR_INTERNAL, name, ": written, but its elements share memory");
   return t;
+}
+
+// An output that is written while `in` is still being read; `same`: unless it is all of it, element for element.
+void apart(const char* name, const at::Tensor& t, const char* in_name, const at::Tensor& in, bool same = false) {
+  if (!t.numel() || !in.numel()) return;
+  const bool one = t.data_ptr() == in.data_ptr() && t.strides() == in.strides() && t.scalar_type() == in.scalar_type();
+  if (one && same) return;
+  const at::MemOverlapStatus s = at::get_overlap_status(t, in);
+  if (t.data_ptr() == in.data_ptr() || s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial)
+    refuse(VTQ_ERR_INTERNAL, name, ": shares memory with ", in_name);
 }
 
 void* ptr(const at::Tensor& t) { return t.data_ptr(); }
@@ -245,6 +256,7 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
       const ScalarType c = THPVariable_Unpack(a[2]).scalar_type();
       out = given(a[10]) ? distinct("q_out", want("q_out", a[10], 3, {c}, &dev, {t, q.size(1), g.kv.head_dim}))
                          : at::zeros(q.sizes(), q.options().dtype(c));
+      if (given(a[10])) apart("q_out", out, "q", q, true);
       if (q.size(1) > 0) {
         g.q = ptr(q), g.q_tok = q.stride(0), g.q_head = q.stride(1), g.heads = q.size(1);
         g.q_out = ptr(out), g.qo_tok = out.stride(0), g.qo_head = out.stride(1);
@@ -282,9 +294,13 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     if (given(a[7]) && PyErr_Occurred()) return nullptr;
     at::Tensor out, lse;
     // Rows that no sequence owns: left alone in the caller's out, zeros (and -inf) in what is allocated here.
-    if (given(a[8])) out = distinct("out", want("out", a[8], 3, {type}, &dev, {t, heads, g.kv.head_dim}));
-    else out = g.kv.seqs ? at::empty(q.sizes(), q.options()) : at::zeros(q.sizes(), q.options());
-    if (!given(a[8])) g.clear |= 1;
+    if (given(a[8])) {
+      out = distinct("out", want("out", a[8], 3, {type}, &dev, {t, heads, g.kv.head_dim}));
+      apart("out", out, "q", q);
+    } else {
+      out = g.kv.seqs ? at::empty(q.sizes(), q.options()) : at::zeros(q.sizes(), q.options());
+      g.clear |= 1;
+    }
     if (PyObject_IsTrue(a[9])) {
       g.clear |= 2;
       lse = g.kv.seqs ? at::empty({t, heads}, q.options().dtype(at::kFloat))

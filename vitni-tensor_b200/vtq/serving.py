@@ -155,7 +155,7 @@ def attention_paged(q, k_pages, v_pages, page_table, kv_len, q_start=None, share
     page_table for every sequence. A query that sees no key gives zeros. scale: 1 / sqrt(head_dim) where not
     given. Returns out [tokens, heads, head_dim], or (out, lse) with lse the float32 [tokens, heads]
     logarithm of the sum of exp(scale q k). Rows that no sequence owns are left alone (in tensors that this
-    function allocates: zeros, and -inf)."""
+    function allocates: zeros, and -inf). out may not share memory with q."""
     return _n.attention_paged(q, k_pages, v_pages, page_table, kv_len, q_start, shared_len, scale, out, return_lse, status)
 
 
