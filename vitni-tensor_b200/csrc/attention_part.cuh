@@ -4,10 +4,11 @@
 // A warp takes a run of key tiles by itself: 16 query rows against KT keys a step with mma.sync (4 of the 16
 // rows are real where a kv head has 4 query heads and a sequence one token: what counts is that the keys
 // arrive) and no barrier but its own. Bound: HBM by bytes, and close behind it the latency of a warp's own
-// instructions (a tile takes some 600 at 5 cycles each), so that warps count more than tiles in flight: 12 of
-// them with one K and one V tile each, the next K asked for behind this one's scores and the next V behind
-// this one's sum (4 warps with three tiles each: 4.5 TB/s on 64 sequences of 1024 keys). Tiles come by TMA,
-// a box for each page or even piece of one, where pages hold 4 positions or more.
+// instructions (5100 cycles a tile, 2000 of them the scores), so that warps count more than tiles in flight:
+// 12 of them with one K and one V tile each, the next K asked for behind this one's scores, the next V behind
+// this one's sum, the next segment's queries behind its last weights. A new segment costs a warp 3000 cycles
+// beside its tiles. Tiles come by TMA, a box for each page or even piece of one, where pages hold 4 positions
+// or more.
 #pragma once
 #include "attention_plan.cuh"
 
