@@ -125,6 +125,16 @@ def test_attention_head_dims(S, dtype, dim, counts, lens, heads, kv, page, share
     assert attention_close(out, want, size, dtype)
 
 
+@pytest.mark.parametrize("seqs,heads,kv,dim,page,shared", [(256, 64, 4, 128, 16, 90), (128, 32, 2, 256, 16, 50), (256, 64, 4, 64, 8, 130)])
+def test_attention_many_rows_behind_a_short_prefix(S, seqs, heads, kv, dim, page, shared):
+    """Segments of one or two steps, several to a CTA."""
+    counts, lens = [8] * seqs, [shared + 8 + i % 30 for i in range(seqs)]
+    q, kp, vp, table, kv_len, start = attention_case(gen(dim), counts, lens, heads, kv, dim, page, shared, BF16, False)
+    out = S.attention_paged(q, kp, vp, table, kv_len, q_start=start, shared_len=shared)
+    want, size, _ = attention64(q, kp, vp, table, lens, counts, shared)
+    assert attention_close(out, want, size, BF16)
+
+
 def test_outputs_over_inputs(S):
     """Attention refuses to write over its queries; the append takes q itself, but nothing that overlaps it otherwise."""
     q, kp, vp, table, kv_len, _ = attention_case(gen(5), [1, 1], [20, 9], 4, 2, 64, 8, 0, BF16, False)
