@@ -381,3 +381,33 @@ def test_inputs_of_another_stream(S):
         y = S.linear_i8(x * big[0], W)
     s.synchronize()
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("t", [1, 2, 7, 15, 16, 17])
+@pytest.mark.parametrize("k,n", [(1, 3), (8, 128), (129, 200), (1000, 1), (1030, 700), (4096, 4096), (5001, 640), (8192, 1100), (8200, 128), (4096, 40000)])
+@pytest.mark.parametrize("xd", [F32, F16, BF16])
+def test_linear_i8_few_tokens(S, t, k, n, xd):
+    """The bits of the codes' own kernel and the product of its codes, whichever way the call takes."""
+    g = gen(t + k + n)
+    wide = 3 * torch.randn(t, k + 3, generator=g, device="cuda").to(xd)
+    W = weights(S, g, n, k)
+    bias = torch.randn(n, generator=g, device="cuda")
+    for x in (wide[:, :k].contiguous(), wide[:, 1:k + 1]):
+        q, s = S.quantize_tokens(x)
+        for yd in (F32, xd):
+            want = S.linear_i8(q, W, bias=bias, x_scale=s, out_dtype=yd)
+            assert torch.equal(S.linear_i8(x, W, bias=bias, out_dtype=yd), want)
+    x = wide[:, :k].contiguous()
+    x[0] = 0
+    x[-1, k // 2] = float("inf")
+    q, s = S.quantize_tokens(x)
+    assert torch.equal(S.linear_i8(x, W).nan_to_num(7.0), S.linear_i8(q, W, x_scale=s, out_dtype=xd).nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("t", [4, 200])
+def test_linear_i8_over_its_own_input(S, t):
+    x = torch.randn(t, 2048, generator=gen(1), device="cuda")
+    W = weights(S, gen(2), 2048, 2048)
+    want = S.linear_i8(x, W)
+    S.linear_i8(x, W, out=x)
+    assert torch.equal(x, want)
