@@ -18,7 +18,7 @@
 // that V and the cluster size alone decide: plain 32-bit sums move the cut
 // between two tokens by about 1e-7 of the total, which over 1e5 tokens is a
 // different token once in some hundred draws. 128 x 8 rows of 100003 in f32:
-// 31 us (3.3 TB/s: the error sums take instructions, the ends of the pass
+// 27 us (3.9 TB/s: the error sums take instructions, the ends of the pass
 // latency). Greedy, 64 x 8 rows of 32000 in f32,
 // 16 bytes a load: 17 us (3.9 TB/s; 23 with single values).
 #include <cooperative_groups.h>
@@ -79,11 +79,20 @@ template <typename T>
 struct Strips {
   T a[kStrips], b[kStrips];
   __device__ __forceinline__ void load(const T* p, const T* q, int64_t e0, int64_t v1, bool sub) {
+    const int n = (int)min(v1 - e0, (int64_t)kBlock);  // of this lane's places
+    const T *pe = p + e0, *qe = sub && q ? q + e0 : nullptr;
+    if (__all_sync(0xffffffffu, n > 32 * (kStrips - 1))) {
 #pragma unroll
-    for (int k = 0; k < kStrips; k++) {
-      const bool in = e0 + 32 * k < v1;
-      a[k] = in ? p[e0 + 32 * k] : from_f32<T>(0.0f);
-      b[k] = in && sub && q ? q[e0 + 32 * k] : from_f32<T>(0.0f);
+      for (int k = 0; k < kStrips; k++) {
+        a[k] = pe[32 * k];
+        b[k] = qe ? qe[32 * k] : from_f32<T>(0.0f);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kStrips; k++) {
+        a[k] = 32 * k < n ? pe[32 * k] : from_f32<T>(0.0f);
+        b[k] = 32 * k < n && qe ? qe[32 * k] : from_f32<T>(0.0f);
+      }
     }
   }
   __device__ __forceinline__ Left left_at(int k, int64_t e0, int64_t only, bool sub) const {
@@ -156,7 +165,6 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const VerifyP
   // Twice at most: where p - q leaves nothing at all, the token is drawn from p.
   for (int pass = 0; pass < 2; pass++) {
     const bool sub = pass == 0 && acc < n;
-    int64_t last = -1;  // the last token that has any weight
     for (int j = warp; j < mine; j += kWarps) {
       const int64_t e0 = v0 + (int64_t)j * kBlock + lane;
       Strips<T> now;
@@ -169,17 +177,10 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const VerifyP
         const float s = __fadd_rn(hi, r.r), t = __fsub_rn(s, hi);
         lo = __fadd_rn(lo, __fadd_rn(__fadd_rn(__fsub_rn(hi, __fsub_rn(s, t)), __fsub_rn(r.r, t)), r.e));
         hi = s;
-        if (r.r > 0.0f) last = e0 + 32 * k;
       }
       const double s = warp_sum((double)hi + (double)lo);
       if (lane == 0) sums[j] = s;
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const int64_t t = __shfl_xor_sync(0xffffffffu, last, o);
-      last = last > t ? last : t;
-    }
-    if (lane == 0) s_lastw[warp] = last;
     __syncthreads();
     // Inclusive scan of the block sums: each thread a run of them, then the runs.
     const int per = (mine + kThreads - 1) / kThreads, j0 = min(tid * per, mine), j1 = min(j0 + per, mine);
@@ -197,28 +198,50 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const VerifyP
     for (int w = 0; w < warp; w++) before += s_warp[w];
     base += before;
     for (int j = j0; j < j1; j++) sums[j] += base;
-    if (tid == 0) {
-      int64_t l = -1;
-      for (int w = 0; w < kWarps; w++) l = l > s_lastw[w] ? l : s_lastw[w];
-      s_last = l;
-    }
     __syncthreads();
     if (tid == 0) s_total = mine ? sums[mine - 1] : 0.0;
     cl.sync();
     // The other CTAs' totals, in rank order: the same numbers in every CTA.
     double total = 0.0, start = 0.0;
-    int64_t any = -1;
     for (int c = 0; c < size; c++) {
       if (c == rank) start = total;
       total += *cl.map_shared_rank(&s_total, c);
-      const int64_t l = *cl.map_shared_rank(&s_last, c);
-      any = any > l ? any : l;
     }
     if (pass == 0 && sub && !(total > 0.0)) {
       cl.sync();  // everybody has read the totals; the next pass writes them again
       continue;
     }
     const double cut = fmax((double)u[a.K] * total, 0.0);
+    int64_t any = -1;
+    if (!(total > cut)) {
+      // u of 1 or more, or no finite total: the last token that has any weight.
+      int64_t last = -1;
+      for (int j = warp; j < mine; j += kWarps) {
+        const int64_t e0 = v0 + (int64_t)j * kBlock + lane;
+        Strips<T> now;
+        now.load(p, q, e0, v1, sub);
+#pragma unroll
+        for (int k = 0; k < kStrips; k++)
+          if (now.left_at(k, e0, only, sub).r > 0.0f) last = e0 + 32 * k;
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) {
+        const int64_t t = __shfl_xor_sync(0xffffffffu, last, o);
+        last = last > t ? last : t;
+      }
+      if (lane == 0) s_lastw[warp] = last;
+      __syncthreads();
+      if (tid == 0) {
+        int64_t l = -1;
+        for (int w = 0; w < kWarps; w++) l = l > s_lastw[w] ? l : s_lastw[w];
+        s_last = l;
+      }
+      cl.sync();
+      for (int c = 0; c < size; c++) {
+        const int64_t l = *cl.map_shared_rank(&s_last, c);
+        any = any > l ? any : l;
+      }
+    }
     const double end = start + s_total;  // the sum that the next CTA takes for its start
     int32_t* out = a.tokens + (int64_t)b * a.ld_tokens;
     if (rank == 0) {
@@ -226,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const VerifyP
         if (i != acc) out[i] = i < acc ? draft[i] : -1;
       if (tid == 0) {
         a.accepted[b] = acc;
-        if (!(total > cut)) out[acc] = (int32_t)any;  // u of 1 or more, or no finite total
+        if (!(total > cut)) out[acc] = (int32_t)any;
       }
     }
     if (total > cut && !(start > cut) && end > cut) {
