@@ -182,7 +182,7 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
       };
       const int key_a = key_of(0), key_b = key_of(1);
       // The page of a position; -1 behind the prefix.
-      auto page_at = [&](int pos) { return pos < p.prefix ? p.a.kv.table[pos / page_size] : -1; };
+      auto page_at = [&](int pos) { return pos < p.prefix ? p.a.kv.table[p.by_page(pos)] : -1; };
       int seg = step0 / each, kt = (step0 - seg * each) * TPS;
       int g = seg / p.tile_segs;
       bool new_seg = true;
@@ -219,9 +219,9 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
           segs_seen++;
           new_seg = false;
           const int row0 = (seg - g * p.tile_segs) * RT * kTileRows;
-#pragma unroll 4
+#pragma unroll 8
           for (int r = lw * 4 + sub; r < RT * kTileRows; r += 4 * kLoaders) {
-            const int row = row0 + r, tok = row / p.group;
+            const int row = row0 + r, tok = p.by_group(row);
             const bool in = row < rows;
             const T* src = static_cast<const T*>(p.a.q) + (in ? (int64_t)tok * p.a.q_tok + (int64_t)(g * p.group + row - tok * p.group) * p.a.q_head : 0);
 #pragma unroll
@@ -279,7 +279,7 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
             __syncwarp();
             if (lw == h && lane < boxes) {
               const uint32_t dst = (h ? v_s : k_s) + lane * box * 128;
-              const int slot = box_pos % page_size;
+              const int slot = box_pos - p.by_page(box_pos) * page_size;
 #pragma unroll
               for (int c = 0; c < DP / 64; c++) tc5::tma_4d(dst + c * KT * 128, h ? &tmv : &tmk, 64 * c, slot, this_g, this_page, full);
             }
@@ -295,7 +295,7 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
               if (p.a.status) atomicOr(p.a.status, SERVE_BAD_INDEX);
               return false;
             }
-            const int64_t slot = pos % page_size;
+            const int64_t slot = pos - p.by_page(pos) * page_size;
             ko = page * p.a.kv.k_page + slot * p.a.kv.k_slot + this_g * p.a.kv.k_head;
             vo = page * p.a.kv.v_page + slot * p.a.kv.v_slot + this_g * p.a.kv.v_head;
             return true;
