@@ -247,19 +247,19 @@ int part_warps(int dp) { return dp == 64 ? Part<__half, 64>::WARPS : dp == 128 ?
 // keys and 256 rows, 64 keys and 128 rows at head_dim 256; a part's tile 32 keys, 16 there.
 Costs costs(int dp) {
   Costs c;
-  c.tile = dp == 64 ? 315 : dp == 128 ? 560 : 660;
+  c.tile = dp == 64 ? 315 : dp == 128 ? 540 : 660;
   c.segment = 300;
-  c.begin = 27000;  // until the last of the parts is done: a warp by itself is slow
+  c.begin = 25000;  // until the last of the parts is done: a warp by itself is slow
   c.step = dp == 64 ? 4000 : dp == 128 ? 4900 : 3050;
-  c.tile_segment = 20000;
+  c.tile_segment = 10000;
   c.tile_bytes = (dp == 256 ? 16 : 32) * dp * 4;
   return c;
 }
 
 // How the prefix goes to the tensor cores' own tiles, and where: more rows than the 16 that one read of
 // a key serves in the part kernel, and work enough that they end sooner than parts would, by the same costs
-// (parts and tiles, 8 kv heads of 4 rows a token: 64 tokens behind 500 keys 22 and 29 us, 30 behind 1000 23 and
-// 25, behind 2000 28 and 28, 64 behind 2000 40 and 32, 40 behind 6000 54 and 32).
+// (parts and tiles, 8 kv heads of 4 rows a token: 64 tokens behind 500 keys 22 and 26 us, 30 behind 1000 23 and
+// 23, behind 2000 28 and 29, 64 behind 1000 29 and 26, behind 2000 40 and 27, 40 behind 6000 53 and 27).
 struct TileCut {
   bool on;
   int keys, rt, streams, segs, each;  // keys of a tile; see AttnParams
@@ -279,7 +279,7 @@ TileCut tile_cut(const vtq_attention_args& a) {
   if (rows <= kRows || !prefix) return c;
   const Costs cost = costs(padded_dim(a.kv.head_dim));
   const int64_t sms = num_sms(), share = (c.total + sms - 1) / sms, key_tiles = (prefix + (wide ? 15 : 31)) / (wide ? 16 : 32);
-  const int64_t parts = (rows + kRows - 1) / kRows * a.kv.kv_heads * key_tiles * cost.tile / sms + cost.begin / 2;
+  const int64_t parts = (rows + kRows - 1) / kRows * a.kv.kv_heads * key_tiles * cost.tile / sms + cost.begin / 5;
   c.on = share * cost.step + ((share + c.each - 1) / c.each) * cost.tile_segment < parts;
   return c;
 }

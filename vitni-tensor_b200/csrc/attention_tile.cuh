@@ -5,7 +5,8 @@
 // the odd key tiles of one block (two parts of the same rows, joined later), so that a stream's softmax
 // runs beside the other's products. (S twice for each stream, with tiles of 64 keys for TMEM's sake, is
 // slower: an MMA of 64 columns takes as long as one of 128, 5600 cycles a 256 x 128 step.)
-//   softmax warpgroups  a thread a row: S from TMEM, the weights back into TMEM as the second product's A
+//   softmax warpgroups  the query rows of a segment; then a thread a row: S from TMEM, the weights back into
+//                       TMEM as the second product's A
 //   2 loader warps      pages into a ring of swizzled K and V tiles, by TMA where a page holds 4 positions
 //                       or more (gathering rows with 16-byte copies took three warps 5700 cycles a tile)
 //   a warp a stream     one thread issues S = Q K^T (N = KT keys) and O += P V (V as it lies: N-major)
@@ -131,7 +132,7 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
       tc5::bar_init(PV_DONE(r), 1);
       tc5::bar_init(TURN(r), 128);
     }
-    tc5::bar_init(Q_FULL, 32 * kLoaders);
+    tc5::bar_init(Q_FULL, 128 * STREAMS);
     tc5::bar_init(Q_EMPTY, STREAMS);
     for (int i = 0; i < kMasks; i++) tc5::bar_init(MASK(i), kLoaders);
     *abort_flag = 0;
@@ -185,8 +186,6 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
       auto page_at = [&](int pos) { return pos < p.prefix ? p.a.kv.table[p.by_page(pos)] : -1; };
       int seg = step0 / each, kt = (step0 - seg * each) * TPS;
       int g = seg / p.tile_segs;
-      bool new_seg = true;
-      int segs_seen = 0;
       const int tiles = steps * TPS;
       bool ok = true;
       // Waits until ring place n may be filled; meanwhile tells of whatever has landed.
@@ -205,42 +204,6 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
       // The page of this lane's box of the next tile, read a tile ahead.
       int box_page = lane < boxes && steps ? page_at(kt * KT + lane * box) : -1;
       for (int n = 0; n < tiles && ok && !*abort_flag; n++) {
-        const bool with_q = new_seg;
-        if (new_seg) {
-          if (segs_seen) {
-            // The products with the Q before need every tile so far.
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            tell(2 * n);
-            if (!tc5::bar_wait(Q_EMPTY, tc5::phase(segs_seen - 1, 1))) {
-              ok = false;
-              break;
-            }
-          }
-          segs_seen++;
-          new_seg = false;
-          const int row0 = (seg - g * p.tile_segs) * RT * kTileRows;
-#pragma unroll 8
-          for (int r = lw * 4 + sub; r < RT * kTileRows; r += 4 * kLoaders) {
-            const int row = row0 + r, tok = p.by_group(row);
-            const bool in = row < rows;
-            const T* src = static_cast<const T*>(p.a.q) + (in ? (int64_t)tok * p.a.q_tok + (int64_t)(g * p.group + row - tok * p.group) * p.a.q_head : 0);
-#pragma unroll
-            for (int c = 0; c < DP / 64; c++) {
-              const int chunk = c * 8 + (lane & 7);
-              const bool there = in && chunk * 8 < D;
-              const uint32_t at = (r / kTileRows) * L::Q_TILE + place(kTileRows, r % kTileRows, chunk);
-              if (p.q_copies) {
-                copy16(base + at, src + (there ? chunk * 8 : 0), there);
-              } else {
-                T* dst = reinterpret_cast<T*>(gbase + at);
-#pragma unroll
-                for (int e = 0; e < 8; e++) dst[e] = there ? src[chunk * 8 + e] : from_f32<T>(0.0f);
-              }
-            }
-          }
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          __syncwarp();
-        }
         const uint32_t k_s = ring + (2 * n % NSLOT) * L::SLOT, v_s = ring + ((2 * n + 1) % NSLOT) * L::SLOT;
         // A tile that lies whole in pages that exist comes by TMA, a box for each page (or piece of one):
         // every loader warp sees the same pages and takes the same way. The prefix's last tile, one with a
@@ -251,7 +214,6 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
         const int this_kt = kt, this_g = g, this_page = box_page;
         if (++kt == each * TPS) {
           kt = 0;
-          new_seg = true;
           if (++seg, seg % p.tile_segs == 0) g++;
         }
         if (lane < boxes && n + 1 < tiles) box_page = page_at(kt * KT + lane * box);
@@ -335,12 +297,6 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
           asm volatile("cp.async.wait_group 2;" ::: "memory");
           if (told < 2 * n) tell(2 * n);
         }
-        if (with_q) {
-          if (by_box) asm volatile("cp.async.wait_group 0;" ::: "memory");
-          else asm volatile("cp.async.wait_group 2;" ::: "memory");
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          tc5::bar_arrive(Q_FULL);
-        }
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       if (ok && !*abort_flag) tell(2 * tiles);
@@ -419,6 +375,47 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, so = tmem + lanes + kColO + r * DP;
     float m = -INFINITY, l = 0.0f;  // m: what the weights are relative to
     int used = 0;                   // tiles that this stream has had
+    int had = 0;                    // segments that this CTA is done with
+    // The query rows of a segment, by all softmax warps, 8 lanes a row of 128 bytes: the first ones while the first
+    // keys are on their way (5.8 us where the two loaders brought them), the next ones behind a segment's last weights.
+    auto ask_q = [&](int s) {
+      const int g = s / p.tile_segs, row0 = (s - g * p.tile_segs) * RT * kTileRows;
+#pragma unroll 4
+      for (int i = warp * 4 + (lane >> 3); i < RT * kTileRows; i += 16 * STREAMS) {
+        const int q = row0 + i, tok = p.by_group(q);
+        const bool in = q < rows;
+        const T* src = static_cast<const T*>(p.a.q) + (in ? (int64_t)tok * p.a.q_tok + (int64_t)(g * p.group + q - tok * p.group) * p.a.q_head : 0);
+#pragma unroll
+        for (int c = 0; c < DP / 64; c++) {
+          const int chunk = c * 8 + (lane & 7);
+          const bool there = in && chunk * 8 < D;
+          const uint32_t at = (i / kTileRows) * L::Q_TILE + place(kTileRows, i % kTileRows, chunk);
+          if (p.q_copies) {
+            copy16(base + at, src + (there ? chunk * 8 : 0), there);
+          } else {
+            T* dst = reinterpret_cast<T*>(gbase + at);
+#pragma unroll
+            for (int e = 0; e < 8; e++) dst[e] = there ? src[chunk * 8 + e] : from_f32<T>(0.0f);
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto tell_q = [&]() {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc5::bar_arrive(Q_FULL);
+    };
+    // Every product with this segment's queries is done: the next segment's may take their place.
+    auto next_q = [&](int s) {
+      if (!tc5::bar_wait(Q_EMPTY, tc5::phase(had++, 1))) return false;
+      ask_q(s);
+      return true;
+    };
+    if (steps) {
+      ask_q(step0 / each);
+      tell_q();
+    }
     int seg = step0 / each, in = step0 - seg * each;
     for (int i = 0; i < steps; i++) {
       const bool start = i == 0 || in == 0, last = i + 1 == steps || in + 1 == each;
@@ -435,6 +432,13 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
           break;
         }
         if (STREAMS == 2) tc5::bar_arrive(TURN(1 - r));
+        if (last && i + 1 < steps) {
+          if (!next_q(this_seg + 1)) {
+            if (lane == 0) fail();
+            break;
+          }
+          tell_q();
+        }
         continue;
       }
       const int n = i * TPS + (TPS == 2 ? r : 0);
@@ -564,7 +568,7 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
       l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
       used++;
       if (last) {
-        if (!tc5::bar_wait(PV_DONE(r), (used - 1) & 1)) {
+        if ((i + 1 < steps && !next_q(this_seg + 1)) || !tc5::bar_wait(PV_DONE(r), (used - 1) & 1)) {
           if (lane == 0) fail();
           break;
         }
@@ -592,8 +596,10 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
           }
         }
         tc5::fence_before();
+        if (i + 1 < steps) tell_q();
       }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
   tc5::fence_before();
   __syncthreads();
