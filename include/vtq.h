@@ -316,7 +316,8 @@ vtq_status vtq_gather_destroy(vtq_gather* g);
  * checked on the host before anything is launched; a failed call's message is
  * vtq_device_last_error(). Lengths, tables and token ids live on the device:
  * kernels check them against the sizes given and skip what lies outside,
- * OR-ing 2 into the optional status word. Strides are in elements; the last
+ * OR-ing 2 into the optional status word (1: a bounded wait ran out, so that
+ * results are missing). Strides are in elements; the last
  * dimension of every tensor is contiguous. */
 /* Message of this thread's last failed call of this section ("" if none). */
 const char* vtq_device_last_error(void);
@@ -410,7 +411,9 @@ vtq_status vtq_append_kv(const vtq_append_kv_args* args, void* stream);
  * zeros) or 2 (lse: -inf); what cached positions at or behind
  * kv_len hold has no effect, whatever it is.
  * Keys behind the table's width, and pages that do not exist, count as unseen
- * and set the status word; row starts that decrease leave no sequence a row.
+ * and set the status word (2); row starts that decrease leave no sequence a row.
+ * Where a bounded wait ran out (1 in the status word) the rows that it left
+ * without some of their keys are NaN.
  * At most 1024 sequences a call. ws: vtq_attention_paged_workspace_bytes. */
 typedef struct vtq_attention_args {
   vtq_paged_kv kv;

@@ -88,7 +88,8 @@ __global__ void __launch_bounds__(attention_threads<T, DP, RT>(), 1)
       return;
     }
   }
-  part_role<T, DP, P::KT, P::WARPS, RT == 0>(p, tmk, tmv, smem, base, cta - x, p.ctas - x);
+  const int lost = part_role<T, DP, P::KT, P::WARPS, RT == 0>(p, tmk, tmv, smem, base, cta - x, p.ctas - x);
+  if (lost >= 0) lost_parts<T, DP, RT == 0>(p, base, lost);
 }
 
 // Adds the parts of each row (query head of a token): p.join_warps warps a row, one where the rows fill the SMs, more
@@ -121,6 +122,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps, DP > 128 ? 2 : 3) attention_j
     // The parts of the row's place among the sequence's own rows, and among all rows for the prefix.
     int count[2] = {0, 0}, rr[2] = {0, 0};
     const float* slot0[2] = {p.part, p.part};
+    bool lost = false;
 #pragma unroll
     for (int k = 0; k < 2; k++) {
       const int seg0 = k ? of.z : of.x;
@@ -131,7 +133,15 @@ __global__ void __launch_bounds__(32 * kJoinWarps, DP > 128 ? 2 : 3) attention_j
       // other keys.
       const int seg = tiles ? g * p.tile_segs + r / (kTileRows * p.tile_rt) : seg0 + r / kRows * H + g;
       int2 w = make_int2(0, 0);
-      if (pass) w = (tiles ? p.seg_ctas : p.seg_parts)[seg];
+      if (pass) {
+        w = (tiles ? p.seg_ctas : p.seg_parts)[seg];
+        // What the kernel before left for every segment, also where a wait of its ran out; nothing else is followed.
+        if (!parts_ok(w, tiles ? min(p.ctas, p.tiles_total) : p.ctas * p.warps)) {
+          if (p.a.status) atomicOr(p.a.status, KERR_TIMEOUT);
+          lost = true;
+          continue;
+        }
+      }
       rr[k] = r % (tiles ? kTileRows : kRows);
       count[k] = (w.y - w.x + 1) * (tiles && p.tile_rt == 1 ? p.tile_streams : 1);
       if (!pass) continue;
@@ -229,6 +239,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps, DP > 128 ? 2 : 3) attention_j
       asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / split), "r"(32 * split) : "memory");
       if (sub) continue;
     }
+    if (lost) l = __uint_as_float(0x7fc00000u);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: zeros
     T* out = static_cast<T*>(p.a.out) + token * p.a.o_tok + head * p.a.o_head;
 #pragma unroll

@@ -20,7 +20,14 @@ constexpr int kBytesPerCycle = 3500;  // from HBM, of all SMs
 struct Divisor {
   uint32_t mul;
   int shift;
-  __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi(mul, (uint32_t)n) + (uint32_t)n) >> shift); }
+  __host__ __device__ __forceinline__ int operator()(int n) const {
+#ifdef __CUDA_ARCH__
+    const uint32_t high = __umulhi(mul, (uint32_t)n);
+#else
+    const uint32_t high = (uint32_t)((uint64_t)mul * (uint32_t)n >> 32);
+#endif
+    return (int)((high + (uint32_t)n) >> shift);
+  }
 };
 inline Divisor divisor(int64_t d) {
   int s = 0;
@@ -73,16 +80,16 @@ struct Plan {
 };
 __host__ __device__ inline int plan_ints(int B) { return 4 * (B + 2) + 4; }
 
-__device__ __forceinline__ Plan plan_of(int* base, int B) {
+__host__ __device__ __forceinline__ Plan plan_of(int* base, int B) {
   return Plan{base + 4, base + 4 + (B + 2), base + 4 + 2 * (B + 2), base + 4 + 3 * (B + 2)};
 }
 
-__device__ __forceinline__ int seq_rows(const Plan& pl, int b) { return pl.q0[b + 1] - pl.q0[b]; }
+__host__ __device__ __forceinline__ int seq_rows(const Plan& pl, int b) { return pl.q0[b + 1] - pl.q0[b]; }
 
 // Whether every row of a sequence sees the whole prefix. The rows of one that does not (it ends inside
 // the prefix, or is empty) take no part in the prefix's segments: it has all its keys for its own, so
 // that those segments need no mask for rows, and what they hold cannot reach a row that must not see it.
-__device__ __forceinline__ bool sees_prefix(const AttnParams& p, const Plan& pl, int b) {
+__host__ __device__ __forceinline__ bool sees_prefix(const AttnParams& p, const Plan& pl, int b) {
   const int n = seq_rows(pl, b);
   return n > 0 && pl.len[b] - n + 1 >= p.prefix;
 }
@@ -91,7 +98,7 @@ __device__ __forceinline__ bool sees_prefix(const AttnParams& p, const Plan& pl,
 struct Entry {
   int rows, keys;
 };
-__device__ __forceinline__ Entry entry_of(const AttnParams& p, const Plan& pl, int b, int B) {
+__host__ __device__ __forceinline__ Entry entry_of(const AttnParams& p, const Plan& pl, int b, int B) {
   Entry e;
   if (b < B) {
     e.rows = seq_rows(pl, b) * p.group;
@@ -103,8 +110,8 @@ __device__ __forceinline__ Entry entry_of(const AttnParams& p, const Plan& pl, i
   }
   return e;
 }
-__device__ __forceinline__ int blocks_of(const Entry& e) { return (e.rows + kRows - 1) / kRows; }
-__device__ __forceinline__ int tiles_of(const AttnParams& p, const Entry& e) { return (e.keys + p.tile - 1) >> p.tile_shift; }
+__host__ __device__ __forceinline__ int blocks_of(const Entry& e) { return (e.rows + kRows - 1) / kRows; }
+__host__ __device__ __forceinline__ int tiles_of(const AttnParams& p, const Entry& e) { return (e.keys + p.tile - 1) >> p.tile_shift; }
 
 // Built by all threads of a CTA in its shared memory; base[0] = the parts' tiles in all, base[1] = parts in
 // use, base[2] = CTAs that work on the prefix's own tiles (the first ones), by the two sides' cost.
@@ -189,7 +196,7 @@ __device__ void build_plan(const AttnParams& p, int* base) {
 }
 
 // Part w of W covers tiles [first(w), first(w + 1)) of `total`.
-__device__ __forceinline__ int first_tile(int total, int W, int w) { return (int)((int64_t)total * w / W); }
+__host__ __device__ __forceinline__ int first_tile(int total, int W, int w) { return (int)((int64_t)total * w / W); }
 
 // Where a part stands: sequence, row block, head, tile. Tiles lie on multiples of their size, so that pages
 // and boxes do not straddle them: the first one of a sequence behind the prefix may begin inside it.
@@ -199,7 +206,7 @@ struct __align__(16) Cursor {
   int lo, end;          // of b: its keys; the first tile lies at lo, rounded down
 };
 
-__device__ __forceinline__ void enter(const AttnParams& p, const Plan& pl, int B, Cursor& c) {
+__host__ __device__ __forceinline__ void enter(const AttnParams& p, const Plan& pl, int B, Cursor& c) {
   const Entry e = entry_of(p, pl, c.b, B);
   c.mbs = blocks_of(e);
   c.nt = c.mbs ? tiles_of(p, e) : 0;
@@ -207,7 +214,8 @@ __device__ __forceinline__ void enter(const AttnParams& p, const Plan& pl, int B
   c.end = c.b < B ? min(pl.len[c.b], p.keys_max) : pl.len[B];
 }
 
-__device__ Cursor seek(const AttnParams& p, const Plan& pl, int B, int tile) {
+// (Not inlined: one call a part, and its registers would cost the parts' loop spills.)
+__host__ __device__ __noinline__ Cursor seek(const AttnParams& p, const Plan& pl, int B, int tile) {
   int lo = 0, hi = B;  // the last index whose tiles begin at or before `tile`
   while (lo < hi) {
     const int m = (lo + hi + 1) >> 1;
@@ -225,7 +233,7 @@ __device__ Cursor seek(const AttnParams& p, const Plan& pl, int B, int tile) {
 }
 
 // The next tile; t = 0 where it begins another segment. Never called behind the last tile.
-__device__ __forceinline__ void advance(const AttnParams& p, const Plan& pl, int B, Cursor& c) {
+__host__ __device__ __forceinline__ void advance(const AttnParams& p, const Plan& pl, int B, Cursor& c) {
   if (++c.t < c.nt) return;
   c.t = 0;
   if (++c.g == (int)p.a.kv.kv_heads) {
@@ -239,8 +247,23 @@ __device__ __forceinline__ void advance(const AttnParams& p, const Plan& pl, int
   }
 }
 
+// The first and last of a segment's parts, as the joining kernel finds them: whether they are parts of `most`. It
+// follows no others.
+__host__ __device__ inline bool parts_ok(int2 w, int most) { return w.x >= 0 && w.x <= w.y && w.y < most; }
+
+// The part of a segment that a part of the work, tiles [tile0, tile1), takes: of the segment that `c` stands in, at
+// `tile`. Whether it takes the segment's first and last tile, and the tile behind what it takes.
+struct Share {
+  bool first, last;
+  int end;
+};
+__host__ __device__ inline Share share_of(const Cursor& c, int tile, int tile0, int tile1) {
+  const int start = tile - c.t, stop = start + c.nt;
+  return Share{start >= tile0, stop <= tile1, stop < tile1 ? stop : tile1};
+}
+
 // The sequence that owns a row of q, or -1.
-__device__ __forceinline__ int owner(const Plan& pl, int B, int token) {
+__host__ __device__ __forceinline__ int owner(const Plan& pl, int B, int token) {
   int lo = 0, hi = B - 1;
   while (lo < hi) {
     const int m = (lo + hi + 1) >> 1;

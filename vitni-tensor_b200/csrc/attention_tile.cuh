@@ -416,8 +416,8 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
       ask_q(step0 / each);
       tell_q();
     }
-    int seg = step0 / each, in = step0 - seg * each;
-    for (int i = 0; i < steps; i++) {
+    int seg = step0 / each, in = step0 - seg * each, i = 0;
+    for (; i < steps; i++) {
       const bool start = i == 0 || in == 0, last = i + 1 == steps || in + 1 == each;
       const int this_seg = seg;
       if (++in == each) in = 0, seg++;
@@ -600,6 +600,19 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
       }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    // A wait ran out: the segments that this warp's rows have not left yet become NaN (their sums of weights are), so
+    // that the joining kernel finds an entry and a slot for each of them, and rows that lack keys show it.
+    if (i < steps) {
+      for (int s = (step0 + i) / each; s <= (step0 + steps - 1) / each; s++) {
+        if (tid == 0) {
+          if (s * each >= step0) p.seg_ctas[s].x = cta;
+          if ((s + 1) * each <= step0 + steps) p.seg_ctas[s].y = cta;
+        }
+        if (((s % p.tile_segs) * RT + (RT == 2 ? r : 0)) * kTileRows + row < rows)
+          *reinterpret_cast<float2*>(p.tile_part + (int64_t)((cta + s) * STREAMS + r) * (kTileRows * (DP + 2)) + 2 * row) =
+              make_float2(0.0f, __uint_as_float(0x7fc00000u));
+      }
+    }
   }
   tc5::fence_before();
   __syncthreads();
