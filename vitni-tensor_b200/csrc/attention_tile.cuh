@@ -614,6 +614,7 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
       }
     }
   }
+  if (*abort_flag) tc5::settle();
   tc5::fence_before();
   __syncthreads();
   if (warp == kMmaWarp) {

@@ -294,6 +294,7 @@ __global__ void __launch_bounds__(kThreads)
     }
     tc5::fence_before();
   }
+  if (*abort_flag) tc5::settle();
   __syncthreads();
   if (warp == 1) {
     tc5::fence_after();
@@ -508,6 +509,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
       if (lane == 0) arrive_remote(in_leader(ACC_EMPTY(acc)));
     }
   }
+  if (*abort_flag) tc5::settle();
   tc5::fence_before();
   cl.sync();  // the leader's products read the peer's operands and write its accumulators
   if (warp == 1) {

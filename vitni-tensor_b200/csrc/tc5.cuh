@@ -1,5 +1,5 @@
 // tc5.cuh -- tcgen05 (UMMA), TMA and mbarrier helpers of the batched serving kernels, inline PTX.
-// Every wait is bounded (vtq_device.cuh).
+// Every wait is bounded, and a kernel that gave up on one settles before it returns.
 #pragma once
 #include <cuda.h>
 
@@ -52,6 +52,14 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
   while (!bar_try(bar, parity))
     if (clock64() - t0 > (1ll << 32)) return false;
   return true;
+}
+// Before a kernel that gave up on a wait returns its shared memory and TMEM: copies and products that are still on
+// their way (those asked for while the wait ran, by warps that had not seen it run out) take some us to land and
+// get 2^24 cycles, about 10 ms.
+__device__ inline void settle() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < (1ll << 24)) {
+  }
 }
 
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* tm, int x, int y, uint32_t bar) {
