@@ -252,7 +252,8 @@ vtq_status serve_check_kv(const char* fn, const vtq_paged_kv& kv) {
   if (kv.head_dim % 8 || kv.head_dim > 256 || kv.kv_heads > 4096)
     return serve_fail(VTQ_ERR_NOT_IMPLEMENTED,
                       "%s: not implemented (head_dim not a multiple of 8 up to 256, or over 4096 heads)", fn);
-  if (kv.pages && (!kv.k || !kv.v || (!kv.table && kv.seqs * kv.table_width)))
+  // (The table is read before a page's number is compared with how many there are.)
+  if ((kv.pages && (!kv.k || !kv.v)) || (!kv.table && kv.seqs && kv.table_width))
     return serve_fail(VTQ_ERR_INVALID_ARG, "%s: null cache pointer", fn);
   if (!aligned16(kv.k) || !aligned16(kv.v) || kv.k_page % 8 || kv.k_slot % 8 || kv.k_head % 8 ||
       kv.v_page % 8 || kv.v_slot % 8 || kv.v_head % 8)
