@@ -327,7 +327,7 @@ vtq_status check(const char* fn, const vtq_attention_args* a) {
     return serve_fail(VTQ_ERR_INTERNAL, "%s: bad shape (heads not a multiple of kv_heads, or a negative size)", fn);
   if (a->kv.seqs > kMaxSeqs)
     return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "%s: not implemented (over %d sequences in one call)", fn, kMaxSeqs);
-  if (a->tokens > (1 << 20) || a->heads > 65536 || a->tokens * a->heads > INT32_MAX / 2 || a->kv.table_width * a->kv.page_size > INT32_MAX / 2)
+  if (a->tokens > (1 << 20) || a->heads > 65536 || a->tokens * a->heads > INT32_MAX / 2 || a->kv.table_width > INT32_MAX / 2 / a->kv.page_size)
     return serve_fail(VTQ_ERR_NOT_IMPLEMENTED, "%s: not implemented (over 2^20 tokens, 2^16 heads or 2^30 positions)", fn);
   const int64_t tiles = (a->kv.table_width * a->kv.page_size + 15) / 16 + 1;
   if (most_segments(*a) * tiles > INT32_MAX || tile_cut(*a).total > INT32_MAX)
