@@ -335,7 +335,8 @@ vtq_status vtq_quantize_tokens(int32_t x_dtype, const void* x, int64_t ldx, int6
  * quantised on the way as by vtq_quantize_tokens (x_scale NULL), or VTQ_I8 with
  * its x_scale. w is [out_feat][ldw] signed bytes, 16-byte aligned, ldw a
  * multiple of 16; what lies behind in_feat in a row is not used. bias may be
- * NULL. in_feat <= 131072 (the integer sums cannot overflow below that).
+ * NULL. in_feat <= 131072: the largest sum, 131072 times -128 times -128, is 2^31,
+ * and any other fits 32 signed bits.
  * ws: vtq_linear_i8_workspace_bytes; 0 bytes need no ws. */
 typedef struct vtq_linear_i8_args {
   const void* x;

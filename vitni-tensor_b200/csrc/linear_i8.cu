@@ -175,9 +175,13 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint3
       "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one));
 }
 
+// A sum as a float. Only 131072 products of -128 and -128 leave the range of 32 bits: their sum, 2^31, is held as the
+// lowest value, one that no other sum has (the lowest of those is 131072 x 127 x -128).
+__device__ __forceinline__ float sum_f32(int acc) { return acc == INT32_MIN ? 2147483648.0f : __int2float_rn(acc); }
+
 template <typename Y>
 __device__ __forceinline__ void store_y(const I8Params& p, int t, int o, int acc, float wsc, float b) {
-  float v = __int2float_rn(acc) * (p.xs[t] * wsc);
+  float v = sum_f32(acc) * (p.xs[t] * wsc);
   if (p.bias) v += b;
   static_cast<Y*>(p.y)[(int64_t)t * p.ldy + o] = from_f32<Y>(v);
 }
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(kThreads)
       for (int h = 0; h < 2; h++) {
         const int c = c0 + h * splits * (kThreads / 32);
         if (c >= last || *abort_flag) continue;
-        int acc[4] = {0, 0, 0, 0};
+        uint32_t acc[4] = {0, 0, 0, 0};  // modulo 2^32, as the tensor cores add
 #pragma unroll
         for (int s = 0; s < 8; s++)
           if (s < splits) acc[0] += v[h][s].x, acc[1] += v[h][s].y, acc[2] += v[h][s].z, acc[3] += v[h][s].w;
@@ -333,7 +337,7 @@ __global__ void __launch_bounds__(kThreads)
         Y* y = static_cast<Y*>(p.y) + (int64_t)(t0 + c) * p.ldy + o;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          float r = __int2float_rn(acc[i]) * (xs * wsc[i]);
+          float r = sum_f32((int)acc[i]) * (xs * wsc[i]);
           if (p.bias) r += b[i];
           if (o + i < p.N) y[i] = from_f32<Y>(r);
         }
@@ -498,7 +502,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
         if (o < p.N) {
 #pragma unroll
           for (int i = 0; i < 32; i++) {
-            float v = __int2float_rn((int)r[i]) * (xs[i] * wsc);
+            float v = sum_f32((int)r[i]) * (xs[i] * wsc);
             if (p.bias) v += b;
             if (all || t0 + c + i < p.T) y[(int64_t)(c + i) * p.ldy] = from_f32<Y>(v);
           }
