@@ -3,6 +3,9 @@ the largest sums, weights far below a row's largest, scales of zero, outputs tha
 import pytest
 import torch
 
+from tests.test_gpu_serving import BF16, attention_case, gen
+from vtq import Internal
+
 pytestmark = pytest.mark.gpu
 
 
@@ -27,3 +30,33 @@ def test_linear_i8_the_largest_sum(S, t, n):
     q[:, 77] = 0
     y = S.linear_i8(q, W, x_scale=torch.ones(t, device="cuda"))
     assert torch.equal(y, ((code[:, None] * weight).double() * (k - 1)).float())
+
+
+def attention_inputs(tokens=6):
+    lens = [20 + 3 * i for i in range(tokens)]
+    return attention_case(gen(5), [1] * tokens, lens, 4, 2, 64, 8, 0, BF16, False)
+
+
+def test_attention_out_beside_and_over_slices_of_queries(S):
+    """q and out as slices of one tensor: side by side they are taken, one over the other is refused."""
+    q, kp, vp, table, kv_len, _ = attention_inputs()
+    t, want = len(q), S.attention_paged(q, kp, vp, table, kv_len)
+    by_head = torch.zeros(t, 12, 64, dtype=BF16, device="cuda")
+    by_value = torch.zeros(t, 4, 256, dtype=BF16, device="cuda")
+    by_token = torch.zeros(4, 3 * t, 64, dtype=BF16, device="cuda").transpose(0, 1)
+    every_other = torch.zeros(2 * t, 4, 64, dtype=BF16, device="cuda")
+    sliced = {
+        "heads": (by_head[:, 1:5], [by_head[:, 5:9], by_head[:, 8:12]], [by_head[:, 0:4], by_head[:, 2:6], by_head[:, 4:8]]),
+        "values": (by_value[..., 8:72], [by_value[..., 72:136], by_value[..., 192:]], [by_value[..., :64], by_value[..., 40:104], by_value[..., 64:128]]),
+        "tokens": (by_token[2:t + 2], [by_token[t + 2:2 * t + 2]], [by_token[:t], by_token[t + 1:2 * t + 1]]),
+        "every other token": (every_other[::2], [every_other[1::2]], [every_other[:t], every_other[t:]]),
+    }
+    for name, (x, beside, over) in sliced.items():
+        x.copy_(q)
+        for out in beside:
+            S.attention_paged(x, kp, vp, table, kv_len, out=out)
+            assert torch.equal(out, want) and torch.equal(x, q), name
+        for out in over:
+            with pytest.raises(Internal, match="shares memory"):
+                S.attention_paged(x, kp, vp, table, kv_len, out=out)
+            assert torch.equal(x, q), name

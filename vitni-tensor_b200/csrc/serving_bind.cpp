@@ -5,13 +5,13 @@
 // Errors are C++ exceptions inside and Python exceptions (the package's classes, by status) at the border.
 #include <Python.h>
 
-#include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/full.h>
 #include <ATen/ops/zeros.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/util/SmallVector.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -20,6 +20,7 @@
 #include <limits>
 #include <sstream>
 #include <string>
+#include <utility>
 
 #include "../../include/vtq.h"
 
@@ -72,6 +73,42 @@ const at::Tensor& want(const char* name, PyObject* o, int64_t dim, Types types, 
   return t;
 }
 
+// Where a tensor's elements lie, in bytes; dimensions of one element left out.
+struct Span {
+  uintptr_t base;
+  int64_t elt, extent;  // extent: from the first element's first byte to the last one's end
+  c10::SmallVector<std::pair<int64_t, int64_t>, 6> dims;  // (step, size)
+  explicit Span(const at::Tensor& t) : base(reinterpret_cast<uintptr_t>(t.data_ptr())), elt((int64_t)t.element_size()), extent(elt) {
+    for (int64_t i = 0; i < t.dim(); i++)
+      if (t.size(i) > 1) {
+        dims.emplace_back(t.stride(i) * elt, t.size(i));
+        extent += (t.size(i) - 1) * t.stride(i) * elt;
+      }
+  }
+  // The bytes that its elements reach over when those of all steps that are multiples of `period` are laid upon another.
+  int64_t within(int64_t period) const {
+    int64_t n = elt;
+    for (const auto& [step, size] : dims)
+      if (step % period) n += (size - 1) * step;
+    return n;
+  }
+};
+
+// Whether two tensors may have memory in common: no where one ends before the other begins, and no where they are
+// slices of one layout, that is, for some step of theirs, lie in different places of each period of that step (the
+// heads, values or tokens of one fused tensor).
+bool may_share(const Span& a, const Span& b) {
+  if (a.base + a.extent <= b.base || b.base + b.extent <= a.base) return false;
+  for (const Span* s : {&a, &b})
+    for (const auto& dim : s->dims) {
+      const int64_t period = dim.first;
+      if (period <= 0) continue;
+      const int64_t wa = a.within(period), wb = b.within(period), d = (int64_t)(b.base - a.base) % period, at = d < 0 ? d + period : d;
+      if (wa <= at && at + wb <= period) return false;
+    }
+  return true;
+}
+
 // An output: its elements must not share memory (expanded tensors).
 const at::Tensor& distinct(const char* name, const at::Tensor& t) {
   for (int64_t i = 0; i < t.dim(); i++)
@@ -82,11 +119,9 @@ const at::Tensor& distinct(const char* name, const at::Tensor& t) {
 // An output that is written while `in` is still being read; `same`: unless it is all of it, element for element.
 void apart(const char* name, const at::Tensor& t, const char* in_name, const at::Tensor& in, bool same = false) {
   if (!t.numel() || !in.numel()) return;
-  const bool one = t.data_ptr() == in.data_ptr() && t.strides() == in.strides() && t.scalar_type() == in.scalar_type();
-  if (one && same) return;
-  const at::MemOverlapStatus s = at::get_overlap_status(t, in);
-  if (t.data_ptr() == in.data_ptr() || s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial)
-    refuse(VTQ_ERR_INTERNAL, name, ": shares memory with ", in_name);
+  const Span a(t), b(in);
+  if (same && a.base == b.base && a.dims == b.dims && t.scalar_type() == in.scalar_type()) return;
+  if (may_share(a, b)) refuse(VTQ_ERR_INTERNAL, name, ": shares memory with ", in_name);
 }
 
 void* ptr(const at::Tensor& t) { return t.data_ptr(); }
