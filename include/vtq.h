@@ -378,7 +378,7 @@ typedef struct vtq_paged_kv {
  * (a cos - b sin, a sin + b cos), in 32 bits, rounded once to the cache's type.
  * With q (x's type, [tokens][heads][head_dim]) the queries are rotated alike
  * into q_out, in the cache's type (not over q itself unless the types and
- * strides are the same). Two tokens of one call at the same sequence and
+ * strides are the same, and not over k or v). Two tokens of one call at the same sequence and
  * position: which one stays is not defined. */
 #define VTQ_ROPE_HALF 1u
 typedef struct vtq_append_kv_args {

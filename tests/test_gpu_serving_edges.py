@@ -3,7 +3,7 @@ the largest sums, weights far below a row's largest, scales of zero, outputs tha
 import pytest
 import torch
 
-from tests.test_gpu_serving import BF16, attention_case, gen
+from tests.test_gpu_serving import BF16, F32, attention_case, gen
 from vtq import Internal
 
 pytestmark = pytest.mark.gpu
@@ -60,3 +60,57 @@ def test_attention_out_beside_and_over_slices_of_queries(S):
             with pytest.raises(Internal, match="shares memory"):
                 S.attention_paged(x, kp, vp, table, kv_len, out=out)
             assert torch.equal(x, q), name
+
+
+def test_append_q_out_beside_and_over_k_and_v(S):
+    """Slices of one fused projection: q_out may be q or lie beside everything, but not over k or v."""
+    t, heads, kv, dim = 9, 4, 2, 64
+    fused = torch.randn(t, 2 * heads + 2 * kv, dim, generator=gen(3), device="cuda").to(BF16)
+    kp, vp = (torch.zeros(2, 16, kv, dim, dtype=BF16, device="cuda") for _ in range(2))
+    table = torch.arange(2, dtype=torch.int32, device="cuda")[None]
+    seq, pos = torch.zeros(t, dtype=torch.int32, device="cuda"), torch.arange(t, dtype=torch.int32, device="cuda")
+    rope = S.Rope(dim, 64, layout="half")
+    q, k, v, spare = fused[:, :heads], fused[:, heads:heads + kv], fused[:, heads + kv:heads + 2 * kv], fused[:, heads + 2 * kv:]
+    want = S.append_kv(k, v, kp, vp, table, seq, pos, rope=rope, q=q)
+    S.append_kv(k, v, kp, vp, table, seq, pos, rope=rope, q=q, q_out=spare)
+    assert torch.equal(spare, want)
+    before = fused.clone()
+    for first in (1, heads, heads + 1, heads + kv, heads + 2 * kv - 1):
+        with pytest.raises(Internal, match="shares memory"):
+            S.append_kv(k, v, kp, vp, table, seq, pos, rope=rope, q=q, q_out=fused[:, first:first + heads])
+    with pytest.raises(Internal, match="shares memory"):
+        S.append_kv(k, v, kp, vp, table, seq, pos, rope=rope, q=q.contiguous(), q_out=fused[:, heads:2 * heads])
+    assert torch.equal(fused, before)
+    S.append_kv(k, v, kp, vp, table, seq, pos, rope=rope, q=q, q_out=q)
+    assert torch.equal(q, want)
+    one = fused[:1]  # one token: its stride over tokens says nothing
+    S.append_kv(one[:, heads:heads + kv], one[:, heads + kv:heads + 2 * kv], kp, vp, table, seq[:1], pos[:1], q=one[:, :heads],
+                q_out=fused.view(1, -1, dim)[:, :heads])
+    with pytest.raises(Internal, match="shares memory"):
+        S.append_kv(k, v, kp, kp, table, seq, pos)
+
+
+def test_outputs_over_what_is_read_beside_them(S):
+    """Codes over their values, products over their codes, bias or scales, and outputs that overlap themselves."""
+    x = torch.randn(4, 64, generator=gen(4), device="cuda")
+    with pytest.raises(Internal, match="shares memory"):
+        S.quantize_tokens(x, q=x.view(torch.int8)[:, :64])
+    with pytest.raises(Internal, match="shares memory"):
+        S.quantize_tokens(x, scale=x[0, :4])
+    q, s = S.quantize_tokens(x)
+    W = S.I8Weight(torch.ones(16, 64, dtype=torch.int8, device="cuda"), torch.ones(16, device="cuda"))
+    want = S.linear_i8(q, W, x_scale=s)
+    with pytest.raises(Internal, match="shares memory"):
+        S.linear_i8(q, W, x_scale=s, out=q.view(F32))
+    y = torch.zeros(5, 16, device="cuda")
+    with pytest.raises(Internal, match="shares memory"):
+        S.linear_i8(q, W, bias=y[1], x_scale=s, out=y[:4])
+    y[4, :4] = s
+    with pytest.raises(Internal, match="shares memory"):
+        S.linear_i8(q, W, x_scale=y[4, :4], out=y[1:])
+    assert torch.equal(S.linear_i8(q, W, x_scale=y[4, :4], out=y[:4]), want)
+    with pytest.raises(Internal, match="share memory"):
+        S.linear_i8(q, W, x_scale=s, out=y.as_strided((4, 16), (8, 1)))
+    a, kp, vp, table, kv_len, _ = attention_inputs()
+    with pytest.raises(Internal, match="share memory"):
+        S.attention_paged(a, kp, vp, table, kv_len, out=torch.zeros(6, 400, dtype=BF16, device="cuda").as_strided(a.shape, (64, 64, 1)))

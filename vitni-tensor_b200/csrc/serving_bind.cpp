@@ -15,6 +15,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
 #include <limits>
@@ -109,10 +110,16 @@ bool may_share(const Span& a, const Span& b) {
   return true;
 }
 
-// An output: its elements must not share memory (expanded tensors).
+// An output: its elements must not share memory. Each step has to pass what all smaller ones reach over.
 const at::Tensor& distinct(const char* name, const at::Tensor& t) {
-  for (int64_t i = 0; i < t.dim(); i++)
-    if (t.size(i) > 1 && t.stride(i) == 0) refuse(VTQ_ERR_INTERNAL, name, ": written, but its elements share memory");
+  if (!t.numel()) return t;
+  Span a(t);
+  std::sort(a.dims.begin(), a.dims.end());
+  int64_t reach = a.elt;
+  for (const auto& [step, size] : a.dims) {
+    if (step < reach) refuse(VTQ_ERR_INTERNAL, name, ": written, but its elements share memory");
+    reach += (size - 1) * step;
+  }
   return t;
 }
 
@@ -185,6 +192,9 @@ PyObject* quantize_tokens(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
                                : at::empty({t, std::max<int64_t>(16, (n + 15) / 16 * 16)}, x.options().dtype(at::kChar)).narrow(1, 0, n);
     at::Tensor s = given(a[2]) ? distinct("scale", want("scale", a[2], 1, {ScalarType::Float}, &dev, {t}))
                                : at::empty({t}, x.options().dtype(at::kFloat));
+    if (given(a[1])) apart("q", q, "x", x);
+    if (given(a[2])) apart("scale", s, "x", x);
+    if (given(a[1]) && given(a[2])) apart("scale", s, "q", q);
     const int64_t ldq = t > 1 ? q.stride(0) : std::max(n, q.stride(0));
     check(vtq_quantize_tokens(tag(x.scalar_type()), ptr(x), x.stride(0), t, n, static_cast<int8_t*>(ptr(q)), ldq,
                               static_cast<float*>(ptr(s)), stream_of(dev)));
@@ -218,11 +228,16 @@ PyObject* linear_i8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
       out = at::empty({t, n}, x.options().dtype(type));
     }
     vtq_linear_i8_args g = {};
-    g.x = ptr(x);
-    if (codes) g.x_scale = static_cast<const float*>(ptr(want("x_scale", a[5], 1, {ScalarType::Float}, &dev, {t})));
-    g.w = static_cast<const int8_t*>(ptr(w));
-    g.w_scale = static_cast<const float*>(ptr(ws));
-    if (given(a[3])) g.bias = static_cast<const float*>(ptr(want("bias", a[3], 1, {ScalarType::Float}, &dev, {n})));
+    // (Floating x may be written over: its codes are made before anything of out is.)
+    auto read = [&](const char* name, const at::Tensor& r) {
+      if (given(a[6])) apart("out", out, name, r);
+      return ptr(r);
+    };
+    g.x = codes ? read("x", x) : ptr(x);
+    if (codes) g.x_scale = static_cast<const float*>(read("x_scale", want("x_scale", a[5], 1, {ScalarType::Float}, &dev, {t})));
+    g.w = static_cast<const int8_t*>(read("w", w));
+    g.w_scale = static_cast<const float*>(read("w_scale", ws));
+    if (given(a[3])) g.bias = static_cast<const float*>(read("bias", want("bias", a[3], 1, {ScalarType::Float}, &dev, {n})));
     g.y = ptr(out);
     g.ldx = x.stride(0);
     g.ldw = w.stride(0);
@@ -270,6 +285,7 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const c10::cuda::CUDAGuard guard(dev);
     distinct("k_pages", THPVariable_Unpack(a[2]));
     distinct("v_pages", THPVariable_Unpack(a[3]));
+    apart("v_pages", THPVariable_Unpack(a[3]), "k_pages", THPVariable_Unpack(a[2]));
     const at::Tensor& k = want("k", a[0], 3, kFloats, &dev, {-1, g.kv.kv_heads, g.kv.head_dim});
     const int64_t t = k.size(0);
     const at::Tensor& v = want("v", a[1], 3, {k.scalar_type()}, &dev, {t, g.kv.kv_heads, g.kv.head_dim});
@@ -291,7 +307,11 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
       const ScalarType c = THPVariable_Unpack(a[2]).scalar_type();
       out = given(a[10]) ? distinct("q_out", want("q_out", a[10], 3, {c}, &dev, {t, q.size(1), g.kv.head_dim}))
                          : at::zeros(q.sizes(), q.options().dtype(c));
-      if (given(a[10])) apart("q_out", out, "q", q, true);
+      if (given(a[10])) {
+        apart("q_out", out, "q", q, true);
+        apart("q_out", out, "k", k);
+        apart("q_out", out, "v", v);
+      }
       if (q.size(1) > 0) {
         g.q = ptr(q), g.q_tok = q.stride(0), g.q_head = q.stride(1), g.heads = q.size(1);
         g.q_out = ptr(out), g.qo_tok = out.stride(0), g.qo_head = out.stride(1);

@@ -15,9 +15,11 @@ graph, allocates its outputs and scratch through torch (so a graph keeps its own
 the device. Arguments are checked on the host and refused with the package's errors (``Internal`` for
 shapes and layouts, ``NotImplementedOp`` for types and sizes the kernels do not take, ``InvalidArg``
 for tensors on the wrong device); what lies on the device (lengths, page numbers, token ids) is
-bounded by the kernels. ``status``, where a function takes it, is an int32 tensor of one element that
-receives the bit 2 if an index lay outside its range (that token or key was left out), and the bit 1 if
-a bounded wait of the kernels ran out (results are missing; attention's rows that lack keys are NaN).
+bounded by the kernels. An output of the caller's own may not share memory with what the call reads
+beside it (slices of one tensor will do where no element is in both), but for the two cases named below.
+``status``, where a function takes it, is an int32 tensor of one element that receives the bit 2 if an
+index lay outside its range (that token or key was left out), and the bit 1 if a bounded wait of the
+kernels ran out (results are missing; attention's rows that lack keys are NaN).
 """
 from __future__ import annotations
 
@@ -77,7 +79,7 @@ def linear_i8(x, weight, bias=None, out_dtype=None, x_scale=None, out=None, stat
 
     x: [tokens, in_feat], float32 / float16 / bfloat16, quantised on the way as by ``quantize_tokens``; or
     int8 codes with their ``x_scale`` [tokens]. y has ``out_dtype`` (x's own where not given; float32 for
-    codes)."""
+    codes). ``out`` may lie over a floating x."""
     if not isinstance(weight, I8Weight):
         raise InvalidArg("weight: not an I8Weight")
     return _n.linear_i8(x, weight.w, weight.scale, bias, out_dtype, x_scale, out, status)
