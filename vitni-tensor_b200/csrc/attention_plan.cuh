@@ -137,8 +137,8 @@ __device__ void build_plan(const AttnParams& p, int* base) {
   if (s_bad) {  // row starts that decrease: no sequence owns a row (the slots are counted for one owner a row)
     for (int b = tid; b <= B; b += blockDim.x) pl.q0[b] = 0;
     if (tid == 0 && p.a.status) atomicOr(p.a.status, SERVE_BAD_INDEX);
-    __syncthreads();
   }
+  __syncthreads();  // len[B], and the starts
   // Inclusive sums over runs of consecutive sequences, one run a thread.
   const int n = B + 1, per = (n + (int)blockDim.x - 1) / (int)blockDim.x, b0 = min(tid * per, n), b1 = min(b0 + per, n);
   int st = 0, ss = 0;
