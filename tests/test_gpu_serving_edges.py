@@ -3,7 +3,7 @@ the largest sums, weights far below a row's largest, scales of zero, outputs tha
 import pytest
 import torch
 
-from tests.test_gpu_serving import BF16, F32, attention_case, gen
+from tests.test_gpu_serving import BF16, F16, F32, attention64, attention_case, attention_close, gen
 from vtq import Internal
 
 pytestmark = pytest.mark.gpu
@@ -30,6 +30,26 @@ def test_linear_i8_the_largest_sum(S, t, n):
     q[:, 77] = 0
     y = S.linear_i8(q, W, x_scale=torch.ones(t, device="cuda"))
     assert torch.equal(y, ((code[:, None] * weight).double() * (k - 1)).float())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("seqs,shared,at", [(1, 0, 0), (30, 0, 0), (30, 0, 19990), (24, 20000, 0), (24, 20000, 19990)])
+def test_attention_weights_far_below_the_largest(S, dtype, dim, seqs, shared, at):
+    """One key takes nearly all of the weight, 20000 others e^-17 of it each (4e-8: less than the smallest normal
+    number of 16 bits), and its value is 0: the others are all that there is to see."""
+    length = 20000 + (shared > 0)
+    q, kp, vp, table, kv_len, start = attention_case(gen(dim), [1] * seqs, [length] * seqs, 8, 2, dim, 16, shared, dtype, False)
+    q.zero_(), kp.zero_()
+    q[..., 0] = 4
+    vp.uniform_(0.5, 1.5, generator=gen(1))
+    page = table[0, at // 16].long()
+    kp[page, at % 16, :, 0] = 4.25
+    vp[page, at % 16] = 0
+    out, lse = S.attention_paged(q, kp, vp, table, kv_len, shared_len=shared, scale=1.0, return_lse=True)
+    want, size, want_lse = attention64(q, kp, vp, table, [length] * seqs, [1] * seqs, shared, 1.0)
+    assert attention_close(out, want, size, dtype)
+    assert ((lse.double() - want_lse).abs() <= 2 ** -16 + 2 ** -20 * want_lse.abs()).all()
 
 
 def attention_inputs(tokens=6):

@@ -10,8 +10,8 @@
 //   2 loader warps      pages into a ring of swizzled K and V tiles, by TMA where a page holds 4 positions
 //                       or more (gathering rows with 16-byte copies took three warps 5700 cycles a tile)
 //   a warp a stream     one thread issues S = Q K^T (N = KT keys) and O += P V (V as it lies: N-major)
-// O stays in TMEM; it is scaled again only where a row's maximum has grown by more than 2^8 since the
-// last time, until then the weights are taken relative to the old one (at most 256, and l with them).
+// O stays in TMEM; it is scaled again only where a row's maximum has grown by more than 2^8 (f16: 2^4) since the
+// last time, until then the weights are taken relative to the old one (at most 256, and l with them; Weights).
 // Head dims over 128 have room in TMEM for one stream.
 #pragma once
 #include "attention_plan.cuh"
@@ -504,11 +504,12 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
         }
         top = low * p.scale_log2;
       }
+      top -= Weights<T>::tile_up;
       if (start) {
         m = top;
         l = 0.0f;
       } else {
-        const bool grow = top > m + 8.0f || (m == -INFINITY && top > -INFINITY);
+        const bool grow = top > m + Weights<T>::tile_grow || (m == -INFINITY && top > -INFINITY);
         if (__any_sync(0xffffffffu, grow)) {
           const float to = grow ? top : m;
           const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : exp2_fast(m - to);
@@ -555,7 +556,7 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
           e[j].y = exp2_fast(e[j].y);
           if (j & 1) sum1 = add2(sum1, e[j]);
           else sum0 = add2(sum0, e[j]);
-          w[j] = pack2<T>(e[j].x, e[j].y);
+          w[j] = Weights<T>::pack(e[j].x, e[j].y);
         }
 #pragma unroll
         for (int j = 0; j < HALF / 2; j += 16) tmem_st16(sp + c * (HALF / 2) + j, w + j);
