@@ -1,6 +1,6 @@
 // The cut of the attention's work (csrc/attention_plan.cuh) on the host, for test_attention_cut.py: every key of
-// every row block is some part's, once; parts that are lost at any tile still leave an entry for every segment; the
-// joining kernel follows no entry that is none. Prints what is wrong and ends with 1, or ends with 0.
+// every row block is some part's, once; every segment gets its entry, and the joining kernel follows no entry that is
+// none. Prints what is wrong and ends with 1, or ends with 0.
 #include <cstdio>
 #include <cstdlib>
 #include <random>
@@ -51,11 +51,11 @@ struct Cut {
   }
 };
 
-void check(const Cut& c, int parts, std::mt19937& rng) {
+void check(const Cut& c, int parts) {
   const int W = c.total < parts ? c.total : parts, B = c.B, H = c.H, segs = c.pl.segs[B + 1];
   const int stale = (int)0xcdcdcdcd;
   std::vector<std::vector<int>> seen(segs);  // how often each key of a segment is taken
-  std::vector<int2> entries(segs, make_int2(stale, stale)), lost(segs, make_int2(stale, stale));
+  std::vector<int2> entries(segs, make_int2(stale, stale));
   for (int w = 0; w < W; w++) {
     const int tile0 = first_tile(c.total, W, w), tile1 = first_tile(c.total, W, w + 1);
     WANT(tile0 < tile1);
@@ -69,40 +69,12 @@ void check(const Cut& c, int parts, std::mt19937& rng) {
       s.resize(at.end);
       for (int k = key0; k < key0 + c.p.tile; k++)
         if (k >= at.lo && k < at.end) s[k]++;
-      // The part's share of the segment ends here: as attention_part.cuh sees it, and as share_of does from any tile of it.
-      const bool ends = tile + 1 == tile1 || at.t + 1 == at.nt;
-      const Share sh = share_of(at, tile, tile0, tile1);
-      WANT(ends == (sh.end == tile + 1));
-      if (ends) {
-        WANT(sh.first == (tile - at.t >= tile0) && sh.last == (at.t + 1 == at.nt));
-        if (sh.first) entries[id].x = w;
-        if (sh.last) entries[id].y = w;
+      // The part's share of the segment ends here: its entry.
+      if (tile + 1 == tile1 || at.t + 1 == at.nt) {
+        if (tile - at.t >= tile0) entries[id].x = w;
+        if (at.t + 1 == at.nt) entries[id].y = w;
       }
       if (tile + 1 < tile1) advance(c.p, c.pl, B, at);
-    }
-    // Lost at some tile: the walk over what is left enters each segment that was not ended, and ends at tile1.
-    int tile = tile0 + (int)(rng() % (unsigned)(tile1 - tile0));
-    Cursor l = seek(c.p, c.pl, B, tile0);
-    for (int t = tile0; t < tile;) {  // what had been ended before
-      const Share sh = share_of(l, t, tile0, tile1);
-      if (sh.end > tile) break;
-      const int id = c.pl.segs[l.b] + l.mb * H + l.g;
-      if (sh.first) lost[id].x = w;
-      if (sh.last) lost[id].y = w;
-      t = sh.end;
-      l.t = l.nt - 1;
-      if (t < tile1) advance(c.p, c.pl, B, l);
-    }
-    l = seek(c.p, c.pl, B, tile);
-    while (true) {
-      const Share sh = share_of(l, tile, tile0, tile1);
-      const int id = c.pl.segs[l.b] + l.mb * H + l.g;
-      if (sh.first) lost[id].x = w;
-      if (sh.last) lost[id].y = w;
-      WANT(sh.end > tile && sh.end <= tile1);
-      if ((tile = sh.end) == tile1) break;
-      l.t = l.nt - 1;
-      advance(c.p, c.pl, B, l);
     }
   }
   for (int b = 0; b <= B; b++) {
@@ -114,7 +86,6 @@ void check(const Cut& c, int parts, std::mt19937& rng) {
       WANT((int)seen[id].size() == end);
       for (int k = 0; k < end; k++) WANT(seen[id][k] == (k >= lo));
       WANT(parts_ok(entries[id], W));
-      WANT(entries[id].x == lost[id].x && entries[id].y == lost[id].y);
     }
   }
   for (int t = 0; t < (int)c.p.a.tokens; t++) {
@@ -148,7 +119,7 @@ int main() {
     }
     for (bool on_tiles : {false, true}) {
       const Cut c(rows, lens, H, group, tile, keys_max, shared, on_tiles);
-      for (int parts : {1, 7, 8 * 148, 12 * 148}) check(c, parts, rng);
+      for (int parts : {1, 7, 8 * 148, 12 * 148}) check(c, parts);
     }
   }
   return 0;

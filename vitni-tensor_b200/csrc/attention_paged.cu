@@ -88,8 +88,7 @@ __global__ void __launch_bounds__(attention_threads<T, DP, RT>(), 1)
       return;
     }
   }
-  const int lost = part_role<T, DP, P::KT, P::WARPS, RT == 0>(p, tmk, tmv, smem, base, cta - x, p.ctas - x);
-  if (lost >= 0) lost_parts<T, DP, RT == 0>(p, base, lost);
+  part_role<T, DP, P::KT, P::WARPS, RT == 0>(p, tmk, tmv, smem, base, cta - x, p.ctas - x);
 }
 
 // Adds the parts of each row (query head of a token): p.join_warps warps a row, one where the rows fill the SMs, more

@@ -15,41 +15,6 @@
 namespace vtq {
 namespace {
 
-// A wait of a part ran out at `tile`: what it has not left yet, of its tiles [.., tile1), becomes NaN (its sums of
-// weights are). So the joining kernel finds an entry and a slot for each segment, and rows that lack keys show it.
-// Copies that this warp has on their way were asked for before the wait that ran out, 2 s ago.
-template <typename T, int DP, bool ALONE>
-__device__ __noinline__ void lost_parts(const AttnParams& p, int* base, int tile) {
-  const int B = (int)p.a.kv.seqs, H = (int)p.a.kv.kv_heads, D = (int)p.a.kv.head_dim, lane = threadIdx.x & 31;
-  const Plan pl = plan_of(base, B);
-  const int w = (int)(threadIdx.x >> 5) * (p.ctas - base[2]) + (int)blockIdx.x - base[2];
-  const int tile0 = first_tile(base[0], base[1], w), tile1 = first_tile(base[0], base[1], w + 1);
-  const float nan = __uint_as_float(0x7fc00000u);
-  Cursor c = seek(p, pl, B, tile);
-  while (true) {
-    const Share s = share_of(c, tile, tile0, tile1);
-    const int id = pl.segs[c.b] + c.mb * H + c.g;
-    const int rows_in = min(kRows, (c.b == B ? (int)p.a.tokens : seq_rows(pl, c.b)) * p.group - c.mb * kRows);
-    if (lane == 0) {
-      if (s.first) p.seg_parts[id].x = w;
-      if (s.last) p.seg_parts[id].y = w;
-    }
-    if (lane < rows_in) {
-      if (ALONE && s.first && s.last && c.b < B && !(pl.len[B] && sees_prefix(p, pl, c.b))) {
-        const int row = c.mb * kRows + lane, tok = p.by_group(row);
-        const int64_t token = pl.q0[c.b] + tok, head = c.g * p.group + row - tok * p.group;
-        for (int d = 0; d < D; d++) static_cast<T*>(p.a.out)[token * p.a.o_tok + head * p.a.o_head + d] = from_f32<T>(nan);
-        if (p.a.lse) p.a.lse[token * p.a.lse_tok + head] = nan;
-      } else {
-        *reinterpret_cast<float2*>(p.part + (int64_t)(w + id) * (kRows * (DP + 2)) + 2 * lane) = make_float2(0.0f, nan);
-      }
-    }
-    if ((tile = s.end) == tile1) return;
-    c.t = c.nt - 1;
-    advance(p, pl, B, c);
-  }
-}
-
 // DP: head_dim rounded up to what the MMA loop takes (64, 128, 256).
 template <typename T, int DP, int KT, int WARPS>
 struct PartShape {
@@ -58,9 +23,8 @@ struct PartShape {
 };
 
 // The role of CTA `cta` of `ctas`; ALONE: none works on the prefix's own tiles; `base` is the plan, at smem + STAGES_BYTES.
-// The tile at which a wait ran out, or -1.
 template <typename T, int DP, int KT, int WARPS, bool ALONE>
-__device__ __forceinline__ int part_role(const AttnParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, uint8_t* smem,
+__device__ __forceinline__ void part_role(const AttnParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, uint8_t* smem,
                                           int* base, int cta, int ctas) {
   using L = PartShape<T, DP, KT, WARPS>;
   constexpr int CH = DP / 8;  // 16-byte chunks of a row
@@ -70,12 +34,12 @@ __device__ __forceinline__ int part_role(const AttnParams& p, const CUtensorMap&
   // Where this tile and the next one stand, by turns: in shared memory, for the registers are all in use (a spill
   // costs the loop a quarter of its rate).
   __shared__ Cursor s_at[WARPS][2];
-  if (warp >= WARPS) return -1;
+  if (warp >= WARPS) return;
   longlong2* rows = reinterpret_cast<longlong2*>(reinterpret_cast<uint8_t*>(base) + (plan_ints(B) * 4 + 15) / 16 * 16) + warp * KT;
   const Plan pl = plan_of(base, B);
   const int total = base[0], W = base[1];
   const int w = warp * ctas + cta;  // few parts spread over the SMs first
-  if (w >= W) return -1;
+  if (w >= W) return;
   if (lane == 0) {
     for (int s = 0; s < 2; s++) tc5::bar_init(smem_u32(&s_full[warp][s]), 1);
     fence_mbar_init();
@@ -232,8 +196,11 @@ __device__ __forceinline__ int part_role(const AttnParams& p, const CUtensorMap&
       }
   };
   queries(at[0]);
-  int tile = tile0;
-  for (; tile < tile1; tile++) {
+  // A wait that ran out ends the loads, and what this part has not left yet becomes NaN (its sums of weights are): the
+  // joining kernel still finds an entry and a slot for each segment, and rows that lack keys show it. Copies on their
+  // way then were asked for before that wait, 2 s ago.
+  bool ok = true;
+  for (int tile = tile0; tile < tile1; tile++) {
     const int turn = (tile - tile0) & 1;
     const Cursor& c = at[turn];
     if (tile == tile0 || c.t == 0) {
@@ -259,7 +226,7 @@ __device__ __forceinline__ int part_role(const AttnParams& p, const CUtensorMap&
     }
     const uint32_t parity = (uint32_t)turn;
     const uint32_t valid = next.valid;
-    if (!landed(k_full, parity)) break;
+    ok = ok && landed(k_full, parity);
     const int key0 = (c.lo & -KT) + c.t * KT;
     float sc[KT / 8][4];
 #pragma unroll
@@ -280,7 +247,7 @@ __device__ __forceinline__ int part_role(const AttnParams& p, const CUtensorMap&
     __syncwarp();
     if (tile + 1 < tile1) {
       next = find(at[turn ^ 1], page);
-      load(next, at[turn ^ 1], false);
+      if (ok) load(next, at[turn ^ 1], false);
     } else {
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
@@ -328,7 +295,7 @@ __device__ __forceinline__ int part_role(const AttnParams& p, const CUtensorMap&
       pf[n >> 1][2 * (n & 1) + 1] = Weights<T>::pack(e2, e3);
     }
     if (tile + 1 < tile1 && at[turn ^ 1].t == 0) queries(at[turn ^ 1]);
-    if (!landed(v_full, parity)) break;
+    ok = ok && landed(v_full, parity);
     if (!whole) {
       // A weight of 0 times an infinity or a NaN is no 0: keys that are not there (what lies behind a sequence's end
       // in its last page, or was in the stage before) become zeros; values that only some rows must not see are
@@ -384,7 +351,7 @@ __device__ __forceinline__ int part_role(const AttnParams& p, const CUtensorMap&
         mma16<T>(o[2 * i + 1], pf[k], vf[2], vf[3]);
       }
     __syncwarp();
-    if (tile + 1 < tile1) load(next, at[turn ^ 1], true);
+    if (tile + 1 < tile1 && ok) load(next, at[turn ^ 1], true);
     else asm volatile("cp.async.commit_group;" ::: "memory");
     if (tile + 1 == tile1 || at[turn ^ 1].t == 0) {
       // The part's share of the segment ends here.
@@ -393,6 +360,7 @@ __device__ __forceinline__ int part_role(const AttnParams& p, const CUtensorMap&
         l0 += __shfl_xor_sync(0xffffffffu, l0, d);
         l1 += __shfl_xor_sync(0xffffffffu, l1, d);
       }
+      if (!ok) l0 = l1 = __uint_as_float(0x7fc00000u);
       const int id = pl.segs[c.b] + c.mb * H + c.g;
       const bool first = tile - c.t >= tile0, last = c.t + 1 == c.nt;  // of the segment's parts
       if (lane == 0) {
@@ -439,7 +407,6 @@ __device__ __forceinline__ int part_role(const AttnParams& p, const CUtensorMap&
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
-  return tile < tile1 ? tile : -1;
 }
 
 }  // namespace

@@ -214,8 +214,7 @@ __host__ __device__ __forceinline__ void enter(const AttnParams& p, const Plan& 
   c.end = c.b < B ? min(pl.len[c.b], p.keys_max) : pl.len[B];
 }
 
-// (Not inlined: one call a part, and its registers would cost the parts' loop spills.)
-__host__ __device__ __noinline__ Cursor seek(const AttnParams& p, const Plan& pl, int B, int tile) {
+__host__ __device__ __forceinline__ Cursor seek(const AttnParams& p, const Plan& pl, int B, int tile) {
   int lo = 0, hi = B;  // the last index whose tiles begin at or before `tile`
   while (lo < hi) {
     const int m = (lo + hi + 1) >> 1;
@@ -250,17 +249,6 @@ __host__ __device__ __forceinline__ void advance(const AttnParams& p, const Plan
 // The first and last of a segment's parts, as the joining kernel finds them: whether they are parts of `most`. It
 // follows no others.
 __host__ __device__ inline bool parts_ok(int2 w, int most) { return w.x >= 0 && w.x <= w.y && w.y < most; }
-
-// The part of a segment that a part of the work, tiles [tile0, tile1), takes: of the segment that `c` stands in, at
-// `tile`. Whether it takes the segment's first and last tile, and the tile behind what it takes.
-struct Share {
-  bool first, last;
-  int end;
-};
-__host__ __device__ inline Share share_of(const Cursor& c, int tile, int tile0, int tile1) {
-  const int start = tile - c.t, stop = start + c.nt;
-  return Share{start >= tile0, stop <= tile1, stop < tile1 ? stop : tile1};
-}
 
 // The sequence that owns a row of q, or -1.
 __host__ __device__ __forceinline__ int owner(const Plan& pl, int B, int token) {
