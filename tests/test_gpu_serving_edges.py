@@ -1,5 +1,7 @@
 """The batched serving operators on the GPU where their documentation allows a call that is easily got wrong:
 the largest sums, weights far below a row's largest, scales of zero, outputs that lie beside or over inputs."""
+import math
+
 import pytest
 import torch
 
@@ -50,6 +52,21 @@ def test_attention_weights_far_below_the_largest(S, dtype, dim, seqs, shared, at
     want, size, want_lse = attention64(q, kp, vp, table, [length] * seqs, [1] * seqs, shared, 1.0)
     assert attention_close(out, want, size, dtype)
     assert ((lse.double() - want_lse).abs() <= 2 ** -16 + 2 ** -20 * want_lse.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("seqs,shared", [(2, 0), (24, 3000)])
+def test_attention_of_scale_zero(S, dtype, seqs, shared):
+    """Every key weighs the same, however large the products are."""
+    length = shared + 70
+    q, kp, vp, table, kv_len, start = attention_case(gen(2), [1] * seqs, [length] * seqs, 8, 2, 64, 16, shared, dtype, False)
+    most = 1e18 if dtype == BF16 else 2e4
+    q *= most
+    kp *= most / kp.abs().max()
+    out, lse = S.attention_paged(q.clamp(-most, most), kp, vp, table, kv_len, shared_len=shared, scale=0.0, return_lse=True)
+    want, size, _ = attention64(torch.zeros_like(q), kp, vp, table, [length] * seqs, [1] * seqs, shared, 1.0)
+    assert attention_close(out, want, size, dtype)
+    assert ((lse.double() - math.log(length)).abs() <= 2 ** -16).all()
 
 
 def attention_inputs(tokens=6):

@@ -413,8 +413,9 @@ vtq_status vtq_attention_paged(const vtq_attention_args* a, void* ws, size_t ws_
   p.ctas = num_sms();
   p.keys_max = (int)(a->kv.table_width * a->kv.page_size);
   p.prefix = (int)std::min<int64_t>(a->shared_len, p.keys_max);
-  // A scale of 0 weighs every key alike: so does one that no product reaches.
-  p.scale_log2 = a->scale == 0.0f ? 1e-30f : a->scale * 1.4426950408889634f;
+  // A scale of 0 weighs every key alike; so does the smallest number, with which no finite score is above 2^-20 (and
+  // which leaves the -inf of masked keys what it is).
+  p.scale_log2 = a->scale == 0.0f ? 1.4e-45f : a->scale * 1.4426950408889634f;
   p.q_wide = (reinterpret_cast<uintptr_t>(a->q) & 3u) == 0 && a->q_tok % 2 == 0 && a->q_head % 2 == 0;
   p.o_wide = (reinterpret_cast<uintptr_t>(a->out) & 3u) == 0 && a->o_tok % 2 == 0 && a->o_head % 2 == 0;
   uint8_t* at = static_cast<uint8_t*>(ws);
