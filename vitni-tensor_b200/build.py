@@ -1,5 +1,6 @@
-"""Build the sm_100a shared library ``vtq/libvtq.so`` in-tree with nvcc, and the torch
-binding of the batched serving operators, ``vtq/_serving.so``, with the host compiler.
+"""Build the sm_100a shared library ``vtq/libvtq.so`` in-tree with nvcc, and, where torch and its
+headers are there, the torch binding of the batched serving operators, ``vtq/_serving.so``, with the
+host compiler (``vtq.serving`` says so where it is missing; the C library does not need it).
 
 Usage: python vitni-tensor_b200/build.py [--force]
 Every .cu under csrc/ is compiled for sm_100a only, with fp32 contraction
@@ -14,6 +15,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "vtq", "libvtq.so")
+BINDING = os.path.join(HERE, "vtq", "_serving.so")
 OBJ = os.path.join(HERE, "_build")
 
 NVCC_FLAGS = [
@@ -60,7 +62,7 @@ def build(force=False, verbose=False):
 
 def build_binding(force=False, verbose=False):
     """vtq/_serving.so from csrc/serving_bind.cpp, against this interpreter's torch and libvtq.so."""
-    src, out = os.path.join(CSRC, "serving_bind.cpp"), os.path.join(HERE, "vtq", "_serving.so")
+    src, out = os.path.join(CSRC, "serving_bind.cpp"), BINDING
     header = os.path.join(HERE, "..", "include", "vtq.h")
     if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(p) for p in (src, header)):
         return out
@@ -82,6 +84,19 @@ def build_binding(force=False, verbose=False):
     return out
 
 
+def main(args):
+    force = "--force" in args
+    lib = build(force=force, verbose=True)
+    try:
+        out = [lib, build_binding(force=force, verbose=True)]
+    except (ImportError, OSError, TypeError, subprocess.CalledProcessError) as e:
+        if os.path.exists(BINDING):
+            os.remove(BINDING)  # of an earlier build: it may not fit this library
+        print(f"{BINDING} is not built ({e}): vtq.serving needs torch, its headers and a host compiler", file=sys.stderr)
+        out = [lib]
+    print(*out, sep="\n")
+    return 0
+
+
 if __name__ == "__main__":
-    print(build(force="--force" in sys.argv, verbose=True))
-    print(build_binding(force="--force" in sys.argv, verbose=True))
+    sys.exit(main(sys.argv[1:]))
