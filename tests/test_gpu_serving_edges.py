@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests.test_gpu_serving import BF16, F16, F32, attention64, attention_case, attention_close, gen
-from vtq import Internal
+from vtq import Internal, NotImplementedOp
 
 pytestmark = pytest.mark.gpu
 
@@ -151,3 +151,31 @@ def test_outputs_over_what_is_read_beside_them(S):
     a, kp, vp, table, kv_len, _ = attention_inputs()
     with pytest.raises(Internal, match="share memory"):
         S.attention_paged(a, kp, vp, table, kv_len, out=torch.zeros(6, 400, dtype=BF16, device="cuda").as_strided(a.shape, (64, 64, 1)))
+
+
+def test_gradients_are_refused(S):
+    """None of the operators has a gradient: an input that asks for one is refused, unless gradients are off."""
+    q, kp, vp, table, kv_len, _ = attention_inputs(3)
+    x = torch.randn(3, 64, generator=gen(6), device="cuda")
+    W = S.I8Weight.quantize(torch.nn.Parameter(x))  # a conversion of weights: no gradient to lose
+    b = torch.zeros(3, device="cuda")
+    k = torch.randn(3, 2, 64, generator=gen(7), device="cuda").to(BF16)
+    seq, pos = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.arange(3, dtype=torch.int32, device="cuda")
+    p = torch.softmax(torch.randn(1, 2, 50, device="cuda"), -1)
+    draft, u = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.zeros(1, 2, device="cuda")
+    ask = lambda t: t.clone().requires_grad_()  # noqa: E731
+    calls = [
+        lambda f: S.linear_i8(f(x), W), lambda f: S.linear_i8(x, W, bias=f(b)),
+        lambda f: S.append_kv(f(k), k, kp, vp, table, seq, pos), lambda f: S.append_kv(k, f(k), kp, vp, table, seq, pos),
+        lambda f: S.append_kv(k, k, kp, vp, table, seq, pos, q=f(q)),
+        lambda f: S.attention_paged(f(q), kp, vp, table, kv_len), lambda f: S.attention_paged(q, f(kp), vp, table, kv_len),
+        lambda f: S.attention_paged(q, kp, f(vp), table, kv_len), lambda f: S.attention_paged(q, kp, vp, table, kv_len, out=f(q))]
+    for call in calls:
+        with pytest.raises(NotImplementedOp, match="gradient"):
+            call(ask)
+        call(lambda t: t.clone())
+        with torch.no_grad():
+            call(ask)
+        with torch.inference_mode():
+            call(lambda t: t.clone())
+    S.verify_draft(draft, ask(p), None, u)  # whole numbers: nothing to differentiate

@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/full.h>
 #include <ATen/ops/zeros.h>
@@ -74,6 +75,13 @@ const at::Tensor& want(const char* name, PyObject* o, int64_t dim, Types types, 
   return t;
 }
 
+// The operators have no gradient: an input that asks for one would silently lose it.
+const at::Tensor& constant(const char* name, const at::Tensor& t) {
+  if (t.requires_grad() && at::GradMode::is_enabled())
+    refuse(VTQ_ERR_NOT_IMPLEMENTED, name, ": not implemented (its gradient; call under torch.no_grad())");
+  return t;
+}
+
 // Where a tensor's elements lie, in bytes; dimensions of one element left out.
 struct Span {
   uintptr_t base;
@@ -112,6 +120,7 @@ bool may_share(const Span& a, const Span& b) {
 
 // An output: its elements must not share memory. Each step has to pass what all smaller ones reach over.
 const at::Tensor& distinct(const char* name, const at::Tensor& t) {
+  constant(name, t);
   if (!t.numel()) return t;
   Span a(t);
   std::sort(a.dims.begin(), a.dims.end());
@@ -212,6 +221,7 @@ PyObject* linear_i8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const at::Tensor& ws = want("w_scale", a[2], 1, {ScalarType::Float}, &dev, {n});
     const bool codes = given(a[5]);
     const at::Tensor& x = codes ? want("x", a[0], 2, {ScalarType::Char}, &dev, {-1, in}) : want("x", a[0], 2, kFloats, &dev, {-1, in});
+    constant("x", x);
     const c10::cuda::CUDAGuard guard(dev);
     const int64_t t = x.size(0);
     ScalarType type = codes ? ScalarType::Float : x.scalar_type();
@@ -234,10 +244,10 @@ PyObject* linear_i8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
       return ptr(r);
     };
     g.x = codes ? read("x", x) : ptr(x);
-    if (codes) g.x_scale = static_cast<const float*>(read("x_scale", want("x_scale", a[5], 1, {ScalarType::Float}, &dev, {t})));
+    if (codes) g.x_scale = static_cast<const float*>(read("x_scale", constant("x_scale", want("x_scale", a[5], 1, {ScalarType::Float}, &dev, {t}))));
     g.w = static_cast<const int8_t*>(read("w", w));
-    g.w_scale = static_cast<const float*>(read("w_scale", ws));
-    if (given(a[3])) g.bias = static_cast<const float*>(read("bias", want("bias", a[3], 1, {ScalarType::Float}, &dev, {n})));
+    g.w_scale = static_cast<const float*>(read("w_scale", constant("w_scale", ws)));
+    if (given(a[3])) g.bias = static_cast<const float*>(read("bias", constant("bias", want("bias", a[3], 1, {ScalarType::Float}, &dev, {n}))));
     g.y = ptr(out);
     g.ldx = x.stride(0);
     g.ldw = w.stride(0);
@@ -261,6 +271,7 @@ vtq_paged_kv paged(PyObject* k_pages, PyObject* v_pages, PyObject* table, at::De
   dev = k.device();
   const at::Tensor& v = want("v_pages", v_pages, 4, {k.scalar_type()}, &dev, {k.size(0), k.size(1), k.size(2), k.size(3)});
   const at::Tensor& t = want("page_table", table, 2, kInt, &dev);
+  constant("k_pages", k), constant("v_pages", v);
   vtq_paged_kv kv = {};
   kv.k = ptr(k);
   kv.v = ptr(v);
@@ -289,6 +300,7 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const at::Tensor& k = want("k", a[0], 3, kFloats, &dev, {-1, g.kv.kv_heads, g.kv.head_dim});
     const int64_t t = k.size(0);
     const at::Tensor& v = want("v", a[1], 3, {k.scalar_type()}, &dev, {t, g.kv.kv_heads, g.kv.head_dim});
+    constant("k", k), constant("v", v);
     g.k = ptr(k), g.k_tok = k.stride(0), g.k_head = k.stride(1);
     g.v = ptr(v), g.v_tok = v.stride(0), g.v_head = v.stride(1);
     g.seq = static_cast<const int32_t*>(ptr(want("seq", a[5], 1, kInt, &dev, {t})));
@@ -303,7 +315,7 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     }
     at::Tensor out;
     if (given(a[9])) {
-      const at::Tensor& q = want("q", a[9], 3, {k.scalar_type()}, &dev, {t, -1, g.kv.head_dim});
+      const at::Tensor& q = constant("q", want("q", a[9], 3, {k.scalar_type()}, &dev, {t, -1, g.kv.head_dim}));
       const ScalarType c = THPVariable_Unpack(a[2]).scalar_type();
       out = given(a[10]) ? distinct("q_out", want("q_out", a[10], 3, {c}, &dev, {t, q.size(1), g.kv.head_dim}))
                          : at::zeros(q.sizes(), q.options().dtype(c));
@@ -337,7 +349,7 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     g.kv = paged(a[1], a[2], a[3], dev);
     const c10::cuda::CUDAGuard guard(dev);
     const ScalarType type = THPVariable_Unpack(a[1]).scalar_type();
-    const at::Tensor& q = want("q", a[0], 3, {type}, &dev, {-1, -1, g.kv.head_dim});
+    const at::Tensor& q = constant("q", want("q", a[0], 3, {type}, &dev, {-1, -1, g.kv.head_dim}));
     const int64_t t = q.size(0), heads = q.size(1);
     g.kv_len = static_cast<const int32_t*>(ptr(want("kv_len", a[4], 1, kInt, &dev, {g.kv.seqs})));
     const bool starts = given(a[5]);

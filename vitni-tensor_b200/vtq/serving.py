@@ -20,6 +20,10 @@ beside it (slices of one tensor will do where no element is in both), but for th
 ``status``, where a function takes it, is an int32 tensor of one element that receives the bit 2 if an
 index lay outside its range (that token or key was left out), and the bit 1 if a bounded wait of the
 kernels ran out (results are missing; attention's rows that lack keys are NaN).
+
+None of them has a gradient. Where gradients are on, an input that asks for one is refused
+(``NotImplementedOp``) by the linears, the append and the attention; codes of weights and tokens, and
+the verification's tokens, are whole numbers and made all the same.
 """
 from __future__ import annotations
 
