@@ -179,3 +179,27 @@ def test_gradients_are_refused(S):
         with torch.inference_mode():
             call(lambda t: t.clone())
     S.verify_draft(draft, ask(p), None, u)  # whole numbers: nothing to differentiate
+
+
+def test_written_tensors_say_so(S):
+    """What an operator writes into a tensor of the caller's raises its version, as torch's own in-place operations do."""
+    q, kp, vp, table, kv_len, _ = attention_inputs(3)
+    x = torch.randn(3, 64, generator=gen(6), device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    codes, scale, y = torch.empty(3, 64, dtype=torch.int8, device="cuda"), torch.empty(3, device="cuda"), torch.empty(3, 3, device="cuda")
+    k = torch.randn(3, 2, 64, generator=gen(7), device="cuda").to(BF16)
+    seq, pos = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.arange(3, dtype=torch.int32, device="cuda")
+    q_out, out = torch.empty_like(q), torch.empty_like(q)
+    W = S.I8Weight.quantize(x)
+    for call, written, read in (
+            (lambda: S.quantize_tokens(x, q=codes, scale=scale), [codes, scale], [x]),
+            (lambda: S.linear_i8(x, W, out=y, status=status), [y, status], [x, W.w, W.scale]),
+            (lambda: S.append_kv(k, k, kp, vp, table, seq, pos, q=q, q_out=q_out, status=status), [kp, vp, q_out, status], [k, q, table]),
+            (lambda: S.attention_paged(q, kp, vp, table, kv_len, out=out, status=status), [out, status], [q, kp, vp, table])):
+        was = [t._version for t in written], [t._version for t in read]
+        call()
+        assert all(t._version > v for t, v in zip(written, was[0]))
+        assert [t._version for t in read] == was[1]
+    with torch.inference_mode():
+        free = torch.empty_like(q)
+    assert torch.equal(S.attention_paged(q, kp, vp, table, kv_len, out=free), out)

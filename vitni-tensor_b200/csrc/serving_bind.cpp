@@ -140,6 +140,14 @@ void apart(const char* name, const at::Tensor& t, const char* in_name, const at:
   if (may_share(a, b)) refuse(VTQ_ERR_INTERNAL, name, ": shares memory with ", in_name);
 }
 
+// What a call wrote into a tensor of the caller's raises its version, as torch's own in-place operations do.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void written(PyObject* o) {
+  if (given(o)) written(THPVariable_Unpack(o));
+}
+
 void* ptr(const at::Tensor& t) { return t.data_ptr(); }
 
 uint32_t* status_of(PyObject* o, const at::Device& dev) {
@@ -207,6 +215,7 @@ PyObject* quantize_tokens(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const int64_t ldq = t > 1 ? q.stride(0) : std::max(n, q.stride(0));
     check(vtq_quantize_tokens(tag(x.scalar_type()), ptr(x), x.stride(0), t, n, static_cast<int8_t*>(ptr(q)), ldq,
                               static_cast<float*>(ptr(s)), stream_of(dev)));
+    written(a[1]), written(a[2]);
     return pair(q, s);
   });
 }
@@ -262,6 +271,7 @@ PyObject* linear_i8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     at::Tensor s;
     if (need) s = scratch(need, dev);
     check(vtq_linear_i8(&g, need ? ptr(s) : nullptr, need, stream_of(dev)));
+    written(a[6]), written(a[7]);
     return wrap(out);
   });
 }
@@ -335,6 +345,7 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     g.x_dtype = tag(k.scalar_type());
     g.status = status_of(a[11], dev);
     check(vtq_append_kv(&g, stream_of(dev)));
+    written(a[2]), written(a[3]), written(a[10]), written(a[11]);
     if (!out.defined()) Py_RETURN_NONE;
     return wrap(out);
   });
@@ -384,6 +395,7 @@ PyObject* attention_paged(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     at::Tensor s;
     if (need) s = scratch(need, dev);
     check(vtq_attention_paged(&g, need ? ptr(s) : nullptr, need, stream_of(dev)));
+    written(a[8]), written(a[10]);
     return lse.defined() ? pair(out, lse) : wrap(out);
   });
 }
