@@ -82,17 +82,23 @@ const at::Tensor& constant(const char* name, const at::Tensor& t) {
   return t;
 }
 
+// From a tensor's first element's first byte to the last one's end.
+int64_t extent(const at::Tensor& t) {
+  const auto size = t.sizes(), stride = t.strides();
+  int64_t n = 1;
+  for (size_t i = 0; i < size.size(); i++) n += (size[i] - 1) * stride[i];
+  return n * (int64_t)t.element_size();
+}
+
 // Where a tensor's elements lie, in bytes; dimensions of one element left out.
 struct Span {
   uintptr_t base;
-  int64_t elt, extent;  // extent: from the first element's first byte to the last one's end
+  int64_t elt;
   c10::SmallVector<std::pair<int64_t, int64_t>, 6> dims;  // (step, size)
-  explicit Span(const at::Tensor& t) : base(reinterpret_cast<uintptr_t>(t.data_ptr())), elt((int64_t)t.element_size()), extent(elt) {
-    for (int64_t i = 0; i < t.dim(); i++)
-      if (t.size(i) > 1) {
-        dims.emplace_back(t.stride(i) * elt, t.size(i));
-        extent += (t.size(i) - 1) * t.stride(i) * elt;
-      }
+  explicit Span(const at::Tensor& t) : base(reinterpret_cast<uintptr_t>(t.data_ptr())), elt((int64_t)t.element_size()) {
+    const auto size = t.sizes(), stride = t.strides();
+    for (size_t i = 0; i < size.size(); i++)
+      if (size[i] > 1) dims.emplace_back(stride[i] * elt, size[i]);
   }
   // The bytes that its elements reach over when those of all steps that are multiples of `period` are laid upon another.
   int64_t within(int64_t period) const {
@@ -103,11 +109,10 @@ struct Span {
   }
 };
 
-// Whether two tensors may have memory in common: no where one ends before the other begins, and no where they are
-// slices of one layout, that is, for some step of theirs, lie in different places of each period of that step (the
-// heads, values or tokens of one fused tensor).
+// Whether two tensors whose extents overlap may have memory in common: no where they are slices of one layout, that is,
+// for some step of theirs, lie in different places of each period of that step (the heads, values or tokens of one
+// fused tensor).
 bool may_share(const Span& a, const Span& b) {
-  if (a.base + a.extent <= b.base || b.base + b.extent <= a.base) return false;
   for (const Span* s : {&a, &b})
     for (const auto& dim : s->dims) {
       const int64_t period = dim.first;
@@ -121,7 +126,7 @@ bool may_share(const Span& a, const Span& b) {
 // An output: its elements must not share memory. Each step has to pass what all smaller ones reach over.
 const at::Tensor& distinct(const char* name, const at::Tensor& t) {
   constant(name, t);
-  if (!t.numel()) return t;
+  if (t.is_non_overlapping_and_dense() || !t.numel()) return t;
   Span a(t);
   std::sort(a.dims.begin(), a.dims.end());
   int64_t reach = a.elt;
@@ -135,6 +140,8 @@ const at::Tensor& distinct(const char* name, const at::Tensor& t) {
 // An output that is written while `in` is still being read; `same`: unless it is all of it, element for element.
 void apart(const char* name, const at::Tensor& t, const char* in_name, const at::Tensor& in, bool same = false) {
   if (!t.numel() || !in.numel()) return;
+  const uintptr_t t0 = reinterpret_cast<uintptr_t>(t.data_ptr()), in0 = reinterpret_cast<uintptr_t>(in.data_ptr());
+  if (t0 + extent(t) <= in0 || in0 + extent(in) <= t0) return;
   const Span a(t), b(in);
   if (same && a.base == b.base && a.dims == b.dims && t.scalar_type() == in.scalar_type()) return;
   if (may_share(a, b)) refuse(VTQ_ERR_INTERNAL, name, ": shares memory with ", in_name);
