@@ -203,3 +203,25 @@ def test_written_tensors_say_so(S):
     with torch.inference_mode():
         free = torch.empty_like(q)
     assert torch.equal(S.attention_paged(q, kp, vp, table, kv_len, out=free), out)
+
+
+@pytest.mark.parametrize("seqs,shared", [(3, 0), (40, 700)])
+def test_caches_and_tables_without_pages(S, seqs, shared):
+    """Every entry of the table is a page that does not exist: no key, zeros, and the status says so; a table without
+    entries has no position at all."""
+    q = torch.randn(seqs, 8, 64, generator=gen(1), device="cuda").to(F16)
+    none = torch.empty(0, 16, 2, 64, dtype=F16, device="cuda")
+    some = torch.full((2, 16, 2, 64), math.nan, dtype=F16, device="cuda")
+    length = torch.full((seqs,), shared + 9, dtype=torch.int32, device="cuda")
+    pos = torch.arange(seqs, dtype=torch.int32, device="cuda")
+    for pages, width in ((none, 50), (some, 0), (none, 0)):
+        table = torch.full((seqs, width), 2, dtype=torch.int32, device="cuda")
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out, lse = S.attention_paged(q, pages, pages, table, length, shared_len=shared, return_lse=True, status=status)
+        assert (out == 0).all() and torch.isneginf(lse).all() and status.item() == 2
+        status.zero_()
+        other = pages.clone()
+        S.append_kv(q[:, :2], q[:, :2], pages, other, table, pos, pos, status=status)
+        assert status.item() == 2 and (len(pages) == 0 or torch.isnan(pages).all())
+        S.attention_paged(q, pages, pages, table, torch.zeros_like(length), shared_len=shared, status=status.zero_())
+        assert status.item() == 0
