@@ -3,7 +3,8 @@
 //
 //   (a, b) -> (a cos - b sin, a sin + b cos),  cos / sin of pos * frequency from a 32-bit table
 //
-// Bound: HBM by bytes (each input read once, each output written once), latency for a decode step. A
+// Bound: HBM by bytes (each input read once, each output written once), latency for a decode step; as it is, issue slots
+// (65 % filled, 100 instructions a unit of four f32 values, cos and sin loaded for every head) come before HBM. A
 // thread takes a unit: 16 bytes of neighbouring values (and, where the pairs are (i, i + rot / 2), the 16
 // bytes of their partners), so that a warp's loads and stores are whole lines: two neighbouring 16-byte
 // pieces a thread instead keep L1 half busy with the same sectors twice.

@@ -17,10 +17,13 @@
 // (together about 48 bits), everything above a lane is in 64 bits, in an order
 // that V and the cluster size alone decide: plain 32-bit sums move the cut
 // between two tokens by about 1e-7 of the total, which over 1e5 tokens is a
-// different token once in some hundred draws. 128 x 8 rows of 100003 in f32:
-// 27 us (3.9 TB/s: the error sums take instructions, the ends of the pass
-// latency). Greedy, 64 x 8 rows of 32000 in f32,
-// 16 bytes a load: 17 us (3.9 TB/s; 23 with single values).
+// different token once in some hundred draws. 128 x 8 rows of 100003 in f32,
+// two thirds of the sequences with a rejection: 27 us for 85 MB (3.2 TB/s,
+// floor 13 us: the error sums take instructions, the ends of the pass latency).
+// Greedy, 64 x 8 rows of 32000 in f32, 3.2 rows a sequence needed (26 MB, 4 us):
+// 16 us for the 34 MB that groups of four rows read, 23 with single values a
+// load. Not HBM bounds it but two groups in a chain, each its load, its
+// reduction and a cluster barrier.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -16,7 +16,8 @@ the device. Arguments are checked on the host and refused with the package's err
 shapes and layouts, ``NotImplementedOp`` for types and sizes the kernels do not take, ``InvalidArg``
 for tensors on the wrong device); what lies on the device (lengths, page numbers, token ids) is
 bounded by the kernels. An output of the caller's own may not share memory with what the call reads
-beside it (slices of one tensor will do where no element is in both), but for the two cases named below.
+beside it (slices of one tensor will do where they lie in different places of a common step, such as heads of a
+fused projection), but for the two cases named below.
 ``status``, where a function takes it, is an int32 tensor of one element that receives the bit 2 if an
 index lay outside its range (that token or key was left out), and the bit 1 if a bounded wait of the
 kernels ran out (results are missing; attention's rows that lack keys are NaN).
