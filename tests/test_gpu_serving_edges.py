@@ -225,3 +225,22 @@ def test_caches_and_tables_without_pages(S, seqs, shared):
         assert status.item() == 2 and (len(pages) == 0 or torch.isnan(pages).all())
         S.attention_paged(q, pages, pages, table, torch.zeros_like(length), shared_len=shared, status=status.zero_())
         assert status.item() == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("scale", [1.0, -1.0, 0.04])
+@pytest.mark.parametrize("seqs,shared", [(3, 0), (24, 3000)])
+def test_attention_one_key_far_above_all(S, dtype, dim, scale, seqs, shared):
+    """Scores of up to 2^28 (in units of log 2: 1700 x 1536 x 64 / ln 2), which 32 bits round to multiples of 16: the largest key's
+    weight is what the sum holds of it, rounded once to the type, and its value comes out."""
+    length = shared + 70
+    q, kp, vp, table, kv_len, start = attention_case(gen(3), [1] * seqs, [length] * seqs, 8, 2, dim, 16, shared, dtype, False)
+    q.copy_((torch.randint(500, 850, (seqs, 8, 1), generator=gen(4), device="cuda") * 2 * 64 / dim).expand_as(q))
+    kp.fill_(math.copysign(1000, scale))
+    at = length // 2  # in the prefix, or of each sequence's own
+    for b in range(seqs):
+        kp[table[b, at // 16].long(), at % 16] = math.copysign(1536, scale)
+    rows = vp[table[:, at // 16].long(), at % 16].repeat_interleave(4, 1).double()
+    out = S.attention_paged(q, kp, vp, table, kv_len, shared_len=shared, scale=scale)
+    assert attention_close(out, rows, rows.abs(), dtype)

@@ -273,7 +273,7 @@ __device__ __forceinline__ void part_role(const AttnParams& p, const CUtensorMap
       x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
       x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
     }
-    const float n0 = fmaxf(m0, fmaf(x0, scale, -Weights<T>::up)), n1 = fmaxf(m1, fmaf(x1, scale, -Weights<T>::up));
+    const float n0 = fmaxf(m0, Weights<T>::base(x0, scale, Weights<T>::up)), n1 = fmaxf(m1, Weights<T>::base(x1, scale, Weights<T>::up));
     const float u0 = n0 == -INFINITY ? 0.0f : n0, u1 = n1 == -INFINITY ? 0.0f : n1;
     if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
       const float f0 = exp2_fast(m0 - u0), f1 = exp2_fast(m1 - u1);
@@ -291,8 +291,8 @@ __device__ __forceinline__ void part_role(const AttnParams& p, const CUtensorMap
       l1 += e2 + e3;
       // The weights are rounded to the cache's type for the second product: relative to each
       // weight (Weights), so a row's error stays that of its type, as the rounding of v itself.
-      pf[n >> 1][2 * (n & 1)] = Weights<T>::pack(e0, e1);
-      pf[n >> 1][2 * (n & 1) + 1] = Weights<T>::pack(e2, e3);
+      pf[n >> 1][2 * (n & 1)] = pack2<T>(e0, e1);
+      pf[n >> 1][2 * (n & 1) + 1] = pack2<T>(e2, e3);
     }
     if (tile + 1 < tile1 && at[turn ^ 1].t == 0) queries(at[turn ^ 1]);
     ok = ok && landed(v_full, parity);

@@ -311,19 +311,14 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // each came out 44 % too heavy). So they are taken 2^up larger: relative to a maximum that is lower by `up`. The
 // parts' running maximum is exact, their largest weight 2^15 of f16's 2^16; the tiles' may be 2^grow old. Weights down
 // to 2^-29 (2^-25 .. 2^-29 in the tiles) of the largest keep f16's precision, smaller ones are off by 2^-40 (2^-36) of it.
+// What f16's weights are relative to is rounded up, so that none leaves the type however coarse 32 bits are there.
 template <typename T>
 struct Weights {
   static constexpr bool kHalf = std::is_same<T, __half>::value;
   static constexpr float up = kHalf ? 15.0f : 0.0f, tile_up = kHalf ? 11.0f : 0.0f, tile_grow = kHalf ? 4.0f : 8.0f;
-  // Scores of 2^25 and more are rounded by whole units, and weights may leave the type: the largest number then.
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    if constexpr (kHalf) {
-      uint32_t r;
-      asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-      return r;
-    } else {
-      return pack2<T>(lo, hi);
-    }
+  // Of the largest product `x`, what its weights are relative to.
+  static __device__ __forceinline__ float base(float x, float scale, float lower) {
+    return kHalf ? __fmaf_ru(x, scale, -lower) : x * scale;
   }
 };
 template <typename T>

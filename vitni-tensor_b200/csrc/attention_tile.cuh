@@ -490,7 +490,7 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
             t1 = fmaxf(fmaxf(x[j + 2], x[j + 3]), t1);
           }
         }
-        top = fmaxf(t0, t1) * p.scale_log2;
+        top = Weights<T>::base(fmaxf(t0, t1), p.scale_log2, Weights<T>::tile_up);
       }
       if (p.scale_log2 < 0.0f) {  // the largest score is that of the smallest product
         float low = INFINITY;
@@ -502,14 +502,13 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
 #pragma unroll
           for (int j = 0; j < 32; j++) low = fminf(low, z[j]);
         }
-        top = low * p.scale_log2;
+        top = Weights<T>::base(low, p.scale_log2, Weights<T>::tile_up);
       }
-      top -= Weights<T>::tile_up;
       if (start) {
         m = top;
         l = 0.0f;
       } else {
-        const bool grow = top > m + Weights<T>::tile_grow || (m == -INFINITY && top > -INFINITY);
+        const bool grow = top - m > Weights<T>::tile_grow;  // (both -inf: not; m alone: it is)
         if (__any_sync(0xffffffffu, grow)) {
           const float to = grow ? top : m;
           const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : exp2_fast(m - to);
@@ -556,7 +555,7 @@ __device__ __forceinline__ void tile_role(const AttnParams& p, const CUtensorMap
           e[j].y = exp2_fast(e[j].y);
           if (j & 1) sum1 = add2(sum1, e[j]);
           else sum0 = add2(sum0, e[j]);
-          w[j] = Weights<T>::pack(e[j].x, e[j].y);
+          w[j] = pack2<T>(e[j].x, e[j].y);
         }
 #pragma unroll
         for (int j = 0; j < HALF / 2; j += 16) tmem_st16(sp + c * (HALF / 2) + j, w + j);
