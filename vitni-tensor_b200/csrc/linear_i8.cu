@@ -351,10 +351,10 @@ __global__ void __launch_bounds__(kThreads)
 // Many tokens: persistent pairs of CTAs (cta_group::2), each walking tiles of 256 channels x 256 tokens. A
 // CTA brings 128 channels and 128 tokens, 32 KB for 2^22 products: at the 62 bytes a cycle that L2 gives an
 // SM here this feeds the tensor cores, where a CTA by itself (128 x 256, 48 KB) waits: 101 us against 92 on
-// 2048 x 4096 x 14336 in runs of some ms, the codes' kernel of 9 us included (this form now: 94, and 109 in runs of
-// 0.15 s, when the power limit has lowered the clock). The leader (rank 0) issues the products for both; barriers that only it waits for are
-// its own, signalled from the peer. Two accumulators of 256 columns in TMEM, so that one tile is stored while
-// the next one is summed; the operand ring runs on across tiles.
+// 2048 x 4096 x 14336 in runs of some ms, the codes' kernel of 9 us included (94 as it is now, and 109 in runs
+// of 0.15 s, when the power limit has lowered the clock). The leader (rank 0) issues the products for both;
+// barriers that only it waits for are its own, signalled from the peer. Two accumulators of 256 columns in TMEM,
+// so that one tile is stored while the next one is summed; the operand ring runs on across tiles.
 constexpr int PM = 256, PN = 256, kPStages = 6, kPEpiWarps = 8, kPThreads = 64 + 32 * kPEpiWarps;
 constexpr uint32_t kPHalf = 128 * 128, kPStage = 2 * kPHalf;
 

@@ -144,7 +144,7 @@ def append_kv(k, v, k_pages, v_pages, page_table, seq, pos, rope=None, q=None, q
     k_pages, v_pages: [pages, page_size, kv_heads, head_dim], float16 / bfloat16 (a permuted view of another
     order will do). page_table: int32 [sequences, width], the page of each run of page_size positions. seq,
     pos: int32 [tokens]; a token of seq < 0 is padding: its rows of q_out, and the cache, are left alone.
-    q_out may be q itself where the types are the same. Two tokens of a call with the same sequence and
+    q_out may be q itself where the types are the same; k_pages and v_pages lie apart. Two tokens of a call with the same sequence and
     position: which one stays is not defined."""
     table = half = None
     if rope is not None:
